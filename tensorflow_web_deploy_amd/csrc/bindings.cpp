@@ -298,6 +298,145 @@ void attn_fused_bf16(torch::Tensor Q, torch::Tensor K, torch::Tensor V,
                          cur_stream());
 }
 
+// ---- fp8 dense layers. Types and shapes are looked at before the device,
+// so that a wrong call is named wherever it is made.
+
+constexpr auto kFp8 = c10::ScalarType::Float8_e4m3fn;
+
+void check_type(const torch::Tensor& t, c10::ScalarType type,
+                const char* name) {
+  TORCH_CHECK(t.scalar_type() == type, name, " must be ", type, ", got ",
+              t.scalar_type());
+}
+
+void check_shape(const torch::Tensor& t, c10::IntArrayRef shape,
+                 const char* name) {
+  TORCH_CHECK(t.sizes() == shape, name, " must be ", shape, ", got ",
+              t.sizes());
+}
+
+void check_whole(const torch::Tensor& t, c10::ScalarType type,
+                 c10::IntArrayRef shape, const char* name) {
+  check_type(t, type, name);
+  check_shape(t, shape, name);
+  TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
+}
+
+// rows of contiguous values that may lie apart, but not over each other
+void check_rows(const torch::Tensor& t, const char* name) {
+  TORCH_CHECK(t.dim() == 2, name, " must be 2D");
+  TORCH_CHECK(t.size(1) <= 1 || t.stride(1) == 1, name,
+              " must have contiguous rows");
+  TORCH_CHECK(t.size(0) <= 1 || t.stride(0) >= t.size(1), name,
+              " must have rows that don't overlap");
+}
+
+int64_t row_stride(const torch::Tensor& t) {
+  return t.size(0) <= 1 ? t.size(1) : t.stride(0);
+}
+
+void check_bf16_or_f32(const torch::Tensor& t, const char* name) {
+  TORCH_CHECK(t.scalar_type() == torch::kBFloat16 ||
+                  t.scalar_type() == torch::kFloat32,
+              name, " must be bf16 or f32, got ", t.scalar_type());
+}
+
+void check_act(int64_t act) {
+  TORCH_CHECK(act == 0 || act == 1 || act == 2 || act == 5,
+              "act must be 0 (none), 1 (relu), 2 (relu6) or 5 (gelu), got ",
+              act);
+}
+
+// all of them on one GPU, which the launches then go to
+void check_devices(c10::ArrayRef<std::pair<const torch::Tensor*, const char*>>
+                       tensors) {
+  const torch::Tensor& first = *tensors[0].first;
+  for (auto& [t, name] : tensors) {
+    TORCH_CHECK(t->is_cuda(), name, " must be on GPU");
+    TORCH_CHECK(t->device() == first.device(), name, " is on ", t->device(),
+                ", ", tensors[0].second, " on ", first.device());
+  }
+}
+
+int64_t blocks128(int64_t n) { return (n + 127) / 128; }
+
+// X [M,K] bf16|f32 -> Q [M,Kp] e4m3, Kp = K up to whole blocks of 128 (the
+// rest 0), and the scales: block_rows 1 (activations): S [Kp/128, M], one for
+// each row and 128 of K; block_rows 128 (weights): S [ceil(M/128), Kp/128]
+void quant_fp8(torch::Tensor X, torch::Tensor Q, torch::Tensor S,
+               int64_t block_rows) {
+  check_bf16_or_f32(X, "X");
+  check_rows(X, "X");
+  TORCH_CHECK(block_rows == 1 || block_rows == 128,
+              "block_rows must be 1 or 128, got ", block_rows);
+  const int64_t M = X.size(0), K = X.size(1), Kb = blocks128(K);
+  TORCH_CHECK(K >= 1 && K <= 1 << 22, "K must be 1 to 2^22, got ", K);
+  TORCH_CHECK(M < 1 << 30 && blocks128(M) * Kb < 1 << 30,
+              "X is too large: ", X.sizes());
+  check_whole(Q, kFp8, {M, Kb * 128}, "Q");
+  if (block_rows == 1)
+    check_whole(S, torch::kFloat32, {Kb, M}, "S");
+  else
+    check_whole(S, torch::kFloat32, {blocks128(M), Kb}, "S");
+  check_devices({{&X, "X"}, {&Q, "Q"}, {&S, "S"}});
+  if (M == 0) return;
+  const c10::DeviceGuard guard(X.device());
+  launch_quant_fp8(X.data_ptr(), X.scalar_type() == torch::kFloat32,
+                   row_stride(X), M, (int)K, Q.data_ptr(), (int)Kb * 128,
+                   S.data_ptr<float>(), (int)block_rows, cur_stream());
+}
+
+// C[M][N] = act(A @ B^T + bias + residual), C bf16. A [M,Kp] with SA
+// [Kp/128, M], B [N,Kp] with SB [ceil(N/128), Kp/128]: as quant_fp8
+// leaves them with block_rows 1 and 128
+void gemm_fp8(torch::Tensor A, torch::Tensor SA, torch::Tensor B,
+              torch::Tensor SB, torch::Tensor C,
+              c10::optional<torch::Tensor> bias,
+              c10::optional<torch::Tensor> residual, int64_t act) {
+  check_type(C, torch::kBFloat16, "C");
+  check_rows(C, "C");
+  check_type(A, kFp8, "A");
+  TORCH_CHECK(A.dim() == 2, "A must be 2D");
+  const int64_t M = C.size(0), N = C.size(1), Kp = A.size(1);
+  TORCH_CHECK(Kp >= 128 && Kp % 128 == 0 && Kp <= 1 << 22,
+              "A must hold whole blocks of 128 along K, 2^22 values at most, "
+              "got ", Kp);
+  TORCH_CHECK(N >= 1 && N < 1 << 30 && M < 1 << 30, "C is too large or empty: ",
+              C.sizes());
+  TORCH_CHECK(blocks128(M) * blocks128(N) < 1 << 30, "C is too large");
+  TORCH_CHECK(M * (Kp / 128) < 1 << 30, "SA is too large");
+  check_whole(A, kFp8, {M, Kp}, "A");
+  check_whole(SA, torch::kFloat32, {Kp / 128, M}, "SA");
+  check_whole(B, kFp8, {N, Kp}, "B");
+  check_whole(SB, torch::kFloat32, {blocks128(N), Kp / 128}, "SB");
+  check_act(act);
+  std::vector<std::pair<const torch::Tensor*, const char*>> all = {
+      {&A, "A"}, {&SA, "SA"}, {&B, "B"}, {&SB, "SB"}, {&C, "C"}};
+  if (bias) {
+    check_whole(*bias, torch::kFloat32, {N}, "bias");
+    all.push_back({&*bias, "bias"});
+  }
+  if (residual) {
+    check_type(*residual, torch::kBFloat16, "residual");
+    check_shape(*residual, {M, N}, "residual");
+    check_rows(*residual, "residual");
+    all.push_back({&*residual, "residual"});
+  }
+  check_devices(all);
+  if (M == 0) return;
+  const c10::DeviceGuard guard(A.device());
+  const int64_t floats = gemm_fp8_workspace((int)M, (int)N, (int)Kp);
+  torch::Tensor ws;
+  if (floats) ws = torch::empty({floats}, SA.options());
+  launch_gemm_fp8(A.data_ptr(), SA.data_ptr<float>(), B.data_ptr(),
+                  SB.data_ptr<float>(), C.data_ptr(), row_stride(C),
+                  bias ? bias->data_ptr<float>() : nullptr,
+                  residual ? residual->data_ptr() : nullptr,
+                  residual ? row_stride(*residual) : 0, (int)M, (int)N,
+                  (int)Kp, (int)act, floats ? ws.data_ptr<float>() : nullptr,
+                  cur_stream());
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -319,6 +458,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gemm_batched_bf16", &gemm_batched_bf16);
   m.def("gemm_strided_bf16", &gemm_strided_bf16);
   m.def("attn_fused_bf16", &attn_fused_bf16);
+  m.def("quant_fp8", &quant_fp8, py::arg("X"), py::arg("Q"), py::arg("S"),
+        py::arg("block_rows") = 1,
+        "round to e4m3 with a scale for each block of 128 along K");
+  m.def("gemm_fp8", &gemm_fp8, py::arg("A"), py::arg("SA"), py::arg("B"),
+        py::arg("SB"), py::arg("C"), py::arg("bias") = py::none(),
+        py::arg("residual") = py::none(), py::arg("act") = 0,
+        "block-scaled fp8 MFMA GEMM: act(A @ B^T + bias + residual)");
   m.def("dwconv_bf16", [](torch::Tensor X, torch::Tensor W2,
                           c10::optional<torch::Tensor> bias,
                           c10::optional<torch::Tensor> residual,

@@ -104,3 +104,18 @@ void launch_attn_fused_bf16(const void* Q, const void* K, const void* V,
                             int64_t sK2, int lkd, int64_t sV1, int64_t sV2,
                             int lvd, int64_t sO1, int64_t sO2, int lod,
                             float scale, hipStream_t stream);
+
+// gemm_fp8.hip — e4m3 with a scale for each 128 values along K.
+// X [M][K] (row stride ldx) bf16 or f32 -> Q [M][Kp], Kp = K up to whole
+// blocks; S [Kp/128][M] (block_rows 1) or [M/128][Kp/128] (block_rows 128)
+void launch_quant_fp8(const void* X, bool f32, int64_t ldx, int64_t M, int K,
+                      void* Q, int Kp, float* S, int block_rows,
+                      hipStream_t stream);
+// floats that launch_gemm_fp8 needs at `part`
+int64_t gemm_fp8_workspace(int M, int N, int Kp);
+// C = act(A @ B^T + bias + residual), C bf16 with row stride ldc; act: 0 none, 1 relu, 2 relu6, 5 gelu
+void launch_gemm_fp8(const void* A, const float* SA, const void* B,
+                     const float* SB, void* C, int64_t ldc,
+                     const float* bias, const void* residual, int64_t ldr,
+                     int M, int N, int Kp, int act, float* part,
+                     hipStream_t stream);

@@ -1,0 +1,354 @@
+"""8-bit dense layers: quant_fp8 and gemm_fp8 against their definition in
+64 bits, and the calls that they refuse (those run without a GPU).
+
+Tolerances. e4m3 values and scales are compared exactly: each of their two
+roundings (the quotient to f32, then to e4m3) belongs to the definition. A
+product is rounded once at the store, by half a step of bf16. Its sums carry
+the matrix unit's own arithmetic, which single products of known size show: a
+product 2^3 next to one of 2^16 among the same 8 neighbours along K is kept, a
+product of 2^2 is lost; in another group of 8 it is kept down to 2^-7. So of
+each 8 products 7 lose less than 2^-13 of the largest one, and each addition
+of a group to the running sum drops less than 2^-23 of it: 16 groups a block
+and one addition for each of the K/128 blocks.
+"""
+import math
+
+import pytest
+import torch
+
+E4M3 = torch.float8_e4m3fn
+TINY = 2.0 ** -126
+
+
+@pytest.fixture(scope="module")
+def E():
+    from tensorflow_web_deploy_amd.ops.native import ext
+    return ext()
+
+
+def up128(n):
+    return -(-n // 128) * 128
+
+
+def quant_ref(x, block_rows):
+    """(e4m3 values as f64 [M, Kp], scales f32) of x in 64 bits, on the CPU."""
+    x = x.detach().cpu().double()
+    m, k = x.shape
+    full = torch.zeros(up128(m) if block_rows == 128 else m, up128(k),
+                       dtype=torch.float64)
+    full[:m, :k] = x
+    b = full.reshape(full.shape[0] // block_rows, block_rows, -1, 128)
+    top = b.abs().amax((1, 3))
+    s = (top / 448.0).float().clamp_min(TINY).double()
+    q = (b / s[:, None, :, None]).float().double()
+    step = torch.exp2(torch.floor(torch.log2(
+        q.abs().clamp(2.0 ** -6, 448.0))) - 3)
+    q = torch.round(q / step) * step  # ties to even
+    return q.reshape(full.shape)[:m], s.float()
+
+
+def run_quant(E, x, block_rows=1):
+    m, k = x.shape
+    kb = up128(k) // 128
+    q = torch.full((m, kb * 128), 7.0, device=x.device).to(E4M3)
+    s = torch.full((kb, m) if block_rows == 1 else (up128(m) // 128, kb), -1.0,
+                   device=x.device)
+    E.quant_fp8(x, q, s, block_rows)
+    return q, s
+
+
+def check_quant(x, q, s, block_rows):
+    rq, rs = quant_ref(x, block_rows)
+    got = s.cpu().t() if block_rows == 1 else s.cpu()
+    assert torch.equal(got, rs)
+    assert torch.equal(q.cpu().double(), rq)
+
+
+# ------------------------------------------------------------- refusals
+
+
+def _gemm_args(m=4, n=5, k=128, **kw):
+    a = {"A": torch.zeros(m, k).to(E4M3), "SA": torch.zeros(k // 128, m),
+         "B": torch.zeros(n, k).to(E4M3),
+         "SB": torch.zeros(up128(n) // 128, k // 128),
+         "C": torch.zeros(m, n, dtype=torch.bfloat16)}
+    a.update(kw)
+    return a
+
+
+@pytest.mark.parametrize("kw,word", [
+    ({"A": torch.zeros(4, 100).to(E4M3)}, "whole blocks"),
+    ({"A": torch.zeros(4, 128)}, "A must be Float8_e4m3fn"),
+    ({"A": torch.zeros(3, 128).to(E4M3)}, "A must be"),
+    ({"A": torch.zeros(0, 0).to(E4M3)}, "whole blocks"),
+    ({"SA": torch.zeros(4, 1)}, "SA must be"),
+    ({"SA": torch.zeros(1, 4, dtype=torch.float64)}, "SA must be Float"),
+    ({"B": torch.zeros(5, 256).to(E4M3)}, "B must be"),
+    ({"B": torch.zeros(128, 5).to(E4M3).t()}, "B must be contiguous"),
+    ({"SB": torch.zeros(2, 1)}, "SB must be"),
+    ({"C": torch.zeros(4, 5)}, "C must be BFloat16"),
+    ({"C": torch.zeros(5, 4, dtype=torch.bfloat16).t()}, "contiguous rows"),
+    ({"C": torch.zeros(1, 5, dtype=torch.bfloat16).expand(4, 5)}, "overlap"),
+    ({"C": torch.zeros(20, dtype=torch.bfloat16)}, "2D"),
+    ({"bias": torch.zeros(4)}, "bias must be"),
+    ({"bias": torch.zeros(5, dtype=torch.bfloat16)}, "bias must be Float"),
+    ({"residual": torch.zeros(4, 5)}, "residual must be BFloat16"),
+    ({"residual": torch.zeros(4, 6, dtype=torch.bfloat16)},
+     "residual must be"),
+    ({"act": 3}, "act must be"),
+    ({"act": -1}, "act must be"),
+    ({}, "A must be on GPU"),
+])
+def test_gemm_refuses(E, kw, word):
+    with pytest.raises(RuntimeError, match=word):
+        E.gemm_fp8(**_gemm_args(**kw))
+
+
+@pytest.mark.parametrize("x,q,s,rows,word", [
+    (torch.zeros(4, 130, dtype=torch.float64), (4, 256), (2, 4), 1,
+     "bf16 or f32"),
+    (torch.zeros(4, 130), (4, 130), (2, 4), 1, "Q must be"),
+    (torch.zeros(4, 130), (4, 256), (4, 2), 1, "S must be"),
+    (torch.zeros(4, 130), (4, 256), (2, 4), 128, "S must be"),
+    (torch.zeros(4, 130), (4, 256), (2, 4), 64, "block_rows"),
+    (torch.zeros(4, 0), (4, 0), (0, 4), 1, "K must be"),
+    (torch.zeros(130, 4).t(), (4, 256), (2, 4), 1, "contiguous rows"),
+    (torch.zeros(130), (4, 256), (2, 4), 1, "2D"),
+    (torch.zeros(4, 130), (4, 256), (2, 4), 1, "on GPU"),
+])
+def test_quant_refuses(E, x, q, s, rows, word):
+    with pytest.raises(RuntimeError, match=word):
+        E.quant_fp8(x, torch.zeros(q).to(E4M3), torch.zeros(s), rows)
+
+
+def test_reference_rounds_to_even_and_keeps_zeros():
+    x = torch.tensor([[448.0, 17.0, 19.0, -17.0, 0.0, 2.0 ** -10, 460.0]])
+    x = torch.cat([x[:, :6], torch.zeros(1, 122)], 1)
+    q, s = quant_ref(x, 1)
+    assert s.item() == 1.0
+    assert q[0, :6].tolist() == [448.0, 16.0, 20.0, -16.0, 0.0, 0.0]
+
+
+# ------------------------------------------------------------ quant_fp8
+
+SIZES = [(1, 1), (1, 128), (3, 127), (17, 129), (2, 768), (33, 1000),
+         (257, 640), (5, 4099)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("block_rows", [1, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,k", SIZES)
+def test_quant(E, m, k, dtype, block_rows):
+    g = torch.Generator().manual_seed(m * 1000 + k)
+    x = torch.randn(m, k, generator=g) * torch.exp2(
+        torch.randint(-30, 30, (m, 1), generator=g).float())
+    x = x.to(dtype).cuda()
+    check_quant(x, *run_quant(E, x, block_rows), block_rows)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_quant_ends_of_the_range(E, dtype):
+    """Blocks of zeros, of the smallest and of the largest numbers."""
+    g = torch.Generator().manual_seed(5)
+    rows = [torch.zeros(128), torch.randn(128, generator=g) * 2.0 ** -140,
+            torch.randn(128, generator=g) * 2.0 ** -118,
+            torch.randn(128, generator=g).clamp(-1, 1) * 3e38,
+            torch.full((128,), 1e-45), torch.full((128,), -0.0)]
+    x = torch.stack(rows).to(dtype).cuda()
+    check_quant(x, *run_quant(E, x), 1)
+
+
+@pytest.mark.gpu
+def test_quant_infinity_and_nan_stay_in_their_block(E):
+    g = torch.Generator().manual_seed(6)
+    x = torch.randn(4, 384, generator=g)
+    x[1, 130] = math.inf
+    x[2, 5] = math.nan
+    q, s = run_quant(E, x.cuda())
+    q, s = q.float().cpu(), s.cpu()
+    assert s[1, 1] == math.inf and s[0, 2].isnan()
+    assert q[1, 130].isnan() and q[2, :128].isnan().all()
+    # finite values over an infinite scale
+    assert q[1, 128:130].abs().sum() == 0 and q[1, 131:256].abs().sum() == 0
+    x[1, 128:256] = 0
+    x[2, :128] = 0
+    keep = torch.ones(4, 384, dtype=torch.bool)
+    keep[1, 128:256] = keep[2, :128] = False
+    rq, rs = quant_ref(x, 1)
+    assert torch.equal(q[keep].double(), rq[keep])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("offset,width", [(0, 300), (1, 300), (7, 301)])
+def test_quant_rows_that_lie_apart(E, dtype, offset, width):
+    g = torch.Generator().manual_seed(7)
+    x = torch.randn(9, 400, generator=g).to(dtype).cuda()
+    v = x[:, offset:offset + width]
+    for rows in (1, 128):
+        check_quant(v, *run_quant(E, v, rows), rows)
+
+
+@pytest.mark.gpu
+def test_quant_no_rows(E):
+    q, s = run_quant(E, torch.zeros(0, 200, device="cuda"))
+    assert q.shape == (0, 256) and s.shape == (2, 0)
+
+
+# ------------------------------------------------------------- gemm_fp8
+
+
+def act_ref(y, act):
+    return {0: lambda v: v, 1: torch.relu, 2: lambda v: v.clamp(0, 6),
+            5: lambda v: 0.5 * v * torch.erfc(-v / math.sqrt(2))}[act](y)
+
+
+def operands(E, m, n, k, seed=0, spread=3.0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(m, k, generator=g) * torch.exp2(
+        (torch.rand(m, 1, generator=g) - 0.5) * 2 * spread)
+    w = torch.randn(n, k, generator=g) * k ** -0.5
+    w *= torch.exp2((torch.rand(n, 1, generator=g) - 0.5) * 2 * spread)
+    return (*run_quant(E, x.cuda()), *run_quant(E, w.cuda(), 128))
+
+
+def values64(q, s, block_rows):
+    q, s = q.cpu().double(), s.cpu().double()
+    s = s.t() if block_rows == 1 else s.repeat_interleave(128, 0)[:len(q)]
+    return q * s.repeat_interleave(128, 1)
+
+
+def check_gemm(got, qa, sa, qb, sb, bias=None, res=None, act=0):
+    a, b = values64(qa, sa, 1), values64(qb, sb, 128)
+    y, size = a @ b.t(), a.abs() @ b.abs().t()
+    if bias is not None:
+        y, size = y + bias.cpu().double(), size + bias.cpu().double().abs()
+    if res is not None:
+        y, size = y + res.cpu().double(), size + res.cpu().double().abs()
+    # relu, relu6 and erf-GELU have slopes below 1.13; erff is within
+    # 2^-21 of erf, times half the value
+    ref = act_ref(y, act)
+    k = qa.shape[1]
+    lost = torch.zeros_like(y)
+    for i in range(0, k, 8):  # 7/2^13 of the largest product of each 8
+        top = [a[:, None, j].abs() * b[None, :, j].abs()
+               for j in range(i, i + 8)]
+        lost += 7 * 2.0 ** -13 * torch.stack(top).amax(0)
+    tol = 1.13 * (lost + (k / 128 + 16) * 2.0 ** -23 * size)
+    tol = tol + 2.0 ** -22 * y.abs()
+    tol = tol + 2.0 ** -8 * ref.abs() + 1e-38
+    off = (got.cpu().double() - ref).abs()
+    assert (off <= tol).all(), (off / tol).max()
+
+
+GEMMS = [(1, 1, 1), (1, 16, 128), (2, 17, 300), (16, 1000, 768),
+         (17, 129, 129), (63, 64, 1000), (65, 200, 4096), (128, 128, 128),
+         (130, 257, 640), (300, 96, 2048), (5, 4096, 1280), (257, 513, 384)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", GEMMS)
+def test_gemm(E, m, n, k):
+    ops = operands(E, m, n, k, seed=m + n + k)
+    c = torch.full((m, n), math.nan, dtype=torch.bfloat16, device="cuda")
+    E.gemm_fp8(*ops, c)
+    check_gemm(c, *ops)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", [0, 1, 2, 5])
+@pytest.mark.parametrize("m,n,k", [(3, 40, 256), (64, 96, 4096),
+                                   (200, 250, 384)])
+def test_gemm_epilogue(E, m, n, k, act):
+    ops = operands(E, m, n, k, seed=act)
+    g = torch.Generator().manual_seed(1)
+    bias = torch.randn(n, generator=g).cuda()
+    res = torch.randn(m, n, generator=g).to(torch.bfloat16).cuda()
+    for b, r in ((bias, None), (None, res), (bias, res)):
+        c = torch.full((m, n), math.nan, dtype=torch.bfloat16, device="cuda")
+        E.gemm_fp8(*ops, c, b, r, act)
+        check_gemm(c, *ops, b, r, act)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("offset", [0, 1, 8])
+@pytest.mark.parametrize("m,n,k", [(40, 72, 256), (40, 71, 8192)])
+def test_gemm_into_a_slice(E, m, n, k, offset):
+    """Columns of a wider tensor: only they are written."""
+    ops = operands(E, m, n, k)
+    wide = torch.full((m + 2, n + 20), 3.0, dtype=torch.bfloat16, device="cuda")
+    res = torch.randn(m, n + 9, device="cuda").to(torch.bfloat16)[:, 3:n + 3]
+    c = wide[1:m + 1, offset:offset + n]
+    E.gemm_fp8(*ops, c, None, res, 0)
+    check_gemm(c, *ops, None, res, 0)
+    wide[1:m + 1, offset:offset + n] = 3.0
+    assert (wide == 3.0).all()
+
+
+@pytest.mark.gpu
+def test_gemm_residual_in_place(E):
+    ops = operands(E, 70, 130, 512)
+    c = torch.randn(70, 130, device="cuda").to(torch.bfloat16)
+    res = c.clone()
+    E.gemm_fp8(*ops, c, None, c, 0)
+    check_gemm(c, *ops, None, res, 0)
+
+
+@pytest.mark.gpu
+def test_gemm_nan_stays_in_its_row(E):
+    qa, sa, qb, sb = operands(E, 20, 33, 256)
+    want = torch.empty(20, 33, dtype=torch.bfloat16, device="cuda")
+    E.gemm_fp8(qa, sa, qb, sb, want)
+    sa[1, 7] = math.nan
+    c = torch.empty_like(want)
+    E.gemm_fp8(qa, sa, qb, sb, c)
+    assert c[7].isnan().all()
+    c[7], want[7] = 0, 0
+    assert torch.equal(c, want)
+
+
+@pytest.mark.gpu
+def test_gemm_no_rows_and_same_bits_again(E):
+    ops = operands(E, 77, 200, 4096)
+    c = [torch.empty(77, 200, dtype=torch.bfloat16, device="cuda")
+         for _ in range(2)]
+    for y in c:
+        E.gemm_fp8(*ops, y)
+    assert torch.equal(*c)
+    qa, sa, qb, sb = ops
+    E.gemm_fp8(qa[:0], sa[:, :0].contiguous(), qb, sb, c[0][:0])
+
+
+@pytest.mark.gpu
+def test_layer_on_a_stream_and_in_a_graph(E):
+    """Rounding and product as a layer runs them: captured, replayed with new
+    inputs, with other work between the replays."""
+    g = torch.Generator().manual_seed(3)
+    x = torch.zeros(50, 700, dtype=torch.bfloat16, device="cuda")
+    qb, sb = run_quant(E, torch.randn(90, 700, generator=g).cuda(), 128)
+    q = torch.empty(50, 768, dtype=E4M3, device="cuda")
+    s = torch.empty(6, 50, device="cuda")
+    c = torch.empty(50, 90, dtype=torch.bfloat16, device="cuda")
+
+    def layer(y):
+        E.quant_fp8(x, q, s)
+        E.gemm_fp8(q, s, qb, sb, y, None, None, 5)
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        layer(c)
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        layer(c)
+    for i in range(3):
+        x.copy_(torch.randn(50, 700, generator=g))
+        graph.replay()
+        got = c.clone()
+        eager = torch.empty_like(c)
+        layer(eager)
+        torch.cuda.synchronize()
+        assert torch.equal(got, eager)
+        check_gemm(got, q, s, qb, sb, None, None, 5)
