@@ -29,6 +29,7 @@ ext = cpp_extension.CUDAExtension(
         os.path.join(CSRC, "jpeg_gpu.hip"),
         os.path.join(CSRC, "gemm_8p.hip"),
         os.path.join(CSRC, "gemm_fp8.hip"),
+        os.path.join(CSRC, "moe.hip"),
     ],
     extra_compile_args={
         "cxx": ["-O3", "-std=c++17"],

@@ -437,6 +437,182 @@ void gemm_fp8(torch::Tensor A, torch::Tensor SA, torch::Tensor B,
                   cur_stream());
 }
 
+// ---- mixture-of-experts layers
+
+// logits [T,E] bf16|f32 -> ids i32 [T,k], weights f32 [T,k]. score: 0 softmax,
+// 1 sigmoid; bias f32 [E] is added for the choice alone. With groups > 1 the
+// experts are taken from the `kept` groups whose `best` (1 or 2) largest
+// score + bias add up to the most. A logit of -inf or NaN shuts an expert for
+// its row; places that no expert is left for get id -1 and weight 0. Choices
+// are those of the scores in 64 bits, the lower index first among equals.
+void moe_route(torch::Tensor logits, c10::optional<torch::Tensor> bias,
+               torch::Tensor ids, torch::Tensor weights, int64_t score,
+               int64_t groups, int64_t kept, int64_t best, bool renorm,
+               double scale) {
+  check_bf16_or_f32(logits, "logits");
+  check_rows(logits, "logits");
+  const int64_t T = logits.size(0), E = logits.size(1);
+  TORCH_CHECK(E >= 1 && E <= 512, "1 to 512 experts, got ", E);
+  TORCH_CHECK(T < 1 << 30, "too many rows: ", T);
+  TORCH_CHECK(score == 0 || score == 1,
+              "score must be 0 (softmax) or 1 (sigmoid), got ", score);
+  TORCH_CHECK(groups >= 1 && groups <= 64 && E % groups == 0,
+              "groups must be 1 to 64 and divide the experts, got ", groups);
+  TORCH_CHECK(kept >= 1 && kept <= groups, "kept must be 1 to groups, got ",
+              kept);
+  TORCH_CHECK(best == 1 || best == 2, "best must be 1 or 2, got ", best);
+  TORCH_CHECK(ids.dim() == 2, "ids must be 2D");
+  const int64_t k = ids.size(1);
+  TORCH_CHECK(k >= 1 && k <= 64 && k <= kept * (E / groups),
+              "k must be 1 to 64 and no more than the kept groups hold, got ",
+              k);
+  check_whole(ids, torch::kInt32, {T, k}, "ids");
+  check_whole(weights, torch::kFloat32, {T, k}, "weights");
+  std::vector<std::pair<const torch::Tensor*, const char*>> all = {
+      {&logits, "logits"}, {&ids, "ids"}, {&weights, "weights"}};
+  if (bias) {
+    check_whole(*bias, torch::kFloat32, {E}, "bias");
+    all.push_back({&*bias, "bias"});
+  }
+  check_devices(all);
+  if (T == 0) return;
+  const c10::DeviceGuard guard(logits.device());
+  launch_moe_route(logits.data_ptr(),
+                   logits.scalar_type() == torch::kFloat32,
+                   row_stride(logits), bias ? bias->data_ptr<float>() : nullptr,
+                   ids.data_ptr<int>(), weights.data_ptr<float>(), (int)T,
+                   (int)E, (int)k, score == 1, (int)groups, (int)kept,
+                   (int)best, renorm, (float)scale, cur_stream());
+}
+
+// A call's rows are taken so many at a time that its workspace stays within
+// some gigabytes and every offset within 32 bits.
+constexpr int64_t kMoeRows = 1 << 17;
+
+void moe_mlp(const torch::Tensor& X, const torch::Tensor& ids,
+             const torch::Tensor& weights, const torch::Tensor& W1,
+             const torch::Tensor* S1, const c10::optional<torch::Tensor>& b1,
+             const torch::Tensor& W2, const torch::Tensor* S2,
+             const c10::optional<torch::Tensor>& b2, const torch::Tensor& Y,
+             const c10::optional<torch::Tensor>& residual, int64_t act) {
+  const bool fp8 = S1 != nullptr;
+  check_type(X, torch::kBFloat16, "X");
+  check_rows(X, "X");
+  const int64_t T = X.size(0), D = X.size(1);
+  TORCH_CHECK(ids.dim() == 2, "ids must be 2D");
+  const int64_t k = ids.size(1);
+  TORCH_CHECK(k >= 1 && k <= 64, "1 to 64 experts a row, got ", k);
+  check_whole(ids, torch::kInt32, {T, k}, "ids");
+  check_whole(weights, torch::kFloat32, {T, k}, "weights");
+  TORCH_CHECK(W1.dim() == 3, "W1 must be 3D");
+  const int64_t E = W1.size(0), H = W1.size(1);
+  TORCH_CHECK(E >= 1 && E <= 1024, "1 to 1024 experts, got ", E);
+  TORCH_CHECK(T < 1 << 30, "too many rows: ", T);
+  TORCH_CHECK(D >= 1 && D <= 1 << 18 && H >= 1 && H <= 1 << 18,
+              "widths must be 1 to 2^18, got ", D, " and ", H);
+  const int64_t unit = fp8 ? 128 : 64;
+  const int64_t Dp = (D + unit - 1) / unit * unit;
+  const int64_t Hp = (H + unit - 1) / unit * unit;
+  const auto wtype = fp8 ? kFp8 : torch::kBFloat16;
+  check_whole(W1, wtype, {E, H, Dp}, "W1");
+  check_whole(W2, wtype, {E, D, Hp}, "W2");
+  check_type(Y, torch::kBFloat16, "Y");
+  check_shape(Y, {T, D}, "Y");
+  check_rows(Y, "Y");
+  check_act(act);
+  std::vector<std::pair<const torch::Tensor*, const char*>> all = {
+      {&X, "X"}, {&ids, "ids"}, {&weights, "weights"},
+      {&W1, "W1"}, {&W2, "W2"}, {&Y, "Y"}};
+  if (fp8) {
+    check_whole(*S1, torch::kFloat32, {E, blocks128(H), Dp / 128}, "S1");
+    check_whole(*S2, torch::kFloat32, {E, blocks128(D), Hp / 128}, "S2");
+    all.push_back({S1, "S1"});
+    all.push_back({S2, "S2"});
+  }
+  if (b1) {
+    check_whole(*b1, torch::kFloat32, {E, H}, "b1");
+    all.push_back({&*b1, "b1"});
+  }
+  if (b2) {
+    check_whole(*b2, torch::kFloat32, {E, D}, "b2");
+    all.push_back({&*b2, "b2"});
+  }
+  if (residual) {
+    check_type(*residual, torch::kBFloat16, "residual");
+    check_shape(*residual, {T, D}, "residual");
+    check_rows(*residual, "residual");
+    all.push_back({&*residual, "residual"});
+  }
+  check_devices(all);
+  if (T == 0) return;
+  const c10::DeviceGuard guard(X.device());
+  const int64_t chunk =
+      std::min(T, std::max<int64_t>(1, std::min(kMoeRows / k,
+                                                (int64_t(1) << 31) / (Dp * 2))));
+  MoeMlp m{};
+  m.W1 = W1.data_ptr();
+  m.W2 = W2.data_ptr();
+  if (fp8) {
+    m.S1 = S1->data_ptr<float>();
+    m.S2 = S2->data_ptr<float>();
+  }
+  if (b1) m.b1 = b1->data_ptr<float>();
+  if (b2) m.b2 = b2->data_ptr<float>();
+  m.ldx = row_stride(X);
+  m.ldy = row_stride(Y);
+  m.ldr = residual ? row_stride(*residual) : 0;
+  m.E = (int)E;
+  m.k = (int)k;
+  m.D = (int)D;
+  m.H = (int)H;
+  m.act = (int)act;
+  m.fp8 = fp8;
+  auto rows = [&](int64_t t) {
+    m.X = (const char*)X.data_ptr() + t * m.ldx * 2;
+    m.Y = (char*)Y.data_ptr() + t * m.ldy * 2;
+    m.residual = residual
+                     ? (const char*)residual->data_ptr() + t * m.ldr * 2
+                     : nullptr;
+    m.ids = ids.data_ptr<int>() + t * k;
+    m.weights = weights.data_ptr<float>() + t * k;
+    m.T = (int)std::min(chunk, T - t);
+  };
+  int64_t bytes = 0;
+  for (int64_t t = 0; t < T; t += chunk) {
+    rows(t);
+    bytes = std::max(bytes, moe_mlp_workspace(m));
+  }
+  auto ws = torch::empty({bytes}, X.options().dtype(torch::kUInt8));
+  for (int64_t t = 0; t < T; t += chunk) {
+    rows(t);
+    launch_moe_mlp(m, ws.data_ptr(), cur_stream());
+  }
+}
+
+// Y[t] = residual[t] + sum_j weights[t,j] (act(X[t] @ W1[e]^T + b1[e])
+//        @ W2[e]^T + b2[e]),  e = ids[t,j]; an id outside of 0..E-1 adds
+// nothing. X, Y, residual bf16 [T,D]; W1 [E,H,D up to 64s], W2
+// [E,D,H up to 64s] bf16, filled up with zeros
+void moe_mlp_bf16(torch::Tensor X, torch::Tensor ids, torch::Tensor weights,
+                  torch::Tensor W1, c10::optional<torch::Tensor> b1,
+                  torch::Tensor W2, c10::optional<torch::Tensor> b2,
+                  torch::Tensor Y, c10::optional<torch::Tensor> residual,
+                  int64_t act) {
+  moe_mlp(X, ids, weights, W1, nullptr, b1, W2, nullptr, b2, Y, residual, act);
+}
+
+// the same on e4m3 weights, each expert's as quant_fp8 leaves them with
+// block_rows 128. X and the hidden rows are rounded to e4m3 with a scale for
+// each 128 values.
+void moe_mlp_fp8(torch::Tensor X, torch::Tensor ids, torch::Tensor weights,
+                 torch::Tensor W1, torch::Tensor S1,
+                 c10::optional<torch::Tensor> b1, torch::Tensor W2,
+                 torch::Tensor S2, c10::optional<torch::Tensor> b2,
+                 torch::Tensor Y, c10::optional<torch::Tensor> residual,
+                 int64_t act) {
+  moe_mlp(X, ids, weights, W1, &S1, b1, W2, &S2, b2, Y, residual, act);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -465,6 +641,20 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("SB"), py::arg("C"), py::arg("bias") = py::none(),
         py::arg("residual") = py::none(), py::arg("act") = 0,
         "block-scaled fp8 MFMA GEMM: act(A @ B^T + bias + residual)");
+  m.def("moe_route", &moe_route, py::arg("logits"), py::arg("bias"),
+        py::arg("ids"), py::arg("weights"), py::arg("score") = 0,
+        py::arg("groups") = 1, py::arg("kept") = 1, py::arg("best") = 1,
+        py::arg("renorm") = true, py::arg("scale") = 1.0,
+        "the experts of each row and their weights");
+  m.def("moe_mlp_bf16", &moe_mlp_bf16, py::arg("X"), py::arg("ids"),
+        py::arg("weights"), py::arg("W1"), py::arg("b1"), py::arg("W2"),
+        py::arg("b2"), py::arg("Y"), py::arg("residual") = py::none(),
+        py::arg("act") = 0, "weighted sum of each row's experts");
+  m.def("moe_mlp_fp8", &moe_mlp_fp8, py::arg("X"), py::arg("ids"),
+        py::arg("weights"), py::arg("W1"), py::arg("S1"), py::arg("b1"),
+        py::arg("W2"), py::arg("S2"), py::arg("b2"), py::arg("Y"),
+        py::arg("residual") = py::none(), py::arg("act") = 0,
+        "weighted sum of each row's experts, on e4m3 weights");
   m.def("dwconv_bf16", [](torch::Tensor X, torch::Tensor W2,
                           c10::optional<torch::Tensor> bias,
                           c10::optional<torch::Tensor> residual,

@@ -112,22 +112,6 @@ struct Dense {
   bool vec;  // rows of C (and of the residual) take 16-byte accesses
 };
 
-template <int ACT, int R>
-__device__ __forceinline__ void activate_all(float (&v)[R]) {
-#pragma unroll
-  for (int e = 0; e < R; ++e) v[e] = activate<ACT>(v[e]);
-}
-
-template <int R>
-__device__ __forceinline__ void activate_by(float (&v)[R], int act) {
-  if (act == 1)
-    activate_all<1>(v);
-  else if (act == 2)
-    activate_all<2>(v);
-  else if (act == 5)
-    activate_all<5>(v);
-}
-
 // R consecutive columns from n on of row m: + bias + residual, activation,
 // one rounding, store
 template <int R>
@@ -200,7 +184,7 @@ __global__ __launch_bounds__(S::THREADS) void gemm_fp8_kernel(Dense d) {
   const int wave_n0 = n0 + wn * S::NT * 16;
   const int top_block = (d.N - 1) / 128;
   f32x4 acc[S::MT][S::NT];
-  product<S, false>(smem, ra, rb, rs, at, first, count, 0, (uint32_t)d.M * 4,
+  product<S>(smem, ra, rb, rs, at, first, count, (uint32_t)d.M * 4,
                     d.SB + (int64_t)min(wave_n0 / 128, top_block) * all, wave,
                     lane, acc);
 

@@ -119,3 +119,26 @@ void launch_gemm_fp8(const void* A, const float* SA, const void* B,
                      const float* bias, const void* residual, int64_t ldr,
                      int M, int N, int Kp, int act, float* part,
                      hipStream_t stream);
+
+// moe.hip — mixture-of-experts layers
+// logits [T][E] (row stride ldx) bf16 or f32 -> the k experts of each row and
+// their weights; rows or experts that have none get id -1 and weight 0.
+// E <= 512, k <= 64, groups <= 64
+void launch_moe_route(const void* X, bool f32, int64_t ldx, const float* bias,
+                      int* ids, float* weights, int T, int E, int k,
+                      bool sigmoid, int groups, int kept, int best,
+                      bool renorm, float scale, hipStream_t stream);
+// Y[t] = residual[t] + sum_j weights[t][j] mlp_{ids[t][j]}(X[t]); ids outside
+// of 0..E-1 name no expert. Weights are bf16 [E][H][D up to 64s] and
+// [E][D][H up to 64s], or e4m3, up to 128s, with their scales.
+struct MoeMlp {
+  const void *X, *W1, *W2, *residual;
+  const int* ids;
+  const float *weights, *S1, *b1, *S2, *b2;
+  void* Y;
+  int64_t ldx, ldy, ldr;
+  int T, E, k, D, H, act;
+  bool fp8;
+};
+int64_t moe_mlp_workspace(const MoeMlp& m);  // bytes
+void launch_moe_mlp(const MoeMlp& m, void* ws, hipStream_t stream);

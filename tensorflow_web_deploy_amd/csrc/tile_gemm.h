@@ -65,9 +65,8 @@ __device__ __forceinline__ void load_lds(__amdgpu_buffer_rsrc_t r, char* to,
     __builtin_amdgcn_raw_ptr_buffer_load_lds(r, lds, 4, (int)at, 0, 0, 0);
 }
 
-// The rows that this lane stages: byte offsets of their first value, and
-// whether the 128 bytes of a step can pass the row's end (bf16 inputs whose
-// width is no multiple of 64; those bytes have to read as 0).
+// The rows that this lane stages: byte offsets of their first value, NOWHERE
+// for a row that isn't there
 template <class S>
 struct Rows {
   uint32_t a[S::CA], b[S::CB], s;
@@ -88,21 +87,20 @@ __device__ __forceinline__ int staged_row(int wave, int count, int i,
   return (wave * count + i) * 8 + (lane >> 3);
 }
 
-template <class S, bool TAIL>
+template <class S>
 __device__ __forceinline__ void stage(char* lds, __amdgpu_buffer_rsrc_t ra,
                                       __amdgpu_buffer_rsrc_t rb,
                                       __amdgpu_buffer_rsrc_t rs,
                                       const Rows<S>& at, int step,
-                                      uint32_t row_bytes, uint32_t s_stride,
+                                      uint32_t s_stride,
                                       int wave, int lane) {
   const int slot = lane & 7;
 #pragma unroll
   for (int i = 0; i < S::CA; ++i) {
     const int r = staged_row<S>(wave, S::CA, i, lane);
     const uint32_t k = (uint32_t)step * STEP + ((slot ^ (r & 7)) << 4);
-    const bool out = TAIL && k >= row_bytes;
     load_lds<16>(ra, lds + (wave * S::CA + i) * 1024,
-                 out || at.a[i] == NOWHERE ? NOWHERE : at.a[i] + k);
+                 at.a[i] == NOWHERE ? NOWHERE : at.a[i] + k);
   }
   char* ldsb = lds + S::BM * STEP;
 #pragma unroll
@@ -170,13 +168,13 @@ __device__ __forceinline__ void compute(const char* lds, float sb, int wm,
 
 // Steps [first, first + count) of the product. sb: the scales of the wave's
 // columns, one a step.
-template <class S, bool TAIL>
+template <class S>
 __device__ __forceinline__ void product(char* smem, __amdgpu_buffer_rsrc_t ra,
                                         __amdgpu_buffer_rsrc_t rb,
                                         __amdgpu_buffer_rsrc_t rs,
                                         const Rows<S>& at, int first,
-                                        int count, uint32_t row_bytes,
-                                        uint32_t s_stride, const float* sb,
+                                        int count, uint32_t s_stride,
+                                        const float* sb,
                                         int wave, int lane,
                                         f32x4 (&acc)[S::MT][S::NT]) {
   const int wm = wave / S::WN, wn = wave % S::WN;
@@ -188,8 +186,8 @@ __device__ __forceinline__ void product(char* smem, __amdgpu_buffer_rsrc_t ra,
 #pragma unroll
   for (int j = 0; j < AHEAD; ++j)
     if (j < count)
-      stage<S, TAIL>(smem + j * S::STAGE, ra, rb, rs, at, first + j,
-                     row_bytes, s_stride, wave, lane);
+      stage<S>(smem + j * S::STAGE, ra, rb, rs, at, first + j,
+                     s_stride, wave, lane);
   int now = 0, next = AHEAD % S::DEPTH;
   for (int j = 0; j < count; ++j) {
     // step j has landed once only the later ones are still on their way
@@ -203,8 +201,8 @@ __device__ __forceinline__ void product(char* smem, __amdgpu_buffer_rsrc_t ra,
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     if (j + AHEAD < count)
-      stage<S, TAIL>(smem + next * S::STAGE, ra, rb, rs, at, first + j + AHEAD,
-                     row_bytes, s_stride, wave, lane);
+      stage<S>(smem + next * S::STAGE, ra, rb, rs, at, first + j + AHEAD,
+                     s_stride, wave, lane);
     compute<S>(smem + now * S::STAGE, S::FP8 ? sb[first + j] : 0.f, wm, wn,
                lane, acc);
     // the stage is free for the load behind the next barrier
@@ -221,6 +219,22 @@ __device__ __forceinline__ float activate(float v) {
   if (ACT == 2) return v < 0.f ? 0.f : v > 6.f ? 6.f : v;
   if (ACT == 5) return 0.5f * v * (1.f + erff(v * 0.70710678f));
   return v;
+}
+
+template <int ACT, int R>
+__device__ __forceinline__ void activate_all(float (&v)[R]) {
+#pragma unroll
+  for (int e = 0; e < R; ++e) v[e] = activate<ACT>(v[e]);
+}
+
+template <int R>
+__device__ __forceinline__ void activate_by(float (&v)[R], int act) {
+  if (act == 1)
+    activate_all<1>(v);
+  else if (act == 2)
+    activate_all<2>(v);
+  else if (act == 5)
+    activate_all<5>(v);
 }
 
 // Workgroups go round the 8 XCDs in turn. Give each XCD a contiguous run of
