@@ -148,38 +148,27 @@ __device__ __forceinline__ void finish(const Dense& d, int64_t m, int n,
 }
 
 template <class S, bool SPLIT>
-__global__ __launch_bounds__(S::THREADS) void gemm_fp8_kernel(Dense d) {
+__global__ __launch_bounds__(S::THREADS, 2) void gemm_fp8_kernel(Dense d) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // 8 rows of tiles at a time, so that what an XCD holds at once shares both
-  // its rows and its columns
-  const int bid = by_xcd(blockIdx.x, d.tiles_m * d.tiles_n);
-  const int group = bid / (8 * d.tiles_n), in = bid - group * 8 * d.tiles_n;
-  const int high = min(8, d.tiles_m - group * 8);
-  const int tm = group * 8 + in % high, tn = in / high;
-  const int64_t m0 = (int64_t)tm * S::BM;
-  const int n0 = tn * S::BN;
+  const Place tile = place_of(blockIdx.x, d.tiles_m, d.tiles_n);
+  const int64_t m0 = (int64_t)tile.m * S::BM;
+  const int n0 = tile.n * S::BN;
   const int all = d.Kp / STEP;
   const int first = SPLIT ? blockIdx.y * d.steps : 0;
   const int count = SPLIT ? min(d.steps, all - first) : all;
 
-  const auto ra = buffer(d.A + m0 * d.Kp,
-                         (uint32_t)(min((int64_t)S::BM, d.M - m0) * d.Kp));
-  const auto rb = buffer(d.B + (int64_t)n0 * d.Kp,
-                         (uint32_t)(min(S::BN, d.N - n0) * (int64_t)d.Kp));
-  const auto rs = buffer(d.SA, (uint32_t)((int64_t)all * d.M * 4));
-  Rows<S> at;
-#pragma unroll
-  for (int i = 0; i < S::CA; ++i)
-    at.a[i] = (uint32_t)staged_row<S>(wave, S::CA, i, lane) * d.Kp;
-#pragma unroll
-  for (int i = 0; i < S::CB; ++i)
-    at.b[i] = (uint32_t)staged_row<S>(wave, S::CB, i, lane) * d.Kp;
-  {
-    const int64_t m = m0 + wave * (S::BM / S::WAVES) + lane;
-    at.s = m < d.M ? (uint32_t)m * 4 : NOWHERE;
-  }
+  const int rows = (int)min((int64_t)S::BM, d.M - m0);
+  const int cols = min(S::BN, d.N - n0);
+  const auto ra = buffer(d.A + m0 * d.Kp, (uint32_t)rows * d.Kp);
+  const auto rb = buffer(d.B + (int64_t)n0 * d.Kp, (uint32_t)cols * d.Kp);
+  const auto rs = buffer(d.SA, (uint32_t)all * d.M * 4);
+  const Rows<S> at = rows_of<S>(
+      wave, lane,
+      [&](int r) { return (uint32_t)min(r, rows - 1) * d.Kp; },
+      [&](int r) { return (uint32_t)min(r, cols - 1) * d.Kp; },
+      [&](int r) { return (uint32_t)(m0 + min(r, rows - 1)) * 4; });
   const int wm = wave / S::WN, wn = wave % S::WN;
   const int wave_n0 = n0 + wn * S::NT * 16;
   const int top_block = (d.N - 1) / 128;
@@ -188,30 +177,23 @@ __global__ __launch_bounds__(S::THREADS) void gemm_fp8_kernel(Dense d) {
                     d.SB + (int64_t)min(wave_n0 / 128, top_block) * all, wave,
                     lane, acc);
 
-  constexpr int R = 4 * S::NT;
-  const int n = wave_n0 + (lane >> 4) * R;
-  float b[R];
 #pragma unroll
-  for (int e = 0; e < R; ++e)
-    b[e] = !SPLIT && d.bias && n + e < d.N ? d.bias[n + e] : 0.f;
+  for (int q = 0; q < S::RUNS; ++q) {
+    const int n = wave_n0 + run_column<S>(q, lane);
+    if (n >= d.N) continue;
+    float b[S::W];
+    load_run(d.bias + n, !SPLIT && d.bias ? d.N - n : 0, b);
 #pragma unroll
-  for (int i = 0; i < S::MT; ++i) {
-    const int64_t m = m0 + wm * S::MT * 16 + i * 16 + (lane & 15);
-    if (m >= d.M) continue;
-    float v[R];
-#pragma unroll
-    for (int e = 0; e < R; ++e) v[e] = acc[i][e / 4][e % 4];
-    if (SPLIT) {
-      float* c = d.part + ((int64_t)blockIdx.y * d.M + m) * d.N + n;
-      if (n + R <= d.N) {
-        __builtin_memcpy(c, v, sizeof(v));
-      } else {
-#pragma unroll
-        for (int e = 0; e < R; ++e)
-          if (n + e < d.N) c[e] = v[e];
-      }
-    } else {
-      finish(d, m, n, v, b);
+    for (int i = 0; i < S::MT; ++i) {
+      const int64_t m = m0 + wm * S::MT * 16 + i * 16 + (lane & 15);
+      if (m >= d.M) continue;
+      float v[S::W];
+      run_of<S>(acc[i], q, v);
+      if (SPLIT)
+        store_run(d.part + ((int64_t)blockIdx.y * d.M + m) * d.N + n, d.N - n,
+                  v);
+      else
+        finish(d, m, n, v, b);
     }
   }
 }
@@ -226,32 +208,28 @@ __global__ __launch_bounds__(256) void gemm_fp8_join_kernel(Dense d,
   const int n = (int)(t - m * per) * 4;
   float v[4] = {0.f, 0.f, 0.f, 0.f}, b[4];
   for (int s = 0; s < slices; ++s) {
-    const float* c = d.part + ((int64_t)s * d.M + m) * d.N + n;
-    if (n + 4 <= d.N) {
-      float w[4];
-      __builtin_memcpy(w, c, sizeof(w));
+    float w[4];
+    load_run(d.part + ((int64_t)s * d.M + m) * d.N + n, d.N - n, w);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] += w[e];
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (n + e < d.N) v[e] += c[e];
-    }
+    for (int e = 0; e < 4; ++e) v[e] += w[e];
   }
-#pragma unroll
-  for (int e = 0; e < 4; ++e)
-    b[e] = d.bias && n + e < d.N ? d.bias[n + e] : 0.f;
+  load_run(d.bias + n, d.bias ? d.N - n : 0, b);
   Dense one = d;
   one.vec = false;
   finish(one, m, n, v, b);
 }
 
-using Tile128 = Shape<true, 128, 128, 2, 2, 2>;
+template <int W>
+using Tile128 = Shape<true, 128, 128, 2, 2, 2, W>;
+template <int W>
+using Tile256 = Shape<true, 256, 256, 2, 4, 2, W>;
 
 int up(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
-template <class S>
+template <template <int> class T>
 void run(Dense d, int slices, hipStream_t stream) {
+  using S = T<8>;   // bf16 results
+  using P = T<4>;   // f32 slices
   d.tiles_m = up(d.M, S::BM);
   d.tiles_n = up(d.N, S::BN);
   const dim3 grid(d.tiles_m * d.tiles_n, slices);
@@ -260,8 +238,8 @@ void run(Dense d, int slices, hipStream_t stream) {
                        dim3(S::THREADS), S::LDS, stream, d);
     return;
   }
-  hipLaunchKernelGGL((gemm_fp8_kernel<S, true>), grid, dim3(S::THREADS),
-                     S::LDS, stream, d);
+  hipLaunchKernelGGL((gemm_fp8_kernel<P, true>), grid, dim3(P::THREADS),
+                     P::LDS, stream, d);
   const int64_t work = (int64_t)d.M * ((d.N + 3) / 4);
   hipLaunchKernelGGL(gemm_fp8_join_kernel, dim3(up(work, 256)), dim3(256),
                      0, stream, d, slices);
@@ -270,7 +248,7 @@ void run(Dense d, int slices, hipStream_t stream) {
 // slices: how often K is cut so that the grid fills the 256 CUs
 void plan(int M, int N, int Kp, int* slices, int* steps) {
   const int64_t tiles =
-      (int64_t)up(M, Tile128::BM) * up(N, Tile128::BN);
+      (int64_t)up(M, 128) * up(N, 128);
   const int all = Kp / STEP;
   int s = 1;
   while (tiles * s < 256 && all / (s * 2) >= 4) s *= 2;
@@ -334,5 +312,8 @@ void launch_gemm_fp8(const void* A, const float* SA, const void* B,
           (!residual || ((uintptr_t)residual % 16 == 0 && ldr % 8 == 0));
   int slices;
   plan(M, N, Kp, &slices, &d.steps);
-  run<Tile128>(d, slices, stream);
+  if (slices == 1 && (int64_t)up(M, 256) * up(N, 256) >= 256)
+    run<Tile256>(d, slices, stream);
+  else
+    run<Tile128>(d, slices, stream);
 }

@@ -369,45 +369,38 @@ struct Experts {
 // kept in the order of the experts. Otherwise: rows as they lie, the result
 // is weighted and goes to its assignment's place, in f32.
 template <class S, bool FIRST>
-__global__ __launch_bounds__(S::THREADS) void experts_kernel(Experts p) {
+__global__ __launch_bounds__(S::THREADS, 2) void experts_kernel(Experts p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int bid = by_xcd(blockIdx.x, p.n_tiles * p.tiles_n);
-  const int group = bid / (8 * p.tiles_n), in = bid - group * 8 * p.tiles_n;
-  const int high = min(8, p.n_tiles - group * 8);
-  const int4 tile = p.tiles[group * 8 + in % high];
+  const Place at_tile = place_of(blockIdx.x, p.n_tiles, p.tiles_n);
+  const int4 tile = p.tiles[at_tile.m];
   const int e = __builtin_amdgcn_readfirstlane(tile.x);
   if (e < 0) return;
   const int at0 = __builtin_amdgcn_readfirstlane(tile.y);
   const int rows = __builtin_amdgcn_readfirstlane(tile.z);
-  const int n0 = in / high * S::BN;
+  const int n0 = at_tile.n * S::BN;
   const int64_t b_row = (int64_t)p.steps * STEP;
   const int blocks_n = (p.n + 127) / 128;
 
+  // at least 1: no tile consists of columns alone that only fill up H, as BN
+  // is a multiple of what H is filled up to
+  const int cols = min(S::BN, p.n - n0);
   const auto rb = buffer(p.B + ((int64_t)e * p.n + n0) * b_row,
-                         (uint32_t)(max(0, min(S::BN, p.n - n0)) * b_row));
+                         (uint32_t)(cols * b_row));
   const auto ra = FIRST ? buffer(p.A, p.a_bytes)
                         : buffer(p.A + at0 * p.a_row,
                                  (uint32_t)(rows * p.a_row));
   const auto rs = buffer(p.SA, p.sa_rows * 4 * p.steps);
-  Rows<S> at;
-  auto token = [&](int r) {  // the row of A and SA behind a row of the tile
-    return p.order[at0 + r] / p.k;
+  // the row of A and SA behind row r of the tile
+  auto place = [&](int r) {
+    r = min(r, rows - 1);
+    return FIRST ? p.order[at0 + r] / p.k : r;
   };
-#pragma unroll
-  for (int i = 0; i < S::CA; ++i) {
-    const int r = staged_row<S>(wave, S::CA, i, lane);
-    at.a[i] = r >= rows ? NOWHERE
-                        : (uint32_t)((FIRST ? token(r) : r) * p.a_row);
-  }
-#pragma unroll
-  for (int i = 0; i < S::CB; ++i)
-    at.b[i] = (uint32_t)staged_row<S>(wave, S::CB, i, lane) * (uint32_t)b_row;
-  if (S::FP8) {
-    const int r = wave * (S::BM / S::WAVES) + lane;
-    at.s = r >= rows ? NOWHERE : (uint32_t)(FIRST ? token(r) : at0 + r) * 4;
-  }
+  const Rows<S> at = rows_of<S>(
+      wave, lane, [&](int r) { return (uint32_t)(place(r) * p.a_row); },
+      [&](int r) { return (uint32_t)(min(r, cols - 1) * b_row); },
+      [&](int r) { return (uint32_t)(place(r) + (FIRST ? 0 : at0)) * 4; });
   const int wm = wave / S::WN, wn = wave % S::WN;
   const int wave_n0 = n0 + wn * S::NT * 16;
   f32x4 acc[S::MT][S::NT];
@@ -417,81 +410,111 @@ __global__ __launch_bounds__(S::THREADS) void experts_kernel(Experts p) {
                     : nullptr,
              wave, lane, acc);
 
-  constexpr int R = 4 * S::NT;
-  const int n = wave_n0 + (lane >> 4) * R;
-  float b[R];
-#pragma unroll
-  for (int q = 0; q < R; ++q)
-    b[q] = p.bias && n + q < p.n ? p.bias[(int64_t)e * p.n + n + q] : 0.f;
+  const float* bias = p.bias ? p.bias + (int64_t)e * p.n : nullptr;
+  auto row = [&](int i) { return wm * S::MT * 16 + i * 16 + (lane & 15); };
+  auto column = [&](int q) { return wave_n0 + run_column<S>(q, lane); };
+  auto load_bias = [&](int q, float(&b)[S::W]) {
+    load_run(bias + column(q), bias ? p.n - column(q) : 0, b);
+  };
 
+  if constexpr (FIRST) {
+    // activated in place; the columns that only fill up H stay 0
+#pragma unroll
+    for (int q = 0; q < S::RUNS; ++q) {
+      float b[S::W];
+      load_bias(q, b);
+#pragma unroll
+      for (int i = 0; i < S::MT; ++i) {
+        float v[S::W];
+        run_of<S>(acc[i], q, v);
+#pragma unroll
+        for (int c = 0; c < S::W; ++c) v[c] += b[c];
+        activate_by(v, p.act);
+#pragma unroll
+        for (int c = 0; c < S::W; ++c)
+          acc[i][q * (S::W / 4) + c / 4][c % 4] =
+              column(q) + c < p.n ? v[c] : 0.f;
+      }
+    }
+  }
   if constexpr (FIRST && S::FP8) {
     // a block of 128 columns is spread over SHARE waves: each leaves the
     // largest value of its rows in LDS
     constexpr int SHARE = 128 / (S::NT * 16);
     uint32_t* top = (uint32_t*)smem;  // [WN][BM]
     __syncthreads();
-    float v[S::MT][R];
 #pragma unroll
     for (int i = 0; i < S::MT; ++i) {
+      uint32_t m = 0;
 #pragma unroll
-      for (int q = 0; q < R; ++q) v[i][q] = acc[i][q / 4][q % 4] + b[q];
-      activate_by(v[i], p.act);
-      uint32_t m = amax_bits(v[i]);
+      for (int q = 0; q < S::RUNS; ++q) {
+        float v[S::W];
+        run_of<S>(acc[i], q, v);
+        m = max(m, amax_bits(v));
+      }
       m = max(m, (uint32_t)__shfl_xor((int)m, 16));
       m = max(m, (uint32_t)__shfl_xor((int)m, 32));
-      if (lane < 16) top[wn * S::BM + wm * S::MT * 16 + i * 16 + lane] = m;
+      if (lane < 16) top[wn * S::BM + row(i)] = m;
     }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < S::MT; ++i) {
-      const int r = wm * S::MT * 16 + i * 16 + (lane & 15);
+      const int r = row(i);
       uint32_t m = 0;
 #pragma unroll
-      for (int q = 0; q < SHARE; ++q)
-        m = max(m, top[(wn / SHARE * SHARE + q) * S::BM + r]);
-      if (r >= rows || n >= p.np) continue;
+      for (int w = 0; w < SHARE; ++w)
+        m = max(m, top[(wn / SHARE * SHARE + w) * S::BM + r]);
+      if (r >= rows || wave_n0 >= p.np) continue;
       const float s = scale_of(m);
-      uint8_t* h = (uint8_t*)p.H + (int64_t)(at0 + r) * p.np + n;
 #pragma unroll
-      for (int q = 0; q < R; q += 8) {
-        float u[8];
+      for (int q = 0; q < S::RUNS; ++q) {
+        float v[S::W];
+        run_of<S>(acc[i], q, v);
+        uint2 h[S::W / 8];
 #pragma unroll
-        for (int c = 0; c < 8; ++c) u[c] = v[i][q + c];
-        *(uint2*)(h + q) = to_fp8(u, s);
+        for (int c = 0; c < S::W / 8; ++c) {
+          float u[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) u[j] = v[c * 8 + j];
+          h[c] = to_fp8(u, s);
+        }
+        uint8_t* to = (uint8_t*)p.H + (int64_t)(at0 + r) * p.np + column(q);
+        __builtin_memcpy(__builtin_assume_aligned(to, sizeof(h)), h,
+                         sizeof(h));
       }
       if (lane < 16 && wn % SHARE == 0)
         p.SH[(int64_t)(wave_n0 / 128) * p.N + at0 + r] = s;
     }
-    return;
-  }
+  } else if constexpr (FIRST) {
 #pragma unroll
-  for (int i = 0; i < S::MT; ++i) {
-    const int r = wm * S::MT * 16 + i * 16 + (lane & 15);
-    if (r >= rows) continue;
-    float v[R];
+    for (int q = 0; q < S::RUNS; ++q)
 #pragma unroll
-    for (int q = 0; q < R; ++q) v[q] = acc[i][q / 4][q % 4] + b[q];
-    if constexpr (FIRST) {
-      activate_by(v, p.act);
-      if (n >= p.np) continue;
-      // rounded to bf16 here: the second product takes no wider operand
-      __bf16 t[R];
+      for (int i = 0; i < S::MT; ++i) {
+        if (row(i) >= rows || column(q) >= p.np) continue;
+        float v[S::W];
+        run_of<S>(acc[i], q, v);
+        // rounded to bf16 here: the second product takes no wider operand
+        __bf16 t[S::W];
 #pragma unroll
-      for (int q = 0; q < R; ++q) t[q] = (__bf16)v[q];
-      __bf16* h = (__bf16*)p.H + (int64_t)(at0 + r) * p.np + n;
-      __builtin_memcpy(__builtin_assume_aligned(h, 16), t, sizeof(t));
-    } else {
-      const int a = p.order[at0 + r];
+        for (int c = 0; c < S::W; ++c) t[c] = (__bf16)v[c];
+        __bf16* h =
+            (__bf16*)p.H + (int64_t)(at0 + row(i)) * p.np + column(q);
+        __builtin_memcpy(__builtin_assume_aligned(h, 16), t, sizeof(t));
+      }
+  } else {
+#pragma unroll
+    for (int i = 0; i < S::MT; ++i) {
+      if (row(i) >= rows) continue;
+      const int a = p.order[at0 + row(i)];
       const float w = p.w[a];
-      float* y = p.Y + (int64_t)a * p.n + n;
 #pragma unroll
-      for (int q = 0; q < R; ++q) v[q] *= w;
-      if (n + R <= p.n) {
-        __builtin_memcpy(y, v, sizeof(v));
-      } else {
+      for (int q = 0; q < S::RUNS; ++q) {
+        float v[S::W], b[S::W];
+        load_bias(q, b);
+        run_of<S>(acc[i], q, v);
 #pragma unroll
-        for (int q = 0; q < R; ++q)
-          if (n + q < p.n) y[q] = v[q];
+        for (int c = 0; c < S::W; ++c) v[c] = (v[c] + b[c]) * w;
+        store_run(p.Y + (int64_t)a * p.n + column(q), p.n - column(q), v);
       }
     }
   }
@@ -527,8 +550,8 @@ __global__ __launch_bounds__(256) void combine_kernel(
   }
 }
 
-template <bool FP8>
-using Tile = Shape<FP8, 128, 128, 2, 2, 2>;
+template <bool FP8, bool FIRST>
+using Tile = Shape<FP8, 128, 128, 2, 2, 2, FIRST ? (FP8 ? 16 : 8) : 4>;
 
 template <class S, bool FIRST>
 void run(Experts p, hipStream_t stream) {
@@ -556,7 +579,7 @@ Layout layout(const MoeMlp& m) {
   l.Dp = up(m.D, unit) * unit;
   l.Hp = up(m.H, unit) * unit;
   l.copy = m.fp8 || m.D != l.Dp || m.ldx % 8 || (uintptr_t)m.X % 16 ||
-           (m.T - 1) * m.ldx * 2 + l.Dp * 2 >= (int64_t)NOWHERE;
+           (m.T - 1) * m.ldx * 2 + l.Dp * 2 > UINT32_MAX;
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     const int64_t was = at;
@@ -614,7 +637,7 @@ void run_mlp(const MoeMlp& m, const Layout& l, char* ws, hipStream_t stream) {
   p.act = m.act;
   p.H = ws + l.h;
   p.SH = (float*)(ws + l.sh);
-  run<Tile<FP8>, true>(p, stream);
+  run<Tile<FP8, true>, true>(p, stream);
 
   p.A = (const uint8_t*)ws + l.h;
   p.a_row = (int64_t)l.Hp * size;
@@ -627,7 +650,7 @@ void run_mlp(const MoeMlp& m, const Layout& l, char* ws, hipStream_t stream) {
   p.steps = l.Hp * size / STEP;
   p.w = m.weights;
   p.Y = (float*)(ws + l.y);
-  run<Tile<FP8>, false>(p, stream);
+  run<Tile<FP8, false>, false>(p, stream);
 
   const int64_t work = (int64_t)m.T * ((m.D + 3) / 4);
   hipLaunchKernelGGL(combine_kernel, dim3(up(work, 256)), dim3(256), 0, stream,

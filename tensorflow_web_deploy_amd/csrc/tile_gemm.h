@@ -13,10 +13,12 @@
 // for both types.
 //
 // The operands are swapped (B is the instruction's first operand), so a lane
-// holds one row m and, over its tiles, 4*NT consecutive columns n: the row
-// scale is one value a lane, and the stores are 16 bytes wide without a
-// detour over LDS. The column that row i of tile t stands for is
-//   n = (i / 4) * 4 * NT + t * 4 + i % 4.
+// holds one row m: the row scale is one value a lane. Which columns the rows
+// i of the NT tiles stand for is free. They are dealt so that a lane ends up
+// with runs of W neighbouring columns, 16 bytes of the result's type (W = 16
+// for e4m3, 8 for bf16, 4 for f32), and 4 lanes with 64 bytes of a row: the
+// stores are wide and fill whole segments without a detour over LDS.
+//   n = t / (W/4) * 4W + (i / 4) * W + t % (W/4) * 4 + i % 4
 #pragma once
 #include <hip/hip_runtime.h>
 
@@ -29,19 +31,22 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
-constexpr int STEP = 128;                 // bytes of a row in one K step
-constexpr uint32_t NOWHERE = 0xfffffff0u;  // past every buffer: reads as 0
+constexpr int STEP = 128;  // bytes of a row in one K step
 
-// BM x BN outputs by WM x WN waves; DEPTH stages in LDS, DEPTH-1 in flight
-template <bool FP8_, int BM_, int BN_, int WM_, int WN_, int DEPTH_>
+// BM x BN outputs by WM x WN waves; DEPTH stages in LDS, DEPTH-1 in flight;
+// W neighbouring columns a lane
+template <bool FP8_, int BM_, int BN_, int WM_, int WN_, int DEPTH_, int W_>
 struct Shape {
   static constexpr bool FP8 = FP8_;
+  static constexpr int W = W_;
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, DEPTH = DEPTH_;
   static constexpr int WAVES = WM * WN, THREADS = WAVES * 64;
   static constexpr int MT = BM / WM / 16, NT = BN / WN / 16;  // a wave's tiles
   static constexpr int CA = BM / 8 / WAVES, CB = BN / 8 / WAVES;
   static_assert(CA * 8 * WAVES == BM && CB * 8 * WAVES == BN, "whole loads");
   static_assert(128 % (NT * 16) == 0, "a wave's columns share a scale");
+  static_assert(NT * 4 % W == 0, "whole runs");
+  static constexpr int RUNS = NT * 4 / W;  // of W columns a lane and row
   // the last wave's load of row scales writes past BM: 64 floats of slack
   static constexpr int SCALES = FP8 ? (BM + 64) * 4 : 0;
   static constexpr int STAGE = (BM + BN) * STEP + SCALES;
@@ -57,16 +62,19 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void* p,
 
 template <int BYTES>
 __device__ __forceinline__ void load_lds(__amdgpu_buffer_rsrc_t r, char* to,
-                                         uint32_t at) {
+                                         uint32_t at, uint32_t step_at) {
   const auto lds = (__attribute__((address_space(3))) void*)to;
   if constexpr (BYTES == 16)
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, lds, 16, (int)at, 0, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, lds, 16, (int)at,
+                                             (int)step_at, 0, 0);
   else
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, lds, 4, (int)at, 0, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, lds, 4, (int)at, (int)step_at,
+                                             0, 0);
 }
 
-// The rows that this lane stages: byte offsets of their first value, NOWHERE
-// for a row that isn't there
+// What this lane stages, as byte offsets at step 0: 16 bytes of a row of A or
+// B a load, and one row scale. A row past the tile's end is another, existing
+// row: its products are never stored, so every load stays inside its buffer.
 template <class S>
 struct Rows {
   uint32_t a[S::CA], b[S::CB], s;
@@ -75,16 +83,38 @@ struct Rows {
 // 8 rows of 128 bytes a load: lane / 8 is the row, lane % 8 the LDS slot.
 // Chunk c of row r lies in slot c ^ key(r), so that the 16 rows of a fragment
 // spread over all banks. key: r % 8 for A; for B the same of the fragment's
-// row i, which the column order above puts at bits 0, 1 and log2(4*NT).
+// row i, which the column order above puts at bits 0, 1 and log2(W).
 template <class S>
 __device__ __forceinline__ int key_b(int n) {
-  return (n & 3) | ((n / (4 * S::NT) & 1) << 2);
+  return (n & 3) | ((n / S::W & 1) << 2);
 }
 
-template <class S>
 __device__ __forceinline__ int staged_row(int wave, int count, int i,
                                           int lane) {
   return (wave * count + i) * 8 + (lane >> 3);
+}
+
+// row_a(r), row_b(r), row_s(r): byte offset of row r of the tile, for r below
+// the tile's BM or BN
+template <class S, class A, class B, class C>
+__device__ __forceinline__ Rows<S> rows_of(int wave, int lane, A row_a,
+                                           B row_b, C row_s) {
+  Rows<S> at;
+#pragma unroll
+  for (int i = 0; i < S::CA; ++i) {
+    const int r = staged_row(wave, S::CA, i, lane);
+    at.a[i] = row_a(r) + (((lane & 7) ^ (r & 7)) << 4);
+  }
+#pragma unroll
+  for (int i = 0; i < S::CB; ++i) {
+    const int r = staged_row(wave, S::CB, i, lane);
+    at.b[i] = row_b(r) + (((lane & 7) ^ key_b<S>(r)) << 4);
+  }
+  // wave w brings the scales from row w*BM/WAVES on, 64 of them: where two
+  // waves overlap they write the same values, and what lies behind BM isn't
+  // read
+  at.s = S::FP8 ? row_s(min(wave * (S::BM / S::WAVES) + lane, S::BM - 1)) : 0;
+  return at;
 }
 
 template <class S>
@@ -92,29 +122,40 @@ __device__ __forceinline__ void stage(char* lds, __amdgpu_buffer_rsrc_t ra,
                                       __amdgpu_buffer_rsrc_t rb,
                                       __amdgpu_buffer_rsrc_t rs,
                                       const Rows<S>& at, int step,
-                                      uint32_t s_stride,
-                                      int wave, int lane) {
-  const int slot = lane & 7;
+                                      uint32_t s_stride, int wave) {
 #pragma unroll
-  for (int i = 0; i < S::CA; ++i) {
-    const int r = staged_row<S>(wave, S::CA, i, lane);
-    const uint32_t k = (uint32_t)step * STEP + ((slot ^ (r & 7)) << 4);
-    load_lds<16>(ra, lds + (wave * S::CA + i) * 1024,
-                 at.a[i] == NOWHERE ? NOWHERE : at.a[i] + k);
-  }
-  char* ldsb = lds + S::BM * STEP;
+  for (int i = 0; i < S::CA; ++i)
+    load_lds<16>(ra, lds + (wave * S::CA + i) * 1024, at.a[i], step * STEP);
 #pragma unroll
-  for (int i = 0; i < S::CB; ++i) {
-    const int r = staged_row<S>(wave, S::CB, i, lane);
-    const uint32_t k = (uint32_t)step * STEP + ((slot ^ key_b<S>(r)) << 4);
-    load_lds<16>(rb, ldsb + (wave * S::CB + i) * 1024, at.b[i] + k);
-  }
-  if (S::FP8) {
-    // wave w brings the rows from w*BM/WAVES on, 64 of them: where two waves
-    // overlap they write the same values
-    load_lds<4>(rs, lds + (S::BM + S::BN) * STEP + wave * (S::BM / S::WAVES) * 4,
-                at.s == NOWHERE ? NOWHERE : at.s + (uint32_t)step * s_stride);
-  }
+  for (int i = 0; i < S::CB; ++i)
+    load_lds<16>(rb, lds + S::BM * STEP + (wave * S::CB + i) * 1024, at.b[i],
+                 step * STEP);
+  if (S::FP8)
+    load_lds<4>(rs,
+                lds + (S::BM + S::BN) * STEP + wave * (S::BM / S::WAVES) * 4,
+                at.s, step * s_stride);
+}
+
+template <class S>
+struct FragA {
+  i32x4 v[2];
+  float f;
+};
+
+template <class S>
+__device__ __forceinline__ FragA<S> read_a(const char* lds, int wm, int i,
+                                           int lane) {
+  const int m = wm * S::MT * 16 + i * 16 + (lane & 15), g = lane >> 4;
+  const char* row = lds + m * STEP;
+  FragA<S> a;
+  a.v[0] = *(const i32x4*)(row + ((g ^ (m & 7)) << 4));
+  a.v[1] = *(const i32x4*)(row + (((g + 4) ^ (m & 7)) << 4));
+  a.f = S::FP8 ? *(const float*)(lds + (S::BM + S::BN) * STEP + m * 4) : 0.f;
+  return a;
+}
+
+__device__ __forceinline__ i32x8 both(const i32x4 (&v)[2]) {
+  return __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
 template <class S>
@@ -126,42 +167,56 @@ __device__ __forceinline__ void compute(const char* lds, float sb, int wm,
   i32x4 b[S::NT][2];
 #pragma unroll
   for (int t = 0; t < S::NT; ++t) {
-    const int n = wn * S::NT * 16 + (i16 >> 2) * 4 * S::NT + t * 4 + (i16 & 3);
+    constexpr int Q = S::W / 4;
+    const int n = wn * S::NT * 16 + t / Q * 4 * S::W + (i16 >> 2) * S::W +
+                  t % Q * 4 + (i16 & 3);
     const char* row = ldsb + n * STEP;
     const int key = key_b<S>(n);
     b[t][0] = *(const i32x4*)(row + ((g ^ key) << 4));
     b[t][1] = *(const i32x4*)(row + (((g + 4) ^ key) << 4));
   }
+  if constexpr (S::FP8) {
+    // Three things at a time: rows i + 2 are read, rows i multiplied, and the
+    // products of rows i - 1 scaled and added, 4 additions behind each
+    // matrix instruction, which takes 8 times the time of one. The order is
+    // held, as the compiler's own puts the additions of a step together.
+    FragA<S> a[3];
+    a[0] = read_a<S>(lds, wm, 0, lane);
+    if (S::MT > 1) a[1] = read_a<S>(lds, wm, 1, lane);
+    __builtin_amdgcn_sched_barrier(0);
+    f32x4 p[2][S::NT];
+    float f[2];
 #pragma unroll
-  for (int i = 0; i < S::MT; ++i) {
-    const int m = wm * S::MT * 16 + i * 16 + i16;
-    const char* row = lds + m * STEP;
-    i32x4 a[2];
-    a[0] = *(const i32x4*)(row + ((g ^ (m & 7)) << 4));
-    a[1] = *(const i32x4*)(row + (((g + 4) ^ (m & 7)) << 4));
-    if constexpr (S::FP8) {
-      const float f =
-          *(const float*)(lds + (S::BM + S::BN) * STEP + m * 4) * sb;
-      const i32x8 a8 = __builtin_shufflevector(a[0], a[1], 0, 1, 2, 3, 4, 5,
-                                               6, 7);
+    for (int i = 0; i <= S::MT; ++i) {
+      if (i + 2 < S::MT) a[(i + 2) % 3] = read_a<S>(lds, wm, i + 2, lane);
+      if (i < S::MT) f[i & 1] = a[i % 3].f * sb;
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int t = 0; t < S::NT; ++t) {
-        const i32x8 b8 = __builtin_shufflevector(b[t][0], b[t][1], 0, 1, 2, 3,
-                                                 4, 5, 6, 7);
-        const f32x4 p = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-            b8, a8, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+        if (i < S::MT)
+          p[i & 1][t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+              both(b[t]), both(a[i % 3].v), f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0,
+              0, 0, 0);
+        if (i > 0)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          acc[i][t][r] = __builtin_fmaf(p[r], f, acc[i][t][r]);
+          for (int r = 0; r < 4; ++r)
+            acc[i - 1][t][r] = __builtin_fmaf(p[(i - 1) & 1][t][r],
+                                              f[(i - 1) & 1],
+                                              acc[i - 1][t][r]);
+        __builtin_amdgcn_sched_barrier(0);
       }
-    } else {
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < S::MT; ++i) {
+      const FragA<S> a = read_a<S>(lds, wm, i, lane);
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int t = 0; t < S::NT; ++t)
           acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
               __builtin_bit_cast(bf16x8, b[t][h]),
-              __builtin_bit_cast(bf16x8, a[h]), acc[i][t], 0, 0, 0);
+              __builtin_bit_cast(bf16x8, a.v[h]), acc[i][t], 0, 0, 0);
     }
   }
 }
@@ -187,7 +242,12 @@ __device__ __forceinline__ void product(char* smem, __amdgpu_buffer_rsrc_t ra,
   for (int j = 0; j < AHEAD; ++j)
     if (j < count)
       stage<S>(smem + j * S::STAGE, ra, rb, rs, at, first + j,
-                     s_stride, wave, lane);
+                     s_stride, wave);
+  // constant memory, so that the scale comes by a scalar load: a vector load
+  // here would wait for every stage that is on its way
+  const auto sbc =
+      (const __attribute__((address_space(4))) float*)(uintptr_t)sb;
+  float fb = S::FP8 && count > 0 ? sbc[first] : 0.f;
   int now = 0, next = AHEAD % S::DEPTH;
   for (int j = 0; j < count; ++j) {
     // step j has landed once only the later ones are still on their way
@@ -199,17 +259,71 @@ __device__ __forceinline__ void product(char* smem, __amdgpu_buffer_rsrc_t ra,
     else
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
+    asm volatile("" ::"s"(fb) : "memory");  // here, not among the LDS reads
     if (j + AHEAD < count)
       stage<S>(smem + next * S::STAGE, ra, rb, rs, at, first + j + AHEAD,
-                     s_stride, wave, lane);
-    compute<S>(smem + now * S::STAGE, S::FP8 ? sb[first + j] : 0.f, wm, wn,
-               lane, acc);
+                     s_stride, wave);
+    compute<S>(smem + now * S::STAGE, fb, wm, wn, lane, acc);
     // the stage is free for the load behind the next barrier
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (S::FP8) fb = sbc[first + min(j + 1, count - 1)];
     now = now + 1 == S::DEPTH ? 0 : now + 1;
     next = next + 1 == S::DEPTH ? 0 : next + 1;
   }
+}
+
+// Run q of a lane's columns in row tile i: v[c] is column
+//   run_column(q) + c,  counted from the wave's first one.
+template <class S>
+__device__ __forceinline__ int run_column(int q, int lane) {
+  return q * 4 * S::W + (lane >> 4) * S::W;
+}
+
+template <class S>
+__device__ __forceinline__ void run_of(const f32x4 (&acc)[S::NT], int q,
+                                       float (&v)[S::W]) {
+#pragma unroll
+  for (int c = 0; c < S::W; ++c) v[c] = acc[q * (S::W / 4) + c / 4][c % 4];
+}
+
+// R numbers from p on that the caller knows to be there, or those below
+// `have` and 0 for the rest
+template <int R>
+__device__ __forceinline__ void load_run(const float* p, int have,
+                                         float (&v)[R]) {
+  if (have >= R) {
+    __builtin_memcpy(v, p, sizeof(v));
+  } else {
+#pragma unroll
+    for (int c = 0; c < R; ++c) v[c] = c < have ? p[c] : 0.f;
+  }
+}
+
+template <int R>
+__device__ __forceinline__ void store_run(float* p, int have,
+                                          const float (&v)[R]) {
+  if (have >= R) {
+    __builtin_memcpy(p, v, sizeof(v));
+  } else {
+#pragma unroll
+    for (int c = 0; c < R; ++c)
+      if (c < have) p[c] = v[c];
+  }
+}
+
+// v Phi(v), the erf-GELU. The normal distribution's tail beyond |v| is
+// Abramowitz and Stegun's 7.1.26, 1/2 t (a1 + .. + a5 t^4) exp(-v^2 / 2) with
+// t = 1 / (1 + p |v| / sqrt 2): off by less than 1e-7, in 13 operations. With
+// erff the activation alone took a quarter of a large product's time.
+__device__ __forceinline__ float gelu(float v) {
+  const float t = __builtin_amdgcn_rcpf(
+      __builtin_fmaf(0.3275911f * 0.70710678f, fabsf(v), 1.f));
+  float h = __builtin_fmaf(0.5f * 1.061405429f, t, 0.5f * -1.453152027f);
+  h = __builtin_fmaf(h, t, 0.5f * 1.421413741f);
+  h = __builtin_fmaf(h, t, 0.5f * -0.284496736f);
+  h = __builtin_fmaf(h, t, 0.5f * 0.254829592f);
+  h *= t * __builtin_amdgcn_exp2f(v * v * -0.72134752f);  // log2(e) / 2
+  return v * (v < 0.f ? h : 1.f - h);
 }
 
 // 0 none, 1 relu, 2 relu6, 5 erf-GELU: the codes of the bf16 GEMM
@@ -217,7 +331,7 @@ template <int ACT>
 __device__ __forceinline__ float activate(float v) {
   if (ACT == 1) return v < 0.f ? 0.f : v;
   if (ACT == 2) return v < 0.f ? 0.f : v > 6.f ? 6.f : v;
-  if (ACT == 5) return 0.5f * v * (1.f + erff(v * 0.70710678f));
+  if (ACT == 5) return gelu(v);
   return v;
 }
 
@@ -238,10 +352,22 @@ __device__ __forceinline__ void activate_by(float (&v)[R], int act) {
 }
 
 // Workgroups go round the 8 XCDs in turn. Give each XCD a contiguous run of
-// tiles, so that neighbours share their rows of A and B in its L2.
-__device__ __forceinline__ int by_xcd(int bid, int n) {
+// tiles, and let the run go down HIGH rows of tiles before it moves a column
+// on: what an XCD holds at once then shares both its rows and its columns in
+// the XCD's L2.
+struct Place {
+  int m, n;
+};
+
+constexpr int HIGH = 8;
+
+__device__ __forceinline__ Place place_of(int bid, int tiles_m, int tiles_n) {
+  const int n = tiles_m * tiles_n;
   const int q = n >> 3, r = n & 7, xcd = bid & 7, off = bid >> 3;
-  return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + off;
+  const int i = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + off;
+  const int band = i / (HIGH * tiles_n), in = i - band * HIGH * tiles_n;
+  const int rows = min(HIGH, tiles_m - band * HIGH);
+  return {band * HIGH + in % rows, in / rows};
 }
 
 }  // namespace tile
