@@ -11,6 +11,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "kernels.h"
 #include "quant_fp8.h"
@@ -35,193 +36,492 @@ struct Route {
   float scale;
 };
 
-__device__ __forceinline__ float exp_of(float v) { return expf(v); }
-__device__ __forceinline__ double exp_of(double v) { return exp(v); }
+// How far the f32 score p and key = p + bias may be off. exp's argument d is
+// rounded three times, which moves exp by 3 * 2^-24 |d| of itself. Softmax:
+// |d| is no more than |ln p|; the sum of up to 512 terms in 32 + 4 steps, the
+// terms' own errors in it, exp and the quotient stay within 64 * 2^-24.
+// Sigmoid: exp counts by 1 - p, |d| (1 - p) is less than |ln p| + 1, and 8
+// roundings cover the rest. Adding the bias rounds the key.
+__device__ __forceinline__ float error_of(float p, float key, bool sigmoid) {
+  const float d = fabsf(__builtin_amdgcn_logf(fmaxf(p, 1e-37f)));  // log2
+  return 0x1p-24f * ((sigmoid ? 8.f : 64.f) + 2.1f * d) * p +
+         0x1p-23f * fabsf(key) + 1e-37f;
+}
 
-template <typename R>
-__device__ __forceinline__ R wave_max(R v) {
-#pragma unroll
-  for (int d = 32; d; d >>= 1) {
-    const R o = __shfl_xor(v, d);
-    v = o > v ? o : v;
+// The largest value, the sum, .. of 16 neighbouring lanes, in all of them
+template <int ROR>
+__device__ __forceinline__ float turned(float v) {
+  static_assert(ROR > 0 && ROR < 16);
+  return __builtin_bit_cast(
+      float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v),
+                                         0x120 + ROR, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float max16(float v) {
+  v = fmaxf(v, turned<8>(v));
+  v = fmaxf(v, turned<4>(v));
+  v = fmaxf(v, turned<2>(v));
+  return fmaxf(v, turned<1>(v));
+}
+__device__ __forceinline__ float sum16(float v) {
+  v += turned<8>(v);
+  v += turned<4>(v);
+  v += turned<2>(v);
+  return v + turned<1>(v);
+}
+
+// what the lanes before this one of its 16 add up to
+template <int SHR>
+__device__ __forceinline__ int shifted(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, 0x110 + SHR, 0xf, 0xf, true);
+}
+__device__ __forceinline__ int before16(int v) {
+  int s = v + shifted<1>(v);
+  s += shifted<2>(s);
+  s += shifted<4>(s);
+  s += shifted<8>(s);
+  return s - v;
+}
+
+// how many of the other 15 lanes hold a larger number
+template <int R = 1>
+__device__ __forceinline__ int above16(float v) {
+  if constexpr (R == 16)
+    return 0;
+  else
+    return (turned<R>(v) > v) + above16<R + 1>(v);
+}
+
+// how many of the 16 lanes' (o, oid) come before (v, id): a larger number, or
+// the same one with a smaller id
+template <int R = 0>
+__device__ __forceinline__ int rank16(float v, float id, float o, float oid) {
+  if constexpr (R == 16) {
+    return 0;
+  } else {
+    float u = o, uid = oid;
+    if constexpr (R > 0) u = turned<R>(o), uid = turned<R>(oid);
+    return (u > v || (u == v && uid < id)) + rank16<R + 1>(v, id, o, oid);
   }
-  return v;
 }
 
-template <typename R>
-__device__ __forceinline__ R wave_sum(R v) {
+// The largest of a wave's numbers, one that is uniform over the wave
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double moved(double v) {
+  const int2 u = __builtin_bit_cast(int2, v);
+  return __builtin_bit_cast(
+      double, make_int2(__builtin_amdgcn_update_dpp(u.x, u.x, CTRL, ROWS, 0xf,
+                                                    false),
+                        __builtin_amdgcn_update_dpp(u.y, u.y, CTRL, ROWS, 0xf,
+                                                    false)));
+}
+__device__ __forceinline__ double lane_of(double v, int lane) {
+  const int2 u = __builtin_bit_cast(int2, v);
+  return __builtin_bit_cast(
+      double, make_int2(__builtin_amdgcn_readlane(u.x, lane),
+                        __builtin_amdgcn_readlane(u.y, lane)));
+}
+__device__ __forceinline__ double wave_max(double v) {
+  v = fmax(v, moved<0x128, 0xf>(v));  // within rows of 16: row_ror 8, 4, 2, 1
+  v = fmax(v, moved<0x124, 0xf>(v));
+  v = fmax(v, moved<0x122, 0xf>(v));
+  v = fmax(v, moved<0x121, 0xf>(v));
+  return fmax(fmax(lane_of(v, 0), lane_of(v, 16)),
+              fmax(lane_of(v, 32), lane_of(v, 48)));
+}
+
+// One row by one wave in 64 bits, lane l with the experts l + 64 v
+template <typename T, int V>
+__device__ __forceinline__ void route_exactly(const Route& p, int64_t t,
+                                              double* lds, int lane) {
+  const double NONE = -INFINITY;
+  float x[V];
+  double s[V], key[V];
+  float top = -INFINITY;
 #pragma unroll
-  for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
-  return v;
-}
-
-// How far the f32 score p and key = p + bias may be off: exp's argument is at
-// most 104 wide where p isn't 0, its rounding and those of exp, sum, division
-// and addition stay within 128 * 2^-24 of p and 2^-23 of the key.
-__device__ __forceinline__ float error_of(float p, float key) {
-  return 0x1p-17f * p + 0x1p-23f * fabsf(key) + 1e-37f;
-}
-
-// One row by one wave, lane l with the experts l + 64 v. With R = float it
-// answers whether every decision is safe from rounding; if not, nothing has
-// been written and the row is done again with R = double. Which experts are
-// chosen, and their order, is so that of the scores in 64 bits, the lower
-// index first among equals.
-template <typename R, int V>
-__device__ bool route_row(const Route& p, int64_t t, const float (&x)[V],
-                          const float (&b)[V], R* lds, int lane) {
-  constexpr bool FAST = sizeof(R) == 4;
-  const R NONE = -(R)INFINITY;
-  R s[V], key[V];
+  for (int v = 0; v < V; ++v) {
+    const int e = v * 64 + lane;
+    x[v] = e < p.E ? (float)((const T*)p.x)[t * p.ldx + e] : -INFINITY;
+    if (!(x[v] > -INFINITY)) x[v] = -INFINITY;
+    top = fmaxf(top, x[v]);
+  }
   if (p.sigmoid) {
 #pragma unroll
     for (int v = 0; v < V; ++v)
-      s[v] = x[v] > -INFINITY ? 1 / (1 + exp_of(-(R)x[v])) : 0;
+      s[v] = x[v] > -INFINITY ? 1 / (1 + exp(-(double)x[v])) : 0;
   } else {
-    float top = x[0];
-#pragma unroll
-    for (int v = 1; v < V; ++v) top = fmaxf(top, x[v]);
-    top = wave_max(top);
-    R sum = 0;
+    top = (float)wave_max((double)top);
+    double sum = 0;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       // an infinite logit leaves nothing to the finite ones
-      s[v] = x[v] == top ? (R)1 : exp_of((R)x[v] - (R)top);
+      s[v] = x[v] == top ? 1 : exp((double)x[v] - (double)top);
       if (!(x[v] > -INFINITY)) s[v] = 0;
       sum += s[v];
     }
-    sum = wave_sum(sum);
+#pragma unroll
+    for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
 #pragma unroll
     for (int v = 0; v < V; ++v) s[v] = sum > 0 ? s[v] / sum : 0;
   }
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    key[v] = s[v] + (R)b[v];
+    const int e = v * 64 + lane;
+    key[v] = s[v] + (e < p.E && p.bias ? (double)p.bias[e] : 0);
     if (!(x[v] > -INFINITY) || !(key[v] > NONE)) key[v] = NONE;
+  }
+  if (p.groups > 1) {
+    const int size = p.E / p.groups;
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (v * 64 + lane < p.E) lds[v * 64 + lane] = key[v];
+    __builtin_amdgcn_wave_barrier();
+    double first = NONE, second = NONE;
+    if (lane < p.groups) {
+#pragma unroll 4
+      for (int i = 0; i < size; ++i) {
+        const double y = lds[lane * size + i];
+        second = fmax(second, fmin(first, y));
+        first = fmax(first, y);
+      }
+    }
+    const double total =
+        p.best == 2 && second > NONE ? first + second : first;
+    int rank = 0;
+    for (int g = 0; g < p.groups; ++g) {
+      const double o = lane_of(total, g);
+      rank += o > total || (o == total && g < lane);
+    }
+    const uint64_t kept = __ballot(lane < p.groups && rank < p.kept);
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (!(kept >> ((v * 64 + lane) / size & 63) & 1)) key[v] = NONE;
+  }
+  double mine = 0, sum = 0;
+  int id = -1;
+  for (int j = 0; j < p.k; ++j) {
+    double best = key[0];
+#pragma unroll
+    for (int v = 1; v < V; ++v) best = fmax(best, key[v]);
+    best = wave_max(best);
+    if (!(best > NONE)) break;
+    double sv = 0;
+    bool found = false;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const uint64_t has = __ballot(key[v] == best);
+      if (found || !has) continue;
+      found = true;
+      const int at = __builtin_ctzll(has);
+      sv = lane_of(s[v], at);
+      if (lane == at) key[v] = NONE;
+      if (lane == j) mine = sv, id = v * 64 + at;
+    }
+    sum += sv;
+  }
+  if (lane < p.k) {
+    if (p.renorm) mine = sum > 0 ? mine / sum : 0;
+    p.ids[t * p.k + lane] = id;
+    p.weights[t * p.k + lane] = (float)(mine * p.scale);
+  }
+}
+
+// LDS of one row in f32: the scores, the keys (with groups), what the groups
+// come to and the size of its parts, and the chosen ones
+struct RouteLds {
+  int p, key, total, round, list, floats;
+  __host__ __device__ RouteLds(int V, int groups, int k) {
+    p = 0;
+    key = 16 * V;
+    total = key + (groups > 1 ? 16 * V : 0);
+    round = total + (groups > 1 ? groups : 0);
+    list = (round + (groups > 1 ? groups : 0) + 1) & ~1;
+    floats = (list + 2 * (k < 16 ? 32 : k + 1) + 3) & ~3;
+  }
+};
+
+// Expert of a lane's place v: runs of 4 neighbours a lane (V >= 4), 64 a turn,
+// so that each lane has some of every group of experts that is wide
+template <int V>
+__device__ __forceinline__ int expert_at(int l, int v) {
+  return V >= 4 ? v / 4 * 64 + l * 4 + v % 4 : l;
+}
+
+// 16 lanes a row, 4 rows a wave: the steps across lanes stay within rows of the register file, and one
+// instruction serves 4 rows. Everything is decided in f32; a row where
+// rounding could change what is chosen or its order, or whose scores leave
+// the range of f32, is then done again in 64 bits, so that the choice is that
+// of the scores in 64 bits, the lower index first among equals. That is one
+// row in some hundreds, unless logits repeat a lot.
+template <typename T, int V>
+__global__ __launch_bounds__(256) void route_kernel(Route p) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const float NONE = -INFINITY;
+  const RouteLds at(V, p.groups, p.k);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int l = lane & 15;
+  const int64_t t0 = ((int64_t)blockIdx.x * 4 + wave) * 4;
+  if (t0 >= p.T) return;
+  const int64_t t = t0 + (lane >> 4);
+  float* wave_lds = (float*)smem + wave * 4 * at.floats;
+  float* lds = wave_lds + (lane >> 4) * at.floats;
+  constexpr int RUN = V >= 4 ? 4 : 1;
+  const int E = t < p.T ? p.E : 0;
+
+  float s[V], key[V];
+#pragma unroll
+  for (int v = 0; v < V; v += RUN) {
+    const int e = expert_at<V>(l, v);
+    const T* x = (const T*)p.x + (t < p.T ? t : t0) * p.ldx + e;
+    if (e + RUN <= E) {
+      T u[RUN];
+      __builtin_memcpy(u, x, sizeof(u));
+#pragma unroll
+      for (int i = 0; i < RUN; ++i) key[v + i] = (float)u[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < RUN; ++i)
+        key[v + i] = e + i < E ? (float)x[i] : NONE;
+    }
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v)
+    if (!(key[v] > NONE)) key[v] = NONE;  // NaN: not to be chosen
+  auto to_lds = [&](int where, const float(&y)[V]) {
+#pragma unroll
+    for (int v = 0; v < V; v += RUN)
+      __builtin_memcpy(__builtin_assume_aligned(
+                           lds + where + expert_at<V>(l, v), RUN * 4),
+                       y + v, RUN * 4);
+  };
+  constexpr float LOG2E = 1.44269504f;
+  float most = 1.f;  // no score is larger
+  if (p.sigmoid) {
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      s[v] = __builtin_amdgcn_rcpf(
+          1.f + __builtin_amdgcn_exp2f(key[v] * -LOG2E));
+  } else {
+    float top = key[0], sum = 0;
+#pragma unroll
+    for (int v = 1; v < V; ++v) top = fmaxf(top, key[v]);
+    top = max16(top);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      // an infinite logit leaves nothing to the finite ones
+      s[v] = key[v] == top ? 1.f
+                           : __builtin_amdgcn_exp2f((key[v] - top) * LOG2E);
+      if (!(key[v] > NONE)) s[v] = 0.f;
+      sum += s[v];
+    }
+    sum = 1.f / sum16(sum);
+    most = fminf(sum, 1.f);
+#pragma unroll
+    for (int v = 0; v < V; ++v) s[v] = key[v] > NONE ? s[v] * sum : 0.f;
+  }
+  to_lds(at.p, s);
+  if (p.bias) {
+#pragma unroll
+    for (int v = 0; v < V; v += RUN) {
+      const int e = expert_at<V>(l, v);
+      float b[RUN];
+      load_run(p.bias + e, E - e, b);
+#pragma unroll
+      for (int i = 0; i < RUN; ++i) {
+        const float y = s[v + i] + b[i];
+        key[v + i] = key[v + i] > NONE && y > NONE ? y : NONE;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v) key[v] = key[v] > NONE ? s[v] : NONE;
   }
   bool safe = true;
 
   if (p.groups > 1) {
     const int size = p.E / p.groups;
+    to_lds(at.key, key);
     __builtin_amdgcn_wave_barrier();
+    // no group's sum is off by more than two of the largest score could be
+    const float err = 2 * error_of(most, 0.f, p.sigmoid);
 #pragma unroll
-    for (int v = 0; v < V; ++v)
-      if (v * 64 + lane < p.E) {
-        lds[v * 64 + lane] = key[v];
-        if (FAST) lds[p.E + v * 64 + lane] = error_of(s[v], key[v]);
-      }
-    __builtin_amdgcn_wave_barrier();
-    R first = NONE, second = NONE;
-    float e1 = 0, e2 = 0;
-    if (lane < p.groups)
-      for (int i = 0; i < size; ++i) {
-        const R y = lds[lane * size + i];
-        const float e = FAST ? (float)lds[p.E + lane * size + i] : 0.f;
-        if (y > first) {
-          second = first, e2 = e1;
-          first = y, e1 = e;
-        } else if (y > second) {
-          second = y, e2 = e;
+    for (int q = 0; q < 4; ++q) {
+      const int g = q * 16 + l;
+      if (g >= p.groups) break;
+      float first = NONE, second = NONE;
+      auto see = [&](float y) {
+        second = fmaxf(second, fminf(first, y));
+        first = fmaxf(first, y);
+      };
+      const float* in = lds + at.key + g * size;
+      if (V >= 4 && size % 4 == 0) {
+        int j = l * 4 % size;  // spread over banks
+#pragma unroll 4
+        for (int i = 0; i < size; i += 4) {
+          f32x4 y;
+          __builtin_memcpy(&y, __builtin_assume_aligned(in + j, 16), 16);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) see(y[u]);
+          j = j + 4 == size ? 0 : j + 4;
+        }
+      } else {
+        int j = l % size;
+#pragma unroll 4
+        for (int i = 0; i < size; ++i) {
+          see(in[j]);
+          j = j + 1 == size ? 0 : j + 1;
         }
       }
-    R total = first;
-    if (p.best == 2 && second > NONE) total += second, e1 += e2;
-    e1 += 0x1p-23f * fabsf((float)total);
-    int rank = 0;
-    for (int g = 0; g < p.groups; ++g) {
-      const R o = __shfl(total, g);
-      rank += o > total || (o == total && g < lane);
+      lds[at.total + g] = p.best == 2 && second > NONE ? first + second : first;
+      lds[at.round + g] =
+          fabsf(first) + (second > NONE ? fabsf(second) : 0.f);
     }
-    const bool keep = lane < p.groups && rank < p.kept;
-    const uint64_t kept = __ballot(keep);
-    if (FAST) {
-      // the last group that is kept against the first that isn't
-      float low = keep ? (float)total - e1 : INFINITY;
-      float high = lane < p.groups && !keep && total > NONE
-                       ? (float)total + e1 : -INFINITY;
-      low = -wave_max(-low);
-      high = wave_max(high);
-      safe = !(low <= high);
-    }
+    __builtin_amdgcn_wave_barrier();
+    float low = INFINITY, high = NONE;
+    uint64_t kept = 0;
 #pragma unroll
-    for (int v = 0; v < V; ++v)
-      if (!(kept >> ((v * 64 + lane) / size & 63) & 1)) key[v] = NONE;
-  }
-
-  // k times the largest key, and once more for the one that just fails
-  R mine = 0, sum = 0, last_key = 0;
-  int id = -1;
-  float last_e = 0, last_x = 0, last_b = 0;
-  for (int j = 0; j <= p.k; ++j) {
-    R y = key[0];
-    int at = lane, v_at = 0;
-#pragma unroll
-    for (int v = 1; v < V; ++v)
-      if (key[v] > y) y = key[v], at = v * 64 + lane, v_at = v;
-    R top = y;
-    int e = at;
-#pragma unroll
-    for (int d = 32; d; d >>= 1) {
-      const R o = __shfl_xor(top, d);
-      const int oe = __shfl_xor(e, d);
-      if (o > top || (o == top && oe < e)) top = o, e = oe;
-    }
-    if (!(top > NONE)) break;
-    // what the chosen one's lane holds of it
-    R sv = 0;
-    float xv = 0, bv = 0;
-#pragma unroll
-    for (int v = 0; v < V; ++v)
-      if (v == v_at) {
-        sv = s[v], xv = x[v], bv = b[v];
-        if (at == e) key[v] = NONE;
+    for (int q = 0; q < 4; ++q) {
+      const int g = q * 16 + l;
+      if (q * 16 >= p.groups) break;
+      bool keep = false;
+      if (g < p.groups) {
+        const float total = lds[at.total + g];
+        int rank = 0;
+#pragma unroll 8
+        for (int h = 0; h < p.groups; ++h) {
+          const float o = lds[at.total + h];
+          rank += o > total || (o == total && h < g);
+        }
+        keep = rank < p.kept;
+        // the last group that is kept against the first that isn't; one
+        // without any expert left doesn't matter
+        const float e = err + 0x1p-22f * lds[at.round + g];
+        if (total > NONE) {
+          if (keep)
+            low = fminf(low, total - e);
+          else
+            high = fmaxf(high, total + e);
+        }
       }
-    sv = __shfl(sv, e & 63);
-    if (FAST) {
-      xv = __shfl(xv, e & 63), bv = __shfl(bv, e & 63);
-      const float err = error_of((float)sv, (float)top);
-      // equal logits and biases tie in any precision
-      if (j && !(last_key - top > last_e + err) &&
-          !(xv == last_x && bv == last_b))
-        safe = false;
-      last_key = top, last_e = err, last_x = xv, last_b = bv;
+      kept |= (__ballot(keep) >> (lane & 48) & 0xffff) << (16 * q);
     }
-    if (j == p.k) break;
-    if (lane == j) mine = sv, id = e;
-    sum += sv;
-  }
-  // scores that leave the range of f32 still have their ratios
-  if (FAST && p.renorm && __shfl(id, 0) >= 0 && !(sum > (R)1e-30f))
-    safe = false;
-  if (FAST && !safe) return false;
-  if (lane < p.k) {
-    R w = mine;
-    if (p.renorm) w = sum > 0 ? w / sum : 0;
-    p.ids[t * p.k + lane] = id;
-    p.weights[t * p.k + lane] = (float)(w * (R)p.scale);
-  }
-  return true;
-}
-
-// 4 rows a workgroup, a wave each
-template <typename T, int V>
-__global__ __launch_bounds__(256) void route_kernel(Route p) {
-  extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t t = (int64_t)blockIdx.x * 4 + wave;
-  if (t >= p.T) return;
-  float x[V], b[V];
+    safe = !(-max16(-low) <= max16(high));
+    const uint32_t over = (1u << 20) / size + 1;  // e / size for e < 512
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const int e = v * 64 + lane;
-    const bool in = e < p.E;
-    x[v] = in ? (float)((const T*)p.x)[t * p.ldx + e] : -INFINITY;
-    if (!(x[v] > -INFINITY)) x[v] = -INFINITY;  // NaN: not to be chosen
-    b[v] = in && p.bias ? p.bias[e] : 0.f;
+    for (int v = 0; v < V; ++v)
+      if (!(kept >> (min(expert_at<V>(l, v), p.E - 1) * over >> 20) & 1))
+        key[v] = NONE;
   }
-  double* lds = (double*)smem + wave * p.E;
-  if (!route_row<float, V>(p, t, x, b, (float*)lds, lane))
-    route_row<double, V>(p, t, x, b, lds, lane);
+
+  // The k largest keys, and the one that just fails, into a list. Each lane's
+  // own largest key counts: where k + 1 lanes reach a bound, no key below it
+  // can be wanted. For 8 of 256 that leaves some 13 keys; with up to 32, two a
+  // lane, each finds its place by itself.
+  int2* list = (int2*)(lds + at.list);
+  bool few = p.k < 16;
+  if (few) {
+    float own = key[0];
+#pragma unroll
+    for (int v = 1; v < V; ++v) own = fmaxf(own, key[v]);
+    const float bound =
+        -max16(above16(own) <= p.k ? -own : NONE);
+    int count = 0;
+#pragma unroll
+    for (int v = 0; v < V; ++v) count += key[v] >= bound && key[v] > NONE;
+    int to = before16(count);
+    few = !__any(to + count > 32);
+    const bool two = __any(to + count > 16);
+    if (few) {
+      const int2 none = make_int2(-1, __builtin_bit_cast(int, NONE));
+      list[l] = none;
+      if (two) list[l + 16] = none;
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        if (key[v] >= bound && key[v] > NONE)
+          list[to++] = make_int2(expert_at<V>(l, v),
+                                 __builtin_bit_cast(int, key[v]));
+      __builtin_amdgcn_wave_barrier();
+      // places that hold nothing come last, each at its own
+      const int2 a = list[l];
+      const float ka = __builtin_bit_cast(float, a.y);
+      const float ia = a.x < 0 ? 1024.f + l : (float)a.x;
+      int rank = rank16(ka, ia, ka, ia);
+      if (two) {
+        const int2 b = list[l + 16];
+        const float kb = __builtin_bit_cast(float, b.y);
+        const float ib = b.x < 0 ? 1040.f + l : (float)b.x;
+        rank += rank16(ka, ia, kb, ib);
+        const int other = rank16(kb, ib, kb, ib) + rank16(kb, ib, ka, ia);
+        __builtin_amdgcn_wave_barrier();
+        list[other] = b;
+      }
+      __builtin_amdgcn_wave_barrier();
+      list[rank] = a;
+    }
+  }
+  // else k times the largest key, and once more
+  for (int j = 0; j <= p.k && !few; ++j) {
+    float top = key[0];
+#pragma unroll
+    for (int v = 1; v < V; ++v) top = fmaxf(top, key[v]);
+    top = max16(top);
+    // the smallest index that has it
+    int id = 1024;
+#pragma unroll
+    for (int v = V - 1; v >= 0; --v)
+      if (key[v] == top) id = expert_at<V>(l, v);
+    id = (int)-max16(-(float)id);
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (expert_at<V>(l, v) == id) key[v] = NONE;
+    if (l == 0)
+      list[j] = make_int2(top > NONE ? id : -1, __builtin_bit_cast(int, top));
+  }
+  __builtin_amdgcn_wave_barrier();
+
+  float w[4], sum = 0.f;
+  int id[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int j = q * 16 + l;
+    id[q] = -1, w[q] = 0.f;
+    if (j >= p.k) continue;
+    const int2 a = list[j], b = list[j + 1];
+    id[q] = a.x;
+    if (a.x < 0) continue;
+    w[q] = lds[at.p + a.x];
+    sum += w[q];
+    if (b.x < 0) continue;
+    const float ka = __builtin_bit_cast(float, a.y);
+    const float kb = __builtin_bit_cast(float, b.y);
+    if (!(ka - kb > error_of(w[q], ka, p.sigmoid) +
+                        error_of(lds[at.p + b.x], kb, p.sigmoid))) {
+      // equal logits and biases tie in any precision
+      const T* x = (const T*)p.x + t * p.ldx;
+      if (!((float)x[a.x] == (float)x[b.x] &&
+            (!p.bias || p.bias[a.x] == p.bias[b.x])))
+        safe = false;
+    }
+  }
+  sum = sum16(sum);
+  if (p.renorm && id[0] >= 0 && !(sum > 1e-30f)) safe = false;
+  const uint64_t unsafe = __ballot(!safe);
+  const bool again = unsafe >> (lane & 48) & 0xffff;
+  const float scale = p.renorm ? (sum > 0.f ? p.scale / sum : 0.f) : p.scale;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int j = q * 16 + l;
+    if (j >= p.k || t >= p.T || again) continue;
+    p.ids[t * p.k + j] = id[q];
+    p.weights[t * p.k + j] = w[q] * scale;
+  }
+  if (!unsafe) return;
+  // the rows of the wave are done with LDS: it now holds numbers of 64 bits
+  __builtin_amdgcn_wave_barrier();
+  asm volatile("" ::: "memory");
+  for (int r = 0; r < 4; ++r)
+    if (unsafe >> (16 * r) & 0xffff)
+      route_exactly<T, (V + 3) / 4>(p, t0 + r, (double*)wave_lds, lane);
 }
 
 // ----------------------------------------------------------------- plan
@@ -666,23 +966,29 @@ void launch_moe_route(const void* X, bool f32, int64_t ldx, const float* bias,
                       bool renorm, float scale, hipStream_t stream) {
   const Route p{X, bias, ids, weights, ldx, T, E, k, groups, kept, best,
                 sigmoid, renorm, scale};
-  const dim3 grid(up(T, 4));
-  const int lds = 4 * E * 8;
-  auto go = [&](auto x) {
-    using V = decltype(x);
-    if (E <= 64)
-      hipLaunchKernelGGL((route_kernel<V, 1>), grid, dim3(256), lds, stream, p);
-    else if (E <= 128)
-      hipLaunchKernelGGL((route_kernel<V, 2>), grid, dim3(256), lds, stream, p);
-    else if (E <= 256)
-      hipLaunchKernelGGL((route_kernel<V, 4>), grid, dim3(256), lds, stream, p);
-    else
-      hipLaunchKernelGGL((route_kernel<V, 8>), grid, dim3(256), lds, stream, p);
+  const dim3 grid(up(T, 16));
+  auto go = [&](auto x, auto v) {
+    using X_ = decltype(x);
+    constexpr int V = decltype(v)::value;
+    const int lds = RouteLds(V, groups, k).floats * 16 * 4;
+    hipLaunchKernelGGL((route_kernel<X_, V>), grid, dim3(256), lds, stream, p);
   };
-  if (f32)
-    go(0.f);
+  auto by_type = [&](auto v) {
+    if (f32)
+      go(0.f, v);
+    else
+      go((__bf16)0.f, v);
+  };
+  if (E <= 16)
+    by_type(std::integral_constant<int, 1>());
+  else if (E <= 64)
+    by_type(std::integral_constant<int, 4>());
+  else if (E <= 128)
+    by_type(std::integral_constant<int, 8>());
+  else if (E <= 256)
+    by_type(std::integral_constant<int, 16>());
   else
-    go((__bf16)0.f);
+    by_type(std::integral_constant<int, 32>());
 }
 
 int64_t moe_mlp_workspace(const MoeMlp& m) { return layout(m).bytes; }
