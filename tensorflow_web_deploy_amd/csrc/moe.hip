@@ -526,28 +526,43 @@ __global__ __launch_bounds__(256) void route_kernel(Route p) {
 
 // ----------------------------------------------------------------- plan
 
-constexpr int PLAN_THREADS = 256, PLAN_ROWS = 4096;
+constexpr int PLAN_THREADS = 256, PLAN_EACH = 8;
+constexpr int PLAN_ROWS = PLAN_THREADS * PLAN_EACH;
 
 struct Plan {
   const int* ids;
   int* counts;  // [blocks][E]: how many of a block's rows go to an expert
   int* order;   // [N]: the assignments, by expert; behind them nothing
-  int4* tiles;  // {expert, first place in order, rows, 0}; expert -1: none
+  int4* tiles;  // {expert, first place in order, rows, 0}; [n_tiles].x: how
+                // many there are
   int N, E, BM, n_tiles, blocks;
 };
 
+// the experts of the PLAN_EACH rows of a thread; one that isn't there is E
+__device__ __forceinline__ void load_ids(const Plan& p, int a0,
+                                         int (&e)[PLAN_EACH]) {
+#pragma unroll
+  for (int i = 0; i < PLAN_EACH; ++i) {
+    const int a = a0 + i * PLAN_THREADS + threadIdx.x;
+    e[i] = a < p.N ? p.ids[a] : p.E;
+  }
+#pragma unroll
+  for (int i = 0; i < PLAN_EACH; ++i)
+    if ((unsigned)e[i] >= (unsigned)p.E) e[i] = p.E;
+}
+
 __global__ __launch_bounds__(PLAN_THREADS) void plan_count_kernel(Plan p) {
   extern __shared__ int count[];
-  for (int e = threadIdx.x; e < p.E; e += PLAN_THREADS) count[e] = 0;
+  int e[PLAN_EACH];
+  load_ids(p, blockIdx.x * PLAN_ROWS, e);
+  for (int i = threadIdx.x; i < p.E; i += PLAN_THREADS) count[i] = 0;
   __syncthreads();
-  const int a0 = blockIdx.x * PLAN_ROWS;
-  for (int i = threadIdx.x; i < PLAN_ROWS && a0 + i < p.N; i += PLAN_THREADS) {
-    const unsigned e = (unsigned)p.ids[a0 + i];
-    if (e < (unsigned)p.E) atomicAdd(&count[e], 1);
-  }
+#pragma unroll
+  for (int i = 0; i < PLAN_EACH; ++i)
+    if (e[i] < p.E) atomicAdd(&count[e[i]], 1);
   __syncthreads();
-  for (int e = threadIdx.x; e < p.E; e += PLAN_THREADS)
-    p.counts[blockIdx.x * p.E + e] = count[e];
+  for (int i = threadIdx.x; i < p.E; i += PLAN_THREADS)
+    p.counts[blockIdx.x * p.E + i] = count[i];
 }
 
 // out[i] = sum of in[0..i), for i up to n: by the first wave, 64 a turn
@@ -579,20 +594,22 @@ __global__ __launch_bounds__(PLAN_THREADS) void plan_place_kernel(Plan p) {
   int* next = lds + p.E;        // [E]
   int* start = lds + 2 * p.E;   // [E + 1]
   int* tile0 = lds + 3 * p.E + 1;  // [E + 1]
-  const int a0 = blockIdx.x * PLAN_ROWS;
+  int mine[PLAN_EACH];
+  load_ids(p, blockIdx.x * PLAN_ROWS, mine);
   if (p.blocks == 1) {
-    for (int e = threadIdx.x; e < p.E; e += PLAN_THREADS) total[e] = 0;
+    for (int e = threadIdx.x; e < p.E; e += PLAN_THREADS)
+      total[e] = next[e] = 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < p.N; i += PLAN_THREADS) {
-      const unsigned e = (unsigned)p.ids[i];
-      if (e < (unsigned)p.E) atomicAdd(&total[e], 1);
-    }
+#pragma unroll
+    for (int i = 0; i < PLAN_EACH; ++i)
+      if (mine[i] < p.E) atomicAdd(&total[mine[i]], 1);
   } else {
     for (int e = threadIdx.x; e < p.E; e += PLAN_THREADS) {
       int before = 0, sum = 0;
+#pragma unroll 8
       for (int b = 0; b < p.blocks; ++b) {
         const int c = p.counts[b * p.E + e];
-        if (b < (int)blockIdx.x) before += c;
+        before += b < (int)blockIdx.x ? c : 0;
         sum += c;
       }
       total[e] = sum;
@@ -603,33 +620,32 @@ __global__ __launch_bounds__(PLAN_THREADS) void plan_place_kernel(Plan p) {
   scan(total, start, p.E);
   __syncthreads();
   for (int e = threadIdx.x; e < p.E; e += PLAN_THREADS) {
-    next[e] = start[e] + (p.blocks == 1 ? 0 : next[e]);
+    next[e] += start[e];
     total[e] = (total[e] + p.BM - 1) / p.BM;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < PLAN_ROWS && a0 + i < p.N; i += PLAN_THREADS) {
-    const unsigned e = (unsigned)p.ids[a0 + i];
-    if (e < (unsigned)p.E) p.order[atomicAdd(&next[e], 1)] = a0 + i;
-  }
+#pragma unroll
+  for (int i = 0; i < PLAN_EACH; ++i)
+    if (mine[i] < p.E)
+      p.order[atomicAdd(&next[mine[i]], 1)] =
+          blockIdx.x * PLAN_ROWS + i * PLAN_THREADS + threadIdx.x;
   if (blockIdx.x != 0) return;
   scan(total, tile0, p.E);
   __syncthreads();
-  for (int i = threadIdx.x; i < p.n_tiles; i += PLAN_THREADS) {
-    int4 t = make_int4(-1, 0, 0, 0);
-    if (i < tile0[p.E]) {
-      int lo = 0, hi = p.E;  // the expert with tile0[e] <= i < tile0[e + 1]
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (tile0[mid] <= i)
-          lo = mid;
-        else
-          hi = mid;
-      }
-      const int at = start[lo] + (i - tile0[lo]) * p.BM;
-      t = make_int4(lo, at, min(p.BM, start[lo + 1] - at), 0);
+  const int tiles = tile0[p.E];
+  for (int i = threadIdx.x; i < tiles; i += PLAN_THREADS) {
+    int lo = 0, hi = p.E;  // the expert with tile0[e] <= i < tile0[e + 1]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (tile0[mid] <= i)
+        lo = mid;
+      else
+        hi = mid;
     }
-    p.tiles[i] = t;
+    const int at = start[lo] + (i - tile0[lo]) * p.BM;
+    p.tiles[i] = make_int4(lo, at, min(p.BM, start[lo + 1] - at), 0);
   }
+  if (threadIdx.x == 0) p.tiles[p.n_tiles] = make_int4(tiles, 0, 0, 0);
 }
 
 // rows of bf16 that no 16-byte load can take as they are: copied once, filled
@@ -661,7 +677,8 @@ struct Experts {
   void* H;            // first: [N][np] bf16 or e4m3
   float* SH;          // first: [np / 128][N]
   const float* w;     // second: [N] by assignment
-  float* Y;           // second: [N][n] by assignment
+  _Float16* Y;        // second: [N][up64(n)] by assignment, over a power of
+  float* SY;          // two for each 64 columns, [N][up64(n) / 64]
 };
 
 // The rows of one tile, all of one expert, times its weights. FIRST: rows are
@@ -673,10 +690,13 @@ __global__ __launch_bounds__(S::THREADS, 2) void experts_kernel(Experts p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Place at_tile = place_of(blockIdx.x, p.n_tiles, p.tiles_n);
+  // the grid is for the most tiles there can be; those that there are get
+  // spread over all XCDs
+  const int tiles = __builtin_amdgcn_readfirstlane(p.tiles[p.n_tiles].x);
+  if ((int)blockIdx.x >= tiles * p.tiles_n) return;
+  const Place at_tile = place_of(blockIdx.x, tiles, p.tiles_n);
   const int4 tile = p.tiles[at_tile.m];
   const int e = __builtin_amdgcn_readfirstlane(tile.x);
-  if (e < 0) return;
   const int at0 = __builtin_amdgcn_readfirstlane(tile.y);
   const int rows = __builtin_amdgcn_readfirstlane(tile.z);
   const int n0 = at_tile.n * S::BN;
@@ -807,51 +827,89 @@ __global__ __launch_bounds__(S::THREADS, 2) void experts_kernel(Experts p) {
       if (row(i) >= rows) continue;
       const int a = p.order[at0 + row(i)];
       const float w = p.w[a];
+      // A row of 64 columns shares a power of two that brings its largest
+      // value under 2^15, and goes out in 16 bits: 2^-12 of the value is lost
+      // where the sum's own rounding to bf16 loses 2^-9, and the terms, the
+      // most that this layer moves, take half the bytes.
+      uint32_t top = 0;
+      float v[S::RUNS][S::W];
 #pragma unroll
       for (int q = 0; q < S::RUNS; ++q) {
-        float v[S::W], b[S::W];
+        float b[S::W];
         load_bias(q, b);
-        run_of<S>(acc[i], q, v);
+        run_of<S>(acc[i], q, v[q]);
 #pragma unroll
-        for (int c = 0; c < S::W; ++c) v[c] = (v[c] + b[c]) * w;
-        store_run(p.Y + (int64_t)a * p.n + column(q), p.n - column(q), v);
+        for (int c = 0; c < S::W; ++c)
+          v[q][c] = column(q) + c < p.n ? (v[q][c] + b[c]) * w : 0.f;
+        top = max(top, amax_bits(v[q]));
       }
+      top = max(top, (uint32_t)__shfl_xor((int)top, 16));
+      top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+      const int up = max((int)(top >> 23), 15) - 14;  // the power of two, biased
+      const float down = __builtin_bit_cast(float, (254 - up) << 23);
+      const int cols64 = (p.n + 63) / 64;
+#pragma unroll
+      for (int q = 0; q < S::RUNS; ++q) {
+        _Float16 h[S::W];
+#pragma unroll
+        for (int c = 0; c < S::W; ++c) h[c] = (_Float16)(v[q][c] * down);
+        if (column(q) < p.np)
+          __builtin_memcpy(__builtin_assume_aligned(
+                               p.Y + (int64_t)a * p.np + column(q), 16),
+                           h, sizeof(h));
+      }
+      if (lane < 16 && wave_n0 < p.np)
+        p.SY[(int64_t)a * cols64 + wave_n0 / 64] =
+            __builtin_bit_cast(float, up << 23);
     }
   }
 }
 
-// each token adds up its experts' rows, in the order of its list
+// each token adds up its experts' rows, in the order of its list: 8 columns a
+// thread
 __global__ __launch_bounds__(256) void combine_kernel(
-    const float* __restrict__ P, const int* __restrict__ ids, int E, int k,
-    int D, const __bf16* residual, int64_t ldr, __bf16* Y, int64_t ldy,
+    const _Float16* __restrict__ P, const float* __restrict__ SP,
+    const int* __restrict__ ids, int E, int k, int D, int Dp,
+    const __bf16* residual, int64_t ldr, __bf16* Y, int64_t ldy, bool vec,
     int64_t n) {
-  const int per = (D + 3) / 4;
+  const int per = (D + 7) / 8;
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= n) return;
   const int64_t t = i / per;
-  const int c = (int)(i - t * per) * 4;
-  const int have = min(4, D - c);
-  float v[4] = {0.f, 0.f, 0.f, 0.f};
+  const int c = (int)(i - t * per) * 8;
+  float v[8] = {};
+#pragma unroll 4
   for (int j = 0; j < k; ++j) {
     if ((unsigned)ids[t * k + j] >= (unsigned)E) continue;
-    const float* y = P + (t * k + j) * D + c;
-    if (have == 4) {
-      float u[4];
-      __builtin_memcpy(u, y, sizeof(u));
+    const int64_t a = t * k + j;
+    _Float16 u[8];
+    __builtin_memcpy(u, __builtin_assume_aligned(P + a * Dp + c, 16),
+                     sizeof(u));
+    const float s = SP[a * (Dp / 64) + c / 64];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) v[q] += u[q];
-    } else {
-      for (int q = 0; q < have; ++q) v[q] += y[q];
-    }
+    for (int q = 0; q < 8; ++q) v[q] = __builtin_fmaf((float)u[q], s, v[q]);
   }
-  for (int q = 0; q < have; ++q) {
-    if (residual) v[q] += (float)residual[t * ldr + c + q];
-    Y[t * ldy + c + q] = (__bf16)v[q];
+  const __bf16* r = residual + t * ldr + c;
+  __bf16* y = Y + t * ldy + c;
+  __bf16 o[8];
+  if (vec && c + 8 <= D) {
+    if (residual) {
+      __builtin_memcpy(o, __builtin_assume_aligned(r, 16), sizeof(o));
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[q] += (float)o[q];
+    }
+#pragma unroll
+    for (int q = 0; q < 8; ++q) o[q] = (__bf16)v[q];
+    __builtin_memcpy(__builtin_assume_aligned(y, 16), o, sizeof(o));
+  } else {
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      if (c + q < D) y[q] = (__bf16)(v[q] + (residual ? (float)r[q] : 0.f));
   }
 }
 
 template <bool FP8, bool FIRST>
-using Tile = Shape<FP8, 128, 128, 2, 2, 2, FIRST ? (FP8 ? 16 : 8) : 4>;
+using Tile = Shape<FP8, 128, 128, 2, 2, 2, FIRST && FP8 ? 16 : 8>;
 
 template <class S, bool FIRST>
 void run(Experts p, hipStream_t stream) {
@@ -864,7 +922,7 @@ int64_t up256(int64_t bytes) { return (bytes + 255) & ~int64_t(255); }
 
 // where a call's intermediate data lie
 struct Layout {
-  int64_t counts, order, tiles, x, sx, h, sh, y, bytes;
+  int64_t counts, order, tiles, x, sx, h, sh, y, sy, bytes;
   int n_tiles, blocks, BM, Dp, Hp;
   bool copy;  // the rows of x are brought into whole steps first
 };
@@ -888,12 +946,13 @@ Layout layout(const MoeMlp& m) {
   };
   l.counts = take(l.blocks > 1 ? (int64_t)l.blocks * m.E * 4 : 0);
   l.order = take(N * 4);
-  l.tiles = take((int64_t)l.n_tiles * 16);
+  l.tiles = take((int64_t)(l.n_tiles + 1) * 16);
   l.x = take(l.copy ? (int64_t)m.T * l.Dp * size : 0);
   l.sx = take(m.fp8 ? (int64_t)m.T * (l.Dp / 128) * 4 : 0);
   l.h = take(N * l.Hp * size);
   l.sh = take(m.fp8 ? N * (l.Hp / 128) * 4 : 0);
-  l.y = take(N * m.D * 4);
+  l.y = take(N * up(m.D, 64) * 64 * 2);
+  l.sy = take(N * up(m.D, 64) * 4);
   l.bytes = at;
   return l;
 }
@@ -946,16 +1005,21 @@ void run_mlp(const MoeMlp& m, const Layout& l, char* ws, hipStream_t stream) {
   p.B = (const uint8_t*)m.W2;
   p.SB = m.S2;
   p.bias = m.b2;
-  p.n = p.np = m.D;
+  p.n = m.D;
+  p.np = up(m.D, 64) * 64;
   p.steps = l.Hp * size / STEP;
   p.w = m.weights;
-  p.Y = (float*)(ws + l.y);
+  p.Y = (_Float16*)(ws + l.y);
+  p.SY = (float*)(ws + l.sy);
   run<Tile<FP8, false>, false>(p, stream);
 
-  const int64_t work = (int64_t)m.T * ((m.D + 3) / 4);
+  const int64_t work = (int64_t)m.T * up(m.D, 8);
+  const bool vec = (uintptr_t)m.Y % 16 == 0 && m.ldy % 8 == 0 &&
+                   (uintptr_t)m.residual % 16 == 0 && m.ldr % 8 == 0;
   hipLaunchKernelGGL(combine_kernel, dim3(up(work, 256)), dim3(256), 0, stream,
-                     p.Y, m.ids, m.E, m.k, m.D, (const __bf16*)m.residual,
-                     m.ldr, (__bf16*)m.Y, m.ldy, work);
+                     p.Y, p.SY, m.ids, m.E, m.k, m.D, p.np,
+                     (const __bf16*)m.residual, m.ldr, (__bf16*)m.Y, m.ldy,
+                     vec, work);
 }
 
 }  // namespace

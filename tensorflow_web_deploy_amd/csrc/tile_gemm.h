@@ -207,16 +207,23 @@ __device__ __forceinline__ void compute(const char* lds, float sb, int wm,
       }
     }
   } else {
+    // rows i + 2 are read while rows i are multiplied
+    FragA<S> a[3];
+    a[0] = read_a<S>(lds, wm, 0, lane);
+    if (S::MT > 1) a[1] = read_a<S>(lds, wm, 1, lane);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < S::MT; ++i) {
-      const FragA<S> a = read_a<S>(lds, wm, i, lane);
+      if (i + 2 < S::MT) a[(i + 2) % 3] = read_a<S>(lds, wm, i + 2, lane);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int t = 0; t < S::NT; ++t)
           acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
               __builtin_bit_cast(bf16x8, b[t][h]),
-              __builtin_bit_cast(bf16x8, a.v[h]), acc[i][t], 0, 0, 0);
+              __builtin_bit_cast(bf16x8, a[i % 3].v[h]), acc[i][t], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
 }
