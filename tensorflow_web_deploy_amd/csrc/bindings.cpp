@@ -322,6 +322,12 @@ void check_whole(const torch::Tensor& t, c10::ScalarType type,
   TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
 }
 
+// the kernels take these 16 bytes at a time
+void check_aligned(const torch::Tensor& t, const char* name) {
+  TORCH_CHECK((uintptr_t)t.data_ptr() % 16 == 0, name,
+              " must start at a multiple of 16 bytes");
+}
+
 // rows of contiguous values that may lie apart, but not over each other
 void check_rows(const torch::Tensor& t, const char* name) {
   TORCH_CHECK(t.dim() == 2, name, " must be 2D");
@@ -374,6 +380,7 @@ void quant_fp8(torch::Tensor X, torch::Tensor Q, torch::Tensor S,
   TORCH_CHECK(M < 1 << 30 && blocks128(M) * Kb < 1 << 30,
               "X is too large: ", X.sizes());
   check_whole(Q, kFp8, {M, Kb * 128}, "Q");
+  check_aligned(Q, "Q");
   if (block_rows == 1)
     check_whole(S, torch::kFloat32, {Kb, M}, "S");
   else
@@ -408,6 +415,8 @@ void gemm_fp8(torch::Tensor A, torch::Tensor SA, torch::Tensor B,
   check_whole(A, kFp8, {M, Kp}, "A");
   check_whole(SA, torch::kFloat32, {Kp / 128, M}, "SA");
   check_whole(B, kFp8, {N, Kp}, "B");
+  check_aligned(A, "A");
+  check_aligned(B, "B");
   check_whole(SB, torch::kFloat32, {blocks128(N), Kp / 128}, "SB");
   check_act(act);
   std::vector<std::pair<const torch::Tensor*, const char*>> all = {
@@ -516,6 +525,8 @@ void moe_mlp(const torch::Tensor& X, const torch::Tensor& ids,
   const auto wtype = fp8 ? kFp8 : torch::kBFloat16;
   check_whole(W1, wtype, {E, H, Dp}, "W1");
   check_whole(W2, wtype, {E, D, Hp}, "W2");
+  check_aligned(W1, "W1");
+  check_aligned(W2, "W2");
   check_type(Y, torch::kBFloat16, "Y");
   check_shape(Y, {T, D}, "Y");
   check_rows(Y, "Y");

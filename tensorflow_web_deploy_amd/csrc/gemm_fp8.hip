@@ -44,6 +44,13 @@ __device__ __forceinline__ void load8(const T* p, int have, float (&v)[8]) {
   }
 }
 
+__device__ __forceinline__ void store_fp8(uint8_t* to, const float (&v)[8],
+                                          float s) {
+  uint32_t q[2];
+  to_fp8(v, s, q);
+  *(uint2*)to = make_uint2(q[0], q[1]);
+}
+
 // 16 lanes take a block of a row, 8 values each; 16 rows a workgroup.
 // Bound by the bytes it moves.
 template <typename T>
@@ -62,7 +69,7 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(
 #pragma unroll
     for (int d = 8; d; d >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
     const float s = scale_of(top);
-    *(uint2*)(Q + m * Kp + k) = to_fp8(v, s);
+    store_fp8(Q + m * Kp + k, v, s);
     if (l == 0) S[kb * M + m] = s;
   }
 }
@@ -94,7 +101,7 @@ __global__ __launch_bounds__(256) void quant_tiles_kernel(
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int64_t m = m0 + i * 16 + r0;
-    if (m < M) *(uint2*)(Q + m * Kp + k) = to_fp8(v[i], s);
+    if (m < M) store_fp8(Q + m * Kp + k, v[i], s);
   }
   if (threadIdx.x == 0) S[blockIdx.x] = s;
 }
@@ -198,6 +205,27 @@ __global__ __launch_bounds__(S::THREADS, 2) void gemm_fp8_kernel(Dense d) {
   }
 }
 
+// up to 16 rows: 16 columns a workgroup, K cut into 8 parts, a wave each
+__global__ __launch_bounds__(512, 4) void gemm_fp8_few_kernel(Dense d) {
+  __shared__ __attribute__((aligned(16))) float part[8 * 256];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n0 = blockIdx.x * 16, all = d.Kp / STEP;
+  const int row = min(lane & 15, d.M - 1), col = min(n0 + (lane & 15), d.N - 1);
+  const f32x4 acc = few_product<true>(
+      d.A + (int64_t)row * d.Kp + (lane >> 4) * 16,
+      d.B + (int64_t)col * d.Kp + (lane >> 4) * 16, d.SA + row, d.M,
+      d.SB + (int64_t)(n0 / 128) * all, all * wave / 8, all * (wave + 1) / 8);
+  const f32x4 sum = few_join<8>(acc, part, 0, wave, lane);
+  const int m = lane & 15, n = n0 + (lane >> 4) * 4;
+  if (wave || m >= d.M || n >= d.N) return;
+  float v[4] = {sum[0], sum[1], sum[2], sum[3]}, b[4];
+  load_run(d.bias + n, d.bias ? d.N - n : 0, b);
+  Dense one = d;
+  one.vec = false;
+  finish(one, m, n, v, b);
+}
+
 // split K: adds up the slices, in their order, and finishes the layer
 __global__ __launch_bounds__(256) void gemm_fp8_join_kernel(Dense d,
                                                             int slices) {
@@ -223,6 +251,9 @@ template <int W>
 using Tile128 = Shape<true, 128, 128, 2, 2, 2, W>;
 template <int W>
 using Tile256 = Shape<true, 256, 256, 2, 4, 2, W>;
+// rows for half a tile: what counts is how much of the weights is on its way
+template <int W>
+using Tile64 = Shape<true, 64, 128, 2, 2, 4, W>;
 
 int up(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
@@ -245,15 +276,23 @@ void run(Dense d, int slices, hipStream_t stream) {
                      0, stream, d, slices);
 }
 
-// slices: how often K is cut so that the grid fills the 256 CUs
-void plan(int M, int N, int Kp, int* slices, int* steps) {
-  const int64_t tiles =
-      (int64_t)up(M, 128) * up(N, 128);
+enum class Way { FEW, TILE64, TILE128, TILE256 };
+
+struct Plan {
+  Way way;
+  int slices, steps;  // K is cut so often that the grid fills the 256 CUs
+};
+
+Plan plan(int M, int N, int Kp) {
   const int all = Kp / STEP;
+  if (M <= 16) return {Way::FEW, 1, all};
+  if ((int64_t)up(M, 256) * up(N, 256) >= 256) return {Way::TILE256, 1, all};
+  const Way way = M <= 64 ? Way::TILE64 : Way::TILE128;
+  const int64_t tiles = (int64_t)up(M, 128) * up(N, 128);
   int s = 1;
   while (tiles * s < 256 && all / (s * 2) >= 4) s *= 2;
-  *steps = up(all, s);
-  *slices = up(all, *steps);
+  const int steps = up(all, s);
+  return {way, up(all, steps), steps};
 }
 
 }  // namespace
@@ -283,9 +322,8 @@ void launch_quant_fp8(const void* X, bool f32, int64_t ldx, int64_t M, int K,
 }
 
 int64_t gemm_fp8_workspace(int M, int N, int Kp) {
-  int slices, steps;
-  plan(M, N, Kp, &slices, &steps);
-  return slices > 1 ? (int64_t)slices * M * N : 0;
+  const Plan p = plan(M, N, Kp);
+  return p.slices > 1 ? (int64_t)p.slices * M * N : 0;
 }
 
 void launch_gemm_fp8(const void* A, const float* SA, const void* B,
@@ -310,10 +348,21 @@ void launch_gemm_fp8(const void* A, const float* SA, const void* B,
   d.ldr = ldr;
   d.vec = (uintptr_t)C % 16 == 0 && ldc % 8 == 0 &&
           (!residual || ((uintptr_t)residual % 16 == 0 && ldr % 8 == 0));
-  int slices;
-  plan(M, N, Kp, &slices, &d.steps);
-  if (slices == 1 && (int64_t)up(M, 256) * up(N, 256) >= 256)
-    run<Tile256>(d, slices, stream);
-  else
-    run<Tile128>(d, slices, stream);
+  const Plan p = plan(M, N, Kp);
+  d.steps = p.steps;
+  switch (p.way) {
+    case Way::FEW:
+      hipLaunchKernelGGL(gemm_fp8_few_kernel, dim3(up(N, 16)), dim3(512), 0,
+                         stream, d);
+      break;
+    case Way::TILE64:
+      run<Tile64>(d, p.slices, stream);
+      break;
+    case Way::TILE128:
+      run<Tile128>(d, p.slices, stream);
+      break;
+    case Way::TILE256:
+      run<Tile256>(d, p.slices, stream);
+      break;
+  }
 }

@@ -665,6 +665,8 @@ __global__ __launch_bounds__(256) void pad_rows_kernel(
 struct Experts {
   const int4* tiles;
   const int* order;
+  const int* ids;    // without a plan: each row is a tile of its own
+  int E;
   int k, N, n_tiles, tiles_n;
   const uint8_t* A;  // rows by token (first product) or by place (second)
   const float* SA;   // [steps][rows]
@@ -680,6 +682,26 @@ struct Experts {
   _Float16* Y;        // second: [N][up64(n)] by assignment, over a power of
   float* SY;          // two for each 64 columns, [N][up64(n) / 64]
 };
+
+// A row's 64 columns of a term share a power of two that brings the largest
+// under 2^15, and go out in 16 bits: 2^-12 of a value is lost where the sum's
+// own rounding to bf16 loses 2^-9, and the terms, the most that a layer of
+// many rows moves, take half the bytes.
+__device__ __forceinline__ int power_over(uint32_t top) {  // its biased form
+  return max((int)(top >> 23), 15) - 14;
+}
+__device__ __forceinline__ float power(int biased) {
+  return __builtin_bit_cast(float, biased << 23);
+}
+template <int R>
+__device__ __forceinline__ void store_terms(_Float16* to, const float (&v)[R],
+                                            int up) {
+  const float down = power(254 - up);
+  _Float16 h[R];
+#pragma unroll
+  for (int c = 0; c < R; ++c) h[c] = (_Float16)(v[c] * down);
+  __builtin_memcpy(__builtin_assume_aligned(to, R * 2), h, sizeof(h));
+}
 
 // The rows of one tile, all of one expert, times its weights. FIRST: rows are
 // gathered by token, the result is activated, rounded to the layer's type and
@@ -790,14 +812,8 @@ __global__ __launch_bounds__(S::THREADS, 2) void experts_kernel(Experts p) {
       for (int q = 0; q < S::RUNS; ++q) {
         float v[S::W];
         run_of<S>(acc[i], q, v);
-        uint2 h[S::W / 8];
-#pragma unroll
-        for (int c = 0; c < S::W / 8; ++c) {
-          float u[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) u[j] = v[c * 8 + j];
-          h[c] = to_fp8(u, s);
-        }
+        uint32_t h[S::W / 4];
+        to_fp8(v, s, h);
         uint8_t* to = (uint8_t*)p.H + (int64_t)(at0 + r) * p.np + column(q);
         __builtin_memcpy(__builtin_assume_aligned(to, sizeof(h)), h,
                          sizeof(h));
@@ -827,10 +843,6 @@ __global__ __launch_bounds__(S::THREADS, 2) void experts_kernel(Experts p) {
       if (row(i) >= rows) continue;
       const int a = p.order[at0 + row(i)];
       const float w = p.w[a];
-      // A row of 64 columns shares a power of two that brings its largest
-      // value under 2^15, and goes out in 16 bits: 2^-12 of the value is lost
-      // where the sum's own rounding to bf16 loses 2^-9, and the terms, the
-      // most that this layer moves, take half the bytes.
       uint32_t top = 0;
       float v[S::RUNS][S::W];
 #pragma unroll
@@ -845,24 +857,116 @@ __global__ __launch_bounds__(S::THREADS, 2) void experts_kernel(Experts p) {
       }
       top = max(top, (uint32_t)__shfl_xor((int)top, 16));
       top = max(top, (uint32_t)__shfl_xor((int)top, 32));
-      const int up = max((int)(top >> 23), 15) - 14;  // the power of two, biased
-      const float down = __builtin_bit_cast(float, (254 - up) << 23);
-      const int cols64 = (p.n + 63) / 64;
+      const int up = power_over(top);
 #pragma unroll
-      for (int q = 0; q < S::RUNS; ++q) {
-        _Float16 h[S::W];
-#pragma unroll
-        for (int c = 0; c < S::W; ++c) h[c] = (_Float16)(v[q][c] * down);
+      for (int q = 0; q < S::RUNS; ++q)
         if (column(q) < p.np)
-          __builtin_memcpy(__builtin_assume_aligned(
-                               p.Y + (int64_t)a * p.np + column(q), 16),
-                           h, sizeof(h));
-      }
+          store_terms(p.Y + (int64_t)a * p.np + column(q), v[q], up);
       if (lane < 16 && wave_n0 < p.np)
-        p.SY[(int64_t)a * cols64 + wave_n0 / 64] =
-            __builtin_bit_cast(float, up << 23);
+        p.SY[(int64_t)a * (p.np / 64) + wave_n0 / 64] = power(up);
     }
   }
+}
+
+// Without a plan, the first product: CW * 16 columns of an assignment a
+// workgroup, K cut into KS parts, a wave each. The 16 rows are all the same.
+template <bool FP8, int CW, int KS>
+__global__ __launch_bounds__(512, 4) void experts_hidden_kernel(Experts p) {
+  static_assert(CW * KS == 8 && (!FP8 || CW == 8));
+  __shared__ __attribute__((aligned(16))) float part[8 * 256];
+  __shared__ uint32_t top[CW];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int cw = wave / KS, ks = wave % KS;
+  const int64_t a = blockIdx.x / p.tiles_n;
+  const int n0 = ((int)(blockIdx.x - a * p.tiles_n) * CW + cw) * 16;
+  const int e = p.ids[a];
+  if ((unsigned)e >= (unsigned)p.E) return;
+  const int64_t row = a / p.k;
+  const int col = min(n0 + (lane & 15), p.n - 1);
+  const int blocks_n = (p.n + 127) / 128;
+  const f32x4 acc = few_product<FP8>(
+      p.A + row * p.a_row + (lane >> 4) * 16,
+      p.B + ((int64_t)e * p.n + col) * ((int64_t)p.steps * STEP) +
+          (lane >> 4) * 16,
+      p.SA + row, p.sa_rows,
+      p.SB + ((int64_t)e * blocks_n + min(n0 / 128, blocks_n - 1)) * p.steps,
+      p.steps * ks / KS, p.steps * (ks + 1) / KS);
+  const f32x4 sum = few_join<KS>(acc, part, cw, ks, lane);
+  const int n = n0 + (lane >> 4) * 4;
+  float v[4] = {sum[0], sum[1], sum[2], sum[3]}, b[4];
+  load_run(p.bias + (int64_t)e * p.n + n, p.bias ? p.n - n : 0, b);
+#pragma unroll
+  for (int c = 0; c < 4; ++c) v[c] += b[c];
+  activate_by(v, p.act);
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    if (n + c >= p.n) v[c] = 0.f;
+  const bool mine = ks == 0 && (lane & 15) == 0 && n0 < p.np;
+  if constexpr (FP8) {
+    uint32_t m = amax_bits(v);
+    m = max(m, (uint32_t)__shfl_xor((int)m, 16));
+    m = max(m, (uint32_t)__shfl_xor((int)m, 32));
+    if (lane == 0) top[cw] = m;
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < CW; ++c) m = max(m, top[c]);
+    if (!mine) return;
+    const float s = scale_of(m);
+    uint32_t h[1];
+    to_fp8(v, s, h);
+    *(uint32_t*)((uint8_t*)p.H + a * p.np + n) = h[0];
+    if (cw == 0 && lane == 0) p.SH[(int64_t)(n0 / 128) * p.N + a] = s;
+  } else if (mine) {
+    __bf16 h[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) h[c] = (__bf16)v[c];
+    __builtin_memcpy(
+        __builtin_assume_aligned((__bf16*)p.H + a * p.np + n, 8), h,
+        sizeof(h));
+  }
+}
+
+// Without a plan, the second product and the sum over a token's experts: 16
+// columns of a token a workgroup. Its 16 rows are all the same one.
+template <bool FP8>
+__global__ __launch_bounds__(512, 4) void experts_sum_kernel(
+    Experts p, const __bf16* residual, int64_t ldr, __bf16* Y, int64_t ldy) {
+  __shared__ __attribute__((aligned(16))) float part[8 * 256];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t t = blockIdx.x / p.tiles_n;
+  const int n0 = (int)(blockIdx.x - t * p.tiles_n) * 16;
+  const int col = min(n0 + (lane & 15), p.n - 1);
+  const int n = n0 + (lane >> 4) * 4;
+  const int blocks_n = (p.n + 127) / 128;
+  f32x4 total = {0.f, 0.f, 0.f, 0.f};
+  for (int j = 0; j < p.k; ++j) {
+    const int64_t a = t * p.k + j;
+    const int e = p.ids[a];
+    if ((unsigned)e >= (unsigned)p.E) continue;
+    const f32x4 acc = few_product<FP8>(
+        p.A + a * p.a_row + (lane >> 4) * 16,
+        p.B + ((int64_t)e * p.n + col) * ((int64_t)p.steps * STEP) +
+            (lane >> 4) * 16,
+        p.SA + a, p.sa_rows,
+        p.SB + ((int64_t)e * blocks_n + n0 / 128) * p.steps,
+        p.steps * wave / 8, p.steps * (wave + 1) / 8);
+    const float w = p.w[a];
+    float b[4];
+    load_run(p.bias + (int64_t)e * p.n + n,
+             p.bias && wave == 0 ? p.n - n : 0, b);
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      total[c] = __builtin_fmaf(acc[c] + b[c], w, total[c]);
+  }
+  const f32x4 sum = few_join<8>(total, part, 0, wave, lane);
+  if (wave || lane & 15) return;
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    if (n + c < p.n)
+      Y[t * ldy + n + c] =
+          (__bf16)(sum[c] + (residual ? (float)residual[t * ldr + n + c] : 0.f));
 }
 
 // each token adds up its experts' rows, in the order of its list: 8 columns a
@@ -909,7 +1013,10 @@ __global__ __launch_bounds__(256) void combine_kernel(
 }
 
 template <bool FP8, bool FIRST>
-using Tile = Shape<FP8, 128, 128, 2, 2, 2, FIRST && FP8 ? 16 : 8>;
+using Tile128 = Shape<FP8, 128, 128, 2, 2, 2, FIRST && FP8 ? 16 : 8>;
+// few rows an expert: what counts is how much of the weights is on its way
+template <bool FP8, bool FIRST>
+using Tile32 = Shape<FP8, 32, 128, 2, 2, 4, FIRST && FP8 ? 16 : 8>;
 
 template <class S, bool FIRST>
 void run(Experts p, hipStream_t stream) {
@@ -921,7 +1028,10 @@ void run(Experts p, hipStream_t stream) {
 int64_t up256(int64_t bytes) { return (bytes + 255) & ~int64_t(255); }
 
 // where a call's intermediate data lie
+// direct: so few rows that a plan isn't worth its launches, two products and
+// no more
 struct Layout {
+  bool direct;
   int64_t counts, order, tiles, x, sx, h, sh, y, sy, bytes;
   int n_tiles, blocks, BM, Dp, Hp;
   bool copy;  // the rows of x are brought into whole steps first
@@ -930,7 +1040,8 @@ struct Layout {
 Layout layout(const MoeMlp& m) {
   Layout l{};
   const int64_t N = (int64_t)m.T * m.k;
-  l.BM = 128;
+  l.direct = N <= 8 && N <= m.E;
+  l.BM = N <= 32 * (int64_t)m.E ? 32 : 128;
   l.n_tiles = (int)(N / l.BM + std::min<int64_t>(N, m.E));
   l.blocks = up(N, PLAN_ROWS);
   const int unit = m.fp8 ? 128 : 64, size = m.fp8 ? 1 : 2;
@@ -960,17 +1071,20 @@ Layout layout(const MoeMlp& m) {
 template <bool FP8>
 void run_mlp(const MoeMlp& m, const Layout& l, char* ws, hipStream_t stream) {
   const int N = m.T * m.k;
-  Plan plan{m.ids, (int*)(ws + l.counts), (int*)(ws + l.order),
+  const Plan plan{m.ids, (int*)(ws + l.counts), (int*)(ws + l.order),
             (int4*)(ws + l.tiles), N, m.E, l.BM, l.n_tiles, l.blocks};
   if (l.blocks > 1)
     hipLaunchKernelGGL(plan_count_kernel, dim3(l.blocks), dim3(PLAN_THREADS),
                        m.E * 4, stream, plan);
-  hipLaunchKernelGGL(plan_place_kernel, dim3(l.blocks), dim3(PLAN_THREADS),
-                     (4 * m.E + 2) * 4, stream, plan);
+  if (!l.direct)
+    hipLaunchKernelGGL(plan_place_kernel, dim3(l.blocks), dim3(PLAN_THREADS),
+                       (4 * m.E + 2) * 4, stream, plan);
 
   Experts p{};
   p.tiles = plan.tiles;
   p.order = plan.order;
+  p.ids = l.direct ? m.ids : nullptr;
+  p.E = m.E;
   p.k = m.k;
   p.N = N;
   p.n_tiles = l.n_tiles;
@@ -996,7 +1110,16 @@ void run_mlp(const MoeMlp& m, const Layout& l, char* ws, hipStream_t stream) {
   p.act = m.act;
   p.H = ws + l.h;
   p.SH = (float*)(ws + l.sh);
-  run<Tile<FP8, true>, true>(p, stream);
+  if (l.direct) {
+    constexpr int CW = FP8 ? 8 : 2;
+    p.tiles_n = up(p.np, CW * 16);
+    hipLaunchKernelGGL((experts_hidden_kernel<FP8, CW, 8 / CW>),
+                       dim3(N * p.tiles_n), dim3(512), 0, stream, p);
+  } else if (l.BM == 32) {
+    run<Tile32<FP8, true>, true>(p, stream);
+  } else {
+    run<Tile128<FP8, true>, true>(p, stream);
+  }
 
   p.A = (const uint8_t*)ws + l.h;
   p.a_row = (int64_t)l.Hp * size;
@@ -1011,15 +1134,25 @@ void run_mlp(const MoeMlp& m, const Layout& l, char* ws, hipStream_t stream) {
   p.w = m.weights;
   p.Y = (_Float16*)(ws + l.y);
   p.SY = (float*)(ws + l.sy);
-  run<Tile<FP8, false>, false>(p, stream);
+  const auto residual = (const __bf16*)m.residual;
+  if (l.direct) {
+    p.tiles_n = up(m.D, 16);
+    hipLaunchKernelGGL((experts_sum_kernel<FP8>), dim3(m.T * p.tiles_n),
+                       dim3(512), 0, stream, p, residual, m.ldr, (__bf16*)m.Y,
+                       m.ldy);
+    return;
+  }
+  if (l.BM == 32)
+    run<Tile32<FP8, false>, false>(p, stream);
+  else
+    run<Tile128<FP8, false>, false>(p, stream);
 
   const int64_t work = (int64_t)m.T * up(m.D, 8);
   const bool vec = (uintptr_t)m.Y % 16 == 0 && m.ldy % 8 == 0 &&
                    (uintptr_t)m.residual % 16 == 0 && m.ldr % 8 == 0;
   hipLaunchKernelGGL(combine_kernel, dim3(up(work, 256)), dim3(256), 0, stream,
                      p.Y, p.SY, m.ids, m.E, m.k, m.D, p.np,
-                     (const __bf16*)m.residual, m.ldr, (__bf16*)m.Y, m.ldy,
-                     vec, work);
+                     residual, m.ldr, (__bf16*)m.Y, m.ldy, vec, work);
 }
 
 }  // namespace

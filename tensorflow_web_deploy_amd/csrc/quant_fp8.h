@@ -26,31 +26,34 @@ __device__ __forceinline__ float scale_of(uint32_t top) {
   return s < 0x1p-126f ? 0x1p-126f : s;
 }
 
-// 8 values over their scale, each quotient rounded to f32 as by a division
+// R values over their scale, each quotient rounded to f32 as by a division
 // and then to the nearest e4m3 value, the even one of two. Values of bf16
 // meet such ties often, so the quotient has to be the exact one: two
 // corrections from the reciprocal of the whole block give it in 5 operations
 // where a division takes twice as many. They need their remainders exact:
 // scales near the ends of the range take the division.
-__device__ __forceinline__ uint2 to_fp8(const float (&v)[8], float s) {
-  float q[8];
+template <int R>
+__device__ __forceinline__ void to_fp8(const float (&v)[R], float s,
+                                       uint32_t (&out)[R / 4]) {
+  float q[R];
   if (s > 0x1p-90f && s < 0x1p120f) {
     const float r = 1.f / s;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
+    for (int e = 0; e < R; ++e) {
       float y = v[e] * r;
       y = __builtin_fmaf(__builtin_fmaf(-y, s, v[e]), r, y);
       q[e] = __builtin_fmaf(__builtin_fmaf(-y, s, v[e]), r, y);
     }
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) q[e] = v[e] / s;
+    for (int e = 0; e < R; ++e) q[e] = v[e] / s;
   }
-  int lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
-  lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], lo, true);
-  int hi = __builtin_amdgcn_cvt_pk_fp8_f32(q[4], q[5], 0, false);
-  hi = __builtin_amdgcn_cvt_pk_fp8_f32(q[6], q[7], hi, true);
-  return make_uint2((uint32_t)lo, (uint32_t)hi);
+#pragma unroll
+  for (int e = 0; e < R; e += 4) {
+    const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[e], q[e + 1], 0, false);
+    out[e / 4] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[e + 2], q[e + 3],
+                                                           lo, true);
+  }
 }
 
 }  // namespace tile

@@ -279,6 +279,94 @@ __device__ __forceinline__ void product(char* smem, __amdgpu_buffer_rsrc_t ra,
   }
 }
 
+// The product of up to 16 rows with 16 columns by one wave, for calls that
+// read their weights for a few rows: bound by the time that the weights take
+// to come, so they go from memory to registers at once, U steps ahead.
+// a, b, sa: this lane's row of A and of B (16 bytes from their start a
+// quarter of the wave) and its row's scale at step 0. As in a tile, a lane
+// ends up with row lane % 16 and the columns lane / 16 * 4 + 0..3.
+template <bool FP8>
+struct FewStep {
+  i32x4 a[2], b[2];
+  float f;
+};
+
+template <bool FP8>
+__device__ __forceinline__ FewStep<FP8> few_step(const uint8_t* a,
+                                                 const uint8_t* b,
+                                                 const float* sa,
+                                                 int64_t s_rows,
+                                                 const float* sb, int step) {
+  FewStep<FP8> r;
+  const int64_t k = (int64_t)step * STEP;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    r.a[h] = *(const i32x4*)(a + k + h * 64);
+    r.b[h] = *(const i32x4*)(b + k + h * 64);
+  }
+  r.f = FP8 ? sa[step * s_rows] * sb[step] : 0.f;
+  return r;
+}
+
+template <bool FP8>
+__device__ __forceinline__ void few_multiply(const FewStep<FP8>& s,
+                                             f32x4& acc) {
+  if constexpr (FP8) {
+    const f32x4 p = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+        both(s.b), both(s.a), f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) acc[r] = __builtin_fmaf(p[r], s.f, acc[r]);
+  } else {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+          __builtin_bit_cast(bf16x8, s.b[h]),
+          __builtin_bit_cast(bf16x8, s.a[h]), acc, 0, 0, 0);
+  }
+}
+
+template <bool FP8>
+__device__ __forceinline__ f32x4 few_product(const uint8_t* a,
+                                             const uint8_t* b, const float* sa,
+                                             int64_t s_rows, const float* sb,
+                                             int first, int last) {
+  constexpr int U = 2;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  if (first >= last) return acc;
+  FewStep<FP8> now[U], next[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    now[u] = few_step<FP8>(a, b, sa, s_rows, sb, min(first + u, last - 1));
+  for (int s = first; s < last; s += U) {
+    if (s + U < last)
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        next[u] = few_step<FP8>(a, b, sa, s_rows, sb,
+                                min(s + U + u, last - 1));
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (s + u < last) few_multiply<FP8>(now[u], acc);
+#pragma unroll
+    for (int u = 0; u < U; ++u) now[u] = next[u];
+  }
+  return acc;
+}
+
+// What KS waves have of the same 16 x 16 results, added up in their order;
+// part: 1 KB of LDS a wave. The sum is for the waves with ks = 0.
+template <int KS>
+__device__ __forceinline__ f32x4 few_join(f32x4 acc, float* part, int group,
+                                          int ks, int lane) {
+  if constexpr (KS == 1) return acc;
+  f32x4* at = (f32x4*)part + group * KS * 64 + lane;
+  at[ks * 64] = acc;
+  __syncthreads();
+  f32x4 sum = at[0];
+#pragma unroll
+  for (int k = 1; k < KS; ++k) sum += at[k * 64];
+  return sum;
+}
+
 // Run q of a lane's columns in row tile i: v[c] is column
 //   run_column(q) + c,  counted from the wave's first one.
 template <class S>
