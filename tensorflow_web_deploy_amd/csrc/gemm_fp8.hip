@@ -25,53 +25,8 @@ using namespace tile;
 // ------------------------------------------------------------ quant_fp8
 
 template <typename T>
-__device__ __forceinline__ float value(const T* p) {
-  return (float)*p;
-}
-
-// 8 values from p on, the ones from `have` on as 0. The copy needs no
-// alignment: rows of an odd width start anywhere.
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, int have, float (&v)[8]) {
-  if (have >= 8) {
-    T t[8];
-    __builtin_memcpy(t, p, sizeof(t));
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = (float)t[e];
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = e < have ? value(p + e) : 0.f;
-  }
-}
-
-__device__ __forceinline__ void store_fp8(uint8_t* to, const float (&v)[8],
-                                          float s) {
-  uint32_t q[2];
-  to_fp8(v, s, q);
-  *(uint2*)to = make_uint2(q[0], q[1]);
-}
-
-// 16 lanes take a block of a row, 8 values each; 16 rows a workgroup.
-// Bound by the bytes it moves.
-template <typename T>
-__global__ __launch_bounds__(256) void quant_rows_kernel(
-    const T* __restrict__ X, int64_t ldx, int64_t M, int K,
-    uint8_t* __restrict__ Q, int Kp, float* __restrict__ S, int per) {
-  const int l = threadIdx.x & 15;
-  const int64_t m = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
-  if (m >= M) return;
-  const int end = min((int)(blockIdx.y + 1) * per, Kp / 128);
-  for (int kb = blockIdx.y * per; kb < end; ++kb) {
-    const int k = kb * 128 + l * 8;
-    float v[8];
-    load8(X + m * ldx + k, K - k, v);
-    uint32_t top = amax_bits(v);
-#pragma unroll
-    for (int d = 8; d; d >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
-    const float s = scale_of(top);
-    store_fp8(Q + m * Kp + k, v, s);
-    if (l == 0) S[kb * M + m] = s;
-  }
+__global__ __launch_bounds__(256) void quant_rows_kernel(QuantRows<T> q) {
+  q.run(blockIdx.x);
 }
 
 // One workgroup a block of 128 x 128: a weight's scales, made once.
@@ -116,56 +71,105 @@ struct Dense {
   float* part;  // split K: one f32 plane of M x N a slice
   int M, N, Kp, tiles_m, tiles_n, steps, act;
   int64_t ldc, ldr;
-  bool vec;  // rows of C (and of the residual) take 16-byte accesses
 };
 
+// what the activation's code comes to: nothing, a clamp, GELU
+enum { PLAIN, CLAMP, GELU };
+
+int kind_of(int act) { return act == 0 ? PLAIN : act == 5 ? GELU : CLAMP; }
+
 // R consecutive columns from n on of row m: + bias + residual, activation,
-// one rounding, store
-template <int R>
+// one rounding, store. WHOLE: the caller knows that they are all there.
+template <int KIND, bool RES, bool WHOLE, int R>
 __device__ __forceinline__ void finish(const Dense& d, int64_t m, int n,
-                                       float (&v)[R], const float (&b)[R]) {
+                                       float (&v)[R], const float (&b)[R],
+                                       const __bf16 (&res)[R]) {
 #pragma unroll
   for (int e = 0; e < R; ++e) v[e] += b[e];
-  const bool whole = d.vec && n + R <= d.N;
-  if (d.residual) {
-    const __bf16* r = d.residual + m * d.ldr + n;
-    if (whole) {
-      __bf16 t[R];
-      __builtin_memcpy(t, __builtin_assume_aligned(r, 16), sizeof(t));
+  if constexpr (RES) {
 #pragma unroll
-      for (int e = 0; e < R; ++e) v[e] += (float)t[e];
-    } else {
-#pragma unroll
-      for (int e = 0; e < R; ++e)
-        if (n + e < d.N) v[e] += (float)r[e];
-    }
+    for (int e = 0; e < R; ++e) v[e] += (float)res[e];
   }
-  activate_by(v, d.act);
-  __bf16* c = d.C + m * d.ldc + n;
-  if (whole) {
-    __bf16 t[R];
+  if constexpr (KIND == CLAMP) {
+    const float high = d.act == 2 ? 6.f : INFINITY;
 #pragma unroll
-    for (int e = 0; e < R; ++e) t[e] = (__bf16)v[e];
-    __builtin_memcpy(__builtin_assume_aligned(c, 16), t, sizeof(t));
+    for (int e = 0; e < R; ++e)
+      v[e] = v[e] < 0.f ? 0.f : v[e] > high ? high : v[e];
+  } else if constexpr (KIND == GELU) {
+    activate_all<5>(v);
+  }
+  __bf16 t[R];
+#pragma unroll
+  for (int e = 0; e < R; ++e) t[e] = (__bf16)v[e];
+  __bf16* c = d.C + m * d.ldc + n;
+  if (WHOLE || n + R <= d.N) {
+    __builtin_memcpy(c, t, sizeof(t));  // rows may start anywhere
   } else {
 #pragma unroll
     for (int e = 0; e < R; ++e)
-      if (n + e < d.N) c[e] = (__bf16)v[e];
+      if (n + e < d.N) c[e] = t[e];
   }
 }
 
-template <class S, bool SPLIT>
-__global__ __launch_bounds__(S::THREADS, 2) void gemm_fp8_kernel(Dense d) {
-  extern __shared__ __attribute__((aligned(16))) char smem[];
+template <bool WHOLE, int R>
+__device__ __forceinline__ void load_residual(const Dense& d, int64_t m, int n,
+                                              __bf16 (&res)[R]) {
+  const __bf16* r = d.residual + m * d.ldr + n;
+  if (WHOLE || n + R <= d.N) {
+    __builtin_memcpy(res, r, sizeof(res));
+  } else {
+#pragma unroll
+    for (int e = 0; e < R; ++e) res[e] = n + e < d.N ? r[e] : (__bf16)0.f;
+  }
+}
+
+// A tile's result. A tile that is all there takes a straight way without a
+// test: with them, and with a choice of activations in it, this took 6 us of
+// the 14 that a tile of 6 steps takes.
+template <class S, int KIND, bool RES, bool WHOLE>
+__device__ __forceinline__ void finish_tile(const Dense& d, int64_t m0, int n0,
+                                            int lane,
+                                            f32x4 (&acc)[S::MT][S::NT]) {
+#pragma unroll
+  for (int q = 0; q < S::RUNS; ++q) {
+    const int n = n0 + run_column<S>(q, lane);
+    if (!WHOLE && n >= d.N) continue;
+    float b[S::W] = {};
+    if (d.bias) load_run(d.bias + n, WHOLE ? S::W : d.N - n, b);
+    __bf16 res[S::MT][S::W];
+    if constexpr (RES) {
+#pragma unroll
+      for (int i = 0; i < S::MT; ++i) {
+        const int64_t m = m0 + i * 16 + (lane & 15);
+        if (WHOLE || m < d.M) load_residual<WHOLE>(d, m, n, res[i]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < S::MT; ++i) {
+      const int64_t m = m0 + i * 16 + (lane & 15);
+      if (!WHOLE && m >= d.M) continue;
+      float v[S::W];
+      run_of<S>(acc[i], q, v);
+      finish<KIND, RES, WHOLE>(d, m, n, v, b, res[i]);
+    }
+  }
+}
+
+struct DenseTile {
+  int64_t m0;  // the tile's rows and columns, and the wave's own
+  int n0, wave_m, wave_n;
+};
+
+// the tile of this workgroup, `count` steps from `first` on
+template <class S>
+__device__ __forceinline__ DenseTile dense_tile(
+    const Dense& d, char* smem, int first, int count,
+    f32x4 (&acc)[S::MT][S::NT]) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Place tile = place_of(blockIdx.x, d.tiles_m, d.tiles_n);
   const int64_t m0 = (int64_t)tile.m * S::BM;
-  const int n0 = tile.n * S::BN;
-  const int all = d.Kp / STEP;
-  const int first = SPLIT ? blockIdx.y * d.steps : 0;
-  const int count = SPLIT ? min(d.steps, all - first) : all;
-
+  const int n0 = tile.n * S::BN, all = d.Kp / STEP;
   const int rows = (int)min((int64_t)S::BM, d.M - m0);
   const int cols = min(S::BN, d.N - n0);
   const auto ra = buffer(d.A + m0 * d.Kp, (uint32_t)rows * d.Kp);
@@ -176,33 +180,66 @@ __global__ __launch_bounds__(S::THREADS, 2) void gemm_fp8_kernel(Dense d) {
       [&](int r) { return (uint32_t)min(r, rows - 1) * d.Kp; },
       [&](int r) { return (uint32_t)min(r, cols - 1) * d.Kp; },
       [&](int r) { return (uint32_t)(m0 + min(r, rows - 1)) * 4; });
-  const int wm = wave / S::WN, wn = wave % S::WN;
-  const int wave_n0 = n0 + wn * S::NT * 16;
-  const int top_block = (d.N - 1) / 128;
-  f32x4 acc[S::MT][S::NT];
+  const int wave_m = wave / S::WN * S::MT * 16;
+  const int wave_n = wave % S::WN * S::NT * 16;
   product<S>(smem, ra, rb, rs, at, first, count, (uint32_t)d.M * 4,
-                    d.SB + (int64_t)min(wave_n0 / 128, top_block) * all, wave,
-                    lane, acc);
+             d.SB + (int64_t)min((n0 + wave_n) / 128, (d.N - 1) / 128) * all,
+             wave, lane, acc);
+  return {m0, n0, wave_m, wave_n};
+}
 
+template <class S, int KIND, bool RES>
+__global__ __launch_bounds__(S::THREADS, 2) void gemm_fp8_kernel(Dense d) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  f32x4 acc[S::MT][S::NT];
+  const auto t = dense_tile<S>(d, smem, 0, d.Kp / STEP, acc);
+  const int lane = threadIdx.x & 63;
+  if (t.m0 + S::BM <= d.M && t.n0 + S::BN <= d.N)
+    finish_tile<S, KIND, RES, true>(d, t.m0 + t.wave_m, t.n0 + t.wave_n, lane,
+                                    acc);
+  else
+    finish_tile<S, KIND, RES, false>(d, t.m0 + t.wave_m, t.n0 + t.wave_n, lane,
+                                     acc);
+}
+
+// split K: the f32 sums of slice blockIdx.y
+template <class S>
+__global__ __launch_bounds__(S::THREADS, 2) void gemm_fp8_slice_kernel(
+    Dense d) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int first = blockIdx.y * d.steps;
+  f32x4 acc[S::MT][S::NT];
+  const auto t =
+      dense_tile<S>(d, smem, first, min(d.steps, d.Kp / STEP - first), acc);
+  const int lane = threadIdx.x & 63;
 #pragma unroll
   for (int q = 0; q < S::RUNS; ++q) {
-    const int n = wave_n0 + run_column<S>(q, lane);
-    if (n >= d.N) continue;
-    float b[S::W];
-    load_run(d.bias + n, !SPLIT && d.bias ? d.N - n : 0, b);
+    const int n = t.n0 + t.wave_n + run_column<S>(q, lane);
 #pragma unroll
     for (int i = 0; i < S::MT; ++i) {
-      const int64_t m = m0 + wm * S::MT * 16 + i * 16 + (lane & 15);
+      const int64_t m = t.m0 + t.wave_m + i * 16 + (lane & 15);
       if (m >= d.M) continue;
       float v[S::W];
       run_of<S>(acc[i], q, v);
-      if (SPLIT)
-        store_run(d.part + ((int64_t)blockIdx.y * d.M + m) * d.N + n, d.N - n,
-                  v);
-      else
-        finish(d, m, n, v, b);
+      store_run(d.part + ((int64_t)blockIdx.y * d.M + m) * d.N + n, d.N - n,
+                v);
     }
   }
+}
+
+// 4 columns of a row, whatever the layer has
+__device__ __forceinline__ void finish4(const Dense& d, int64_t m, int n,
+                                        float (&v)[4]) {
+  float b[4];
+  load_run(d.bias + n, d.bias ? d.N - n : 0, b);
+  __bf16 res[4] = {};
+  if (d.residual) load_residual<false>(d, m, n, res);
+  if (d.act == 0)
+    finish<PLAIN, true, false>(d, m, n, v, b, res);
+  else if (d.act == 5)
+    finish<GELU, true, false>(d, m, n, v, b, res);
+  else
+    finish<CLAMP, true, false>(d, m, n, v, b, res);
 }
 
 // up to 16 rows: 16 columns a workgroup, K cut into 8 parts, a wave each
@@ -219,11 +256,8 @@ __global__ __launch_bounds__(512, 4) void gemm_fp8_few_kernel(Dense d) {
   const f32x4 sum = few_join<8>(acc, part, 0, wave, lane);
   const int m = lane & 15, n = n0 + (lane >> 4) * 4;
   if (wave || m >= d.M || n >= d.N) return;
-  float v[4] = {sum[0], sum[1], sum[2], sum[3]}, b[4];
-  load_run(d.bias + n, d.bias ? d.N - n : 0, b);
-  Dense one = d;
-  one.vec = false;
-  finish(one, m, n, v, b);
+  float v[4] = {sum[0], sum[1], sum[2], sum[3]};
+  finish4(d, m, n, v);
 }
 
 // split K: adds up the slices, in their order, and finishes the layer
@@ -234,17 +268,14 @@ __global__ __launch_bounds__(256) void gemm_fp8_join_kernel(Dense d,
   if (t >= (int64_t)d.M * per) return;
   const int64_t m = t / per;
   const int n = (int)(t - m * per) * 4;
-  float v[4] = {0.f, 0.f, 0.f, 0.f}, b[4];
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
   for (int s = 0; s < slices; ++s) {
     float w[4];
     load_run(d.part + ((int64_t)s * d.M + m) * d.N + n, d.N - n, w);
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] += w[e];
   }
-  load_run(d.bias + n, d.bias ? d.N - n : 0, b);
-  Dense one = d;
-  one.vec = false;
-  finish(one, m, n, v, b);
+  finish4(d, m, n, v);
 }
 
 template <int W>
@@ -264,16 +295,36 @@ void run(Dense d, int slices, hipStream_t stream) {
   d.tiles_m = up(d.M, S::BM);
   d.tiles_n = up(d.N, S::BN);
   const dim3 grid(d.tiles_m * d.tiles_n, slices);
-  if (slices == 1) {
-    hipLaunchKernelGGL((gemm_fp8_kernel<S, false>), grid,
-                       dim3(S::THREADS), S::LDS, stream, d);
+  if (slices > 1) {
+    hipLaunchKernelGGL((gemm_fp8_slice_kernel<P>), grid, dim3(P::THREADS),
+                       P::LDS, stream, d);
+    const int64_t work = (int64_t)d.M * ((d.N + 3) / 4);
+    hipLaunchKernelGGL(gemm_fp8_join_kernel, dim3(up(work, 256)), dim3(256),
+                       0, stream, d, slices);
     return;
   }
-  hipLaunchKernelGGL((gemm_fp8_kernel<P, true>), grid, dim3(P::THREADS),
-                     P::LDS, stream, d);
-  const int64_t work = (int64_t)d.M * ((d.N + 3) / 4);
-  hipLaunchKernelGGL(gemm_fp8_join_kernel, dim3(up(work, 256)), dim3(256),
-                     0, stream, d, slices);
+  auto go = [&](auto kind, auto res) {
+    hipLaunchKernelGGL(
+        (gemm_fp8_kernel<S, decltype(kind)::value, decltype(res)::value>),
+        grid, dim3(S::THREADS), S::LDS, stream, d);
+  };
+  auto by_residual = [&](auto kind) {
+    if (d.residual)
+      go(kind, std::true_type());
+    else
+      go(kind, std::false_type());
+  };
+  switch (kind_of(d.act)) {
+    case PLAIN:
+      by_residual(std::integral_constant<int, PLAIN>());
+      break;
+    case CLAMP:
+      by_residual(std::integral_constant<int, CLAMP>());
+      break;
+    case GELU:
+      by_residual(std::integral_constant<int, GELU>());
+      break;
+  }
 }
 
 enum class Way { FEW, TILE64, TILE128, TILE256 };
@@ -303,12 +354,10 @@ void launch_quant_fp8(const void* X, bool f32, int64_t ldx, int64_t M, int K,
   auto go = [&](const auto* x) {
     using T = std::remove_cv_t<std::remove_pointer_t<decltype(x)>>;
     if (block_rows == 1) {
-      const int rows = up(M, 16), kb = Kp / 128;
-      // enough workgroups to fill the chip, else whole rows
-      const int cuts = std::min(kb, std::max(1, 2048 / rows));
-      const int per = up(kb, cuts);
-      hipLaunchKernelGGL((quant_rows_kernel<T>), dim3(rows, up(kb, per)), dim3(256),
-                         0, stream, x, ldx, M, K, (uint8_t*)Q, Kp, S, per);
+      const auto q = QuantRows<T>::of(x, ldx, M, K, Q, Kp, S);
+      hipLaunchKernelGGL((quant_rows_kernel<T>),
+                         dim3((uint32_t)q.workgroups()), dim3(256), 0, stream,
+                         q);
     } else {
       hipLaunchKernelGGL((quant_tiles_kernel<T>),
                          dim3((uint32_t)(Kp / 128) * up(M, 128)), dim3(256),
@@ -346,8 +395,6 @@ void launch_gemm_fp8(const void* A, const float* SA, const void* B,
   d.act = act;
   d.ldc = ldc;
   d.ldr = ldr;
-  d.vec = (uintptr_t)C % 16 == 0 && ldc % 8 == 0 &&
-          (!residual || ((uintptr_t)residual % 16 == 0 && ldr % 8 == 0));
   const Plan p = plan(M, N, Kp);
   d.steps = p.steps;
   switch (p.way) {

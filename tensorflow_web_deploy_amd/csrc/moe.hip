@@ -551,8 +551,7 @@ __device__ __forceinline__ void load_ids(const Plan& p, int a0,
     if ((unsigned)e[i] >= (unsigned)p.E) e[i] = p.E;
 }
 
-__global__ __launch_bounds__(PLAN_THREADS) void plan_count_kernel(Plan p) {
-  extern __shared__ int count[];
+__device__ __forceinline__ void plan_count(const Plan& p, int* count) {
   int e[PLAN_EACH];
   load_ids(p, blockIdx.x * PLAN_ROWS, e);
   for (int i = threadIdx.x; i < p.E; i += PLAN_THREADS) count[i] = 0;
@@ -588,8 +587,7 @@ __device__ __forceinline__ void scan(const int* in, int* out, int n) {
 // first one lists the tiles. Which place a row gets among its workgroup's of
 // the same expert is left to chance: no result hangs on it, as a row's
 // products don't on the rows beside it.
-__global__ __launch_bounds__(PLAN_THREADS) void plan_place_kernel(Plan p) {
-  extern __shared__ int lds[];
+__device__ __forceinline__ void plan_place(const Plan& p, int* lds) {
   int* total = lds;             // [E], later tiles of each expert
   int* next = lds + p.E;        // [E]
   int* start = lds + 2 * p.E;   // [E + 1]
@@ -648,16 +646,47 @@ __global__ __launch_bounds__(PLAN_THREADS) void plan_place_kernel(Plan p) {
   if (threadIdx.x == 0) p.tiles[p.n_tiles] = make_int4(tiles, 0, 0, 0);
 }
 
-// rows of bf16 that no 16-byte load can take as they are: copied once, filled
-// up with zeros to whole steps
-__global__ __launch_bounds__(256) void pad_rows_kernel(
-    const __bf16* __restrict__ X, int64_t ldx, int D, __bf16* __restrict__ Y,
-    int Dp, int64_t n) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n) return;
-  const int64_t t = i / Dp;
-  const int c = (int)(i - t * Dp);
-  Y[i] = c < D ? X[t * ldx + c] : (__bf16)0.f;
+// Rows of bf16 that no 16-byte load can take as they are: copied once, filled
+// up with zeros to whole steps, 8 values a thread
+struct PadRows {
+  const __bf16* X;
+  int64_t ldx, T;
+  int D;
+  __bf16* Y;
+  int Dp;
+
+  int64_t workgroups() const { return (T * (Dp / 8) + 255) / 256; }
+  __device__ __forceinline__ void run(int64_t block) const {
+    const int64_t i = block * 256 + threadIdx.x, t = i / (Dp / 8);
+    if (t >= T) return;
+    const int c = (int)(i - t * (Dp / 8)) * 8;
+    float v[8];
+    load8(X + t * ldx + c, D - c, v);
+    __bf16 o[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = (__bf16)v[e];
+    __builtin_memcpy(__builtin_assume_aligned(Y + t * Dp + c, 16), o,
+                     sizeof(o));
+  }
+};
+
+// The first plan_blocks workgroups count, or place where one of them does it
+// all; the others bring the layer's input into its form in the same launch.
+template <class Rows>
+__global__ __launch_bounds__(PLAN_THREADS) void prepare_kernel(
+    Plan p, int plan_blocks, Rows rows) {
+  extern __shared__ int lds[];
+  if ((int)blockIdx.x >= plan_blocks)
+    rows.run(blockIdx.x - plan_blocks);
+  else if (p.blocks > 1)
+    plan_count(p, lds);
+  else
+    plan_place(p, lds);
+}
+
+__global__ __launch_bounds__(PLAN_THREADS) void plan_place_kernel(Plan p) {
+  extern __shared__ int lds[];
+  plan_place(p, lds);
 }
 
 // ------------------------------------------------------ grouped products
@@ -1017,6 +1046,8 @@ using Tile128 = Shape<FP8, 128, 128, 2, 2, 2, FIRST && FP8 ? 16 : 8>;
 // few rows an expert: what counts is how much of the weights is on its way
 template <bool FP8, bool FIRST>
 using Tile32 = Shape<FP8, 32, 128, 2, 2, 4, FIRST && FP8 ? 16 : 8>;
+template <bool FP8, bool FIRST>
+using Tile64 = Shape<FP8, 64, 128, 2, 2, 4, FIRST && FP8 ? 16 : 8>;
 
 template <class S, bool FIRST>
 void run(Experts p, hipStream_t stream) {
@@ -1041,7 +1072,7 @@ Layout layout(const MoeMlp& m) {
   Layout l{};
   const int64_t N = (int64_t)m.T * m.k;
   l.direct = N <= 8 && N <= m.E;
-  l.BM = N <= 32 * (int64_t)m.E ? 32 : 128;
+  l.BM = N <= 32 * (int64_t)m.E ? 32 : N <= 96 * (int64_t)m.E ? 64 : 128;
   l.n_tiles = (int)(N / l.BM + std::min<int64_t>(N, m.E));
   l.blocks = up(N, PLAN_ROWS);
   const int unit = m.fp8 ? 128 : 64, size = m.fp8 ? 1 : 2;
@@ -1073,12 +1104,25 @@ void run_mlp(const MoeMlp& m, const Layout& l, char* ws, hipStream_t stream) {
   const int N = m.T * m.k;
   const Plan plan{m.ids, (int*)(ws + l.counts), (int*)(ws + l.order),
             (int4*)(ws + l.tiles), N, m.E, l.BM, l.n_tiles, l.blocks};
-  if (l.blocks > 1)
-    hipLaunchKernelGGL(plan_count_kernel, dim3(l.blocks), dim3(PLAN_THREADS),
-                       m.E * 4, stream, plan);
-  if (!l.direct)
+  const int plan_lds = (4 * m.E + 2) * 4;
+  auto prepare = [&](auto rows, bool some) {
+    const int plan_blocks = l.direct ? 0 : l.blocks;
+    const int64_t blocks = plan_blocks + (some ? rows.workgroups() : 0);
+    if (blocks)
+      hipLaunchKernelGGL((prepare_kernel<decltype(rows)>),
+                         dim3((uint32_t)blocks), dim3(PLAN_THREADS), plan_lds,
+                         stream, plan, plan_blocks, rows);
+  };
+  const auto x = (const __bf16*)m.X;
+  if (FP8)
+    prepare(QuantRows<__bf16>::of(x, m.ldx, m.T, m.D, ws + l.x, l.Dp,
+                                  (float*)(ws + l.sx)),
+            true);
+  else
+    prepare(PadRows{x, m.ldx, m.T, m.D, (__bf16*)(ws + l.x), l.Dp}, l.copy);
+  if (!l.direct && l.blocks > 1)
     hipLaunchKernelGGL(plan_place_kernel, dim3(l.blocks), dim3(PLAN_THREADS),
-                       (4 * m.E + 2) * 4, stream, plan);
+                       plan_lds, stream, plan);
 
   Experts p{};
   p.tiles = plan.tiles;
@@ -1089,13 +1133,6 @@ void run_mlp(const MoeMlp& m, const Layout& l, char* ws, hipStream_t stream) {
   p.N = N;
   p.n_tiles = l.n_tiles;
   const int size = FP8 ? 1 : 2;
-  if (FP8)
-    launch_quant_fp8(m.X, false, m.ldx, m.T, m.D, ws + l.x, l.Dp,
-                     (float*)(ws + l.sx), 1, stream);
-  else if (l.copy)
-    hipLaunchKernelGGL(pad_rows_kernel, dim3(up((int64_t)m.T * l.Dp, 256)),
-                       dim3(256), 0, stream, (const __bf16*)m.X, m.ldx, m.D,
-                       (__bf16*)(ws + l.x), l.Dp, (int64_t)m.T * l.Dp);
   p.A = l.copy ? (const uint8_t*)ws + l.x : (const uint8_t*)m.X;
   p.a_row = l.copy ? (int64_t)l.Dp * size : m.ldx * 2;
   p.a_bytes = (uint32_t)((m.T - 1) * p.a_row + (int64_t)l.Dp * size);
@@ -1117,6 +1154,8 @@ void run_mlp(const MoeMlp& m, const Layout& l, char* ws, hipStream_t stream) {
                        dim3(N * p.tiles_n), dim3(512), 0, stream, p);
   } else if (l.BM == 32) {
     run<Tile32<FP8, true>, true>(p, stream);
+  } else if (l.BM == 64) {
+    run<Tile64<FP8, true>, true>(p, stream);
   } else {
     run<Tile128<FP8, true>, true>(p, stream);
   }
@@ -1144,6 +1183,8 @@ void run_mlp(const MoeMlp& m, const Layout& l, char* ws, hipStream_t stream) {
   }
   if (l.BM == 32)
     run<Tile32<FP8, false>, false>(p, stream);
+  else if (l.BM == 64)
+    run<Tile64<FP8, false>, false>(p, stream);
   else
     run<Tile128<FP8, false>, false>(p, stream);
 

@@ -56,4 +56,74 @@ __device__ __forceinline__ void to_fp8(const float (&v)[R], float s,
   }
 }
 
+// 8 values from p on, the ones from `have` on as 0. The copy needs no
+// alignment: rows of an odd width start anywhere.
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int have, float (&v)[8]) {
+  if (have >= 8) {
+    T t[8];
+    __builtin_memcpy(t, p, sizeof(t));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = (float)t[e];
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = e < have ? (float)p[e] : 0.f;
+  }
+}
+
+__device__ __forceinline__ void store_fp8(uint8_t* to, const float (&v)[8],
+                                          float s) {
+  uint32_t q[2];
+  to_fp8(v, s, q);
+  *(uint2*)to = make_uint2(q[0], q[1]);
+}
+
+// Rows to round, 16 a workgroup and `per` blocks of 128 each: 16 lanes take a
+// block of a row, 8 values each. Bound by the bytes it moves.
+template <typename T>
+struct QuantRows {
+  const T* X;
+  int64_t ldx, M;
+  int K;
+  uint8_t* Q;
+  int Kp;
+  float* S;  // [Kp / 128][M]
+  int per;
+
+  // workgroups of 256 threads, so many that they fill the chip, else whole
+  // rows
+  static QuantRows of(const T* X, int64_t ldx, int64_t M, int K, void* Q,
+                      int Kp, float* S) {
+    const int64_t rows = (M + 15) / 16, kb = Kp / 128;
+    const int64_t cuts =
+        rows >= 2048 ? 1 : kb < 2048 / rows ? kb : 2048 / rows;
+    return {X, ldx, M, K, (uint8_t*)Q, Kp, S, (int)((kb + cuts - 1) / cuts)};
+  }
+  __host__ __device__ int64_t across() const {
+    return (Kp / 128 + per - 1) / per;
+  }
+  int64_t workgroups() const { return (M + 15) / 16 * across(); }
+
+  __device__ __forceinline__ void run(int64_t block) const {
+    const int64_t rows = block / across();
+    const int kb0 = (int)(block - rows * across()) * per;
+    const int l = threadIdx.x & 15;
+    const int64_t m = rows * 16 + (threadIdx.x >> 4);
+    if (m >= M) return;
+    const int end = min(kb0 + per, Kp / 128);
+    for (int kb = kb0; kb < end; ++kb) {
+      const int k = kb * 128 + l * 8;
+      float v[8];
+      load8(X + m * ldx + k, K - k, v);
+      uint32_t top = amax_bits(v);
+#pragma unroll
+      for (int d = 8; d; d >>= 1)
+        top = max(top, (uint32_t)__shfl_xor((int)top, d));
+      const float s = scale_of(top);
+      store_fp8(Q + m * Kp + k, v, s);
+      if (l == 0) S[kb * M + m] = s;
+    }
+  }
+};
+
 }  // namespace tile
