@@ -73,11 +73,6 @@ struct Dense {
   int64_t ldc, ldr;
 };
 
-// what the activation's code comes to: nothing, a clamp, GELU
-enum { PLAIN, CLAMP, GELU };
-
-int kind_of(int act) { return act == 0 ? PLAIN : act == 5 ? GELU : CLAMP; }
-
 // R consecutive columns from n on of row m: + bias + residual, activation,
 // one rounding, store. WHOLE: the caller knows that they are all there.
 template <int KIND, bool RES, bool WHOLE, int R>
@@ -90,14 +85,7 @@ __device__ __forceinline__ void finish(const Dense& d, int64_t m, int n,
 #pragma unroll
     for (int e = 0; e < R; ++e) v[e] += (float)res[e];
   }
-  if constexpr (KIND == CLAMP) {
-    const float high = d.act == 2 ? 6.f : INFINITY;
-#pragma unroll
-    for (int e = 0; e < R; ++e)
-      v[e] = v[e] < 0.f ? 0.f : v[e] > high ? high : v[e];
-  } else if constexpr (KIND == GELU) {
-    activate_all<5>(v);
-  }
+  activate_kind<KIND>(v, d.act);
   __bf16 t[R];
 #pragma unroll
   for (int e = 0; e < R; ++e) t[e] = (__bf16)v[e];

@@ -732,11 +732,130 @@ __device__ __forceinline__ void store_terms(_Float16* to, const float (&v)[R],
   __builtin_memcpy(__builtin_assume_aligned(to, R * 2), h, sizeof(h));
 }
 
+// What becomes of a tile's result; WHOLE: all its rows and columns are there,
+// and it goes a straight way without a test.
+template <class S, bool FIRST, int KIND, bool WHOLE>
+__device__ __forceinline__ void finish_experts(
+    const Experts& p, int e, int at0, int rows, int row0, int wave_n0, int wn,
+    int lane, char* smem, f32x4 (&acc)[S::MT][S::NT]) {
+  const float* bias = p.bias ? p.bias + (int64_t)e * p.n : nullptr;
+  auto row = [&](int i) { return row0 + i * 16 + (lane & 15); };
+  auto column = [&](int q) { return wave_n0 + run_column<S>(q, lane); };
+  float b[S::RUNS][S::W] = {};
+  if (bias)
+#pragma unroll
+    for (int q = 0; q < S::RUNS; ++q)
+      load_run(bias + column(q), WHOLE ? S::W : p.n - column(q), b[q]);
+  // a run's values; what lies behind the last column is 0
+  auto values = [&](int i, int q, float(&v)[S::W]) {
+    run_of<S>(acc[i], q, v);
+#pragma unroll
+    for (int c = 0; c < S::W; ++c) v[c] += b[q][c];
+    activate_kind<KIND>(v, p.act);
+#pragma unroll
+    for (int c = 0; c < S::W; ++c)
+      if (!WHOLE && column(q) + c >= p.n) v[c] = 0.f;
+  };
+
+  if constexpr (FIRST && S::FP8) {
+    // a block of 128 columns is spread over SHARE waves: each leaves the
+    // largest value of its rows in LDS, and its values in the accumulators
+    constexpr int SHARE = 128 / (S::NT * 16);
+    uint32_t* top = (uint32_t*)smem;  // [WN][BM]
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < S::MT; ++i) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int q = 0; q < S::RUNS; ++q) {
+        float v[S::W];
+        values(i, q, v);
+        m = max(m, amax_bits(v));
+#pragma unroll
+        for (int c = 0; c < S::W; ++c)
+          acc[i][q * (S::W / 4) + c / 4][c % 4] = v[c];
+      }
+      m = max(m, (uint32_t)__shfl_xor((int)m, 16));
+      m = max(m, (uint32_t)__shfl_xor((int)m, 32));
+      if (lane < 16) top[wn * S::BM + row(i)] = m;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < S::MT; ++i) {
+      const int r = row(i);
+      uint32_t m = 0;
+#pragma unroll
+      for (int w = 0; w < SHARE; ++w)
+        m = max(m, top[(wn / SHARE * SHARE + w) * S::BM + r]);
+      if (!WHOLE && (r >= rows || wave_n0 >= p.np)) continue;
+      const float s = scale_of(m);
+#pragma unroll
+      for (int q = 0; q < S::RUNS; ++q) {
+        float v[S::W];
+        run_of<S>(acc[i], q, v);
+        uint32_t h[S::W / 4];
+        to_fp8(v, s, h);
+        uint8_t* to = (uint8_t*)p.H + (int64_t)(at0 + r) * p.np + column(q);
+        __builtin_memcpy(__builtin_assume_aligned(to, sizeof(h)), h,
+                         sizeof(h));
+      }
+      if (lane < 16 && wn % SHARE == 0)
+        p.SH[(int64_t)(wave_n0 / 128) * p.N + at0 + r] = s;
+    }
+  } else if constexpr (FIRST) {
+#pragma unroll
+    for (int q = 0; q < S::RUNS; ++q)
+#pragma unroll
+      for (int i = 0; i < S::MT; ++i) {
+        if (!WHOLE && (row(i) >= rows || column(q) >= p.np)) continue;
+        float v[S::W];
+        values(i, q, v);
+        // rounded to bf16 here: the second product takes no wider operand
+        __bf16 t[S::W];
+#pragma unroll
+        for (int c = 0; c < S::W; ++c) t[c] = (__bf16)v[c];
+        __bf16* h =
+            (__bf16*)p.H + (int64_t)(at0 + row(i)) * p.np + column(q);
+        __builtin_memcpy(__builtin_assume_aligned(h, 16), t, sizeof(t));
+      }
+  } else {
+    int a[S::MT];
+    float w[S::MT];
+#pragma unroll
+    for (int i = 0; i < S::MT; ++i)
+      a[i] = p.order[at0 + (WHOLE ? row(i) : min(row(i), rows - 1))];
+#pragma unroll
+    for (int i = 0; i < S::MT; ++i) w[i] = p.w[a[i]];
+#pragma unroll
+    for (int i = 0; i < S::MT; ++i) {
+      if (!WHOLE && row(i) >= rows) continue;
+      uint32_t top = 0;
+      float v[S::RUNS][S::W];
+#pragma unroll
+      for (int q = 0; q < S::RUNS; ++q) {
+        values(i, q, v[q]);
+#pragma unroll
+        for (int c = 0; c < S::W; ++c) v[q][c] *= w[i];
+        top = max(top, amax_bits(v[q]));
+      }
+      top = max(top, (uint32_t)__shfl_xor((int)top, 16));
+      top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+      const int up = power_over(top);
+#pragma unroll
+      for (int q = 0; q < S::RUNS; ++q)
+        if (WHOLE || column(q) < p.np)
+          store_terms(p.Y + (int64_t)a[i] * p.np + column(q), v[q], up);
+      if (lane < 16 && (WHOLE || wave_n0 < p.np))
+        p.SY[(int64_t)a[i] * (p.np / 64) + wave_n0 / 64] = power(up);
+    }
+  }
+}
+
 // The rows of one tile, all of one expert, times its weights. FIRST: rows are
 // gathered by token, the result is activated, rounded to the layer's type and
 // kept in the order of the experts. Otherwise: rows as they lie, the result
 // is weighted and goes to its assignment's place, in f32.
-template <class S, bool FIRST>
+template <class S, bool FIRST, int KIND>
 __global__ __launch_bounds__(S::THREADS, 2) void experts_kernel(Experts p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x & 63;
@@ -781,120 +900,13 @@ __global__ __launch_bounds__(S::THREADS, 2) void experts_kernel(Experts p) {
                     : nullptr,
              wave, lane, acc);
 
-  const float* bias = p.bias ? p.bias + (int64_t)e * p.n : nullptr;
-  auto row = [&](int i) { return wm * S::MT * 16 + i * 16 + (lane & 15); };
-  auto column = [&](int q) { return wave_n0 + run_column<S>(q, lane); };
-  auto load_bias = [&](int q, float(&b)[S::W]) {
-    load_run(bias + column(q), bias ? p.n - column(q) : 0, b);
-  };
-
-  if constexpr (FIRST) {
-    // activated in place; the columns that only fill up H stay 0
-#pragma unroll
-    for (int q = 0; q < S::RUNS; ++q) {
-      float b[S::W];
-      load_bias(q, b);
-#pragma unroll
-      for (int i = 0; i < S::MT; ++i) {
-        float v[S::W];
-        run_of<S>(acc[i], q, v);
-#pragma unroll
-        for (int c = 0; c < S::W; ++c) v[c] += b[c];
-        activate_by(v, p.act);
-#pragma unroll
-        for (int c = 0; c < S::W; ++c)
-          acc[i][q * (S::W / 4) + c / 4][c % 4] =
-              column(q) + c < p.n ? v[c] : 0.f;
-      }
-    }
-  }
-  if constexpr (FIRST && S::FP8) {
-    // a block of 128 columns is spread over SHARE waves: each leaves the
-    // largest value of its rows in LDS
-    constexpr int SHARE = 128 / (S::NT * 16);
-    uint32_t* top = (uint32_t*)smem;  // [WN][BM]
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < S::MT; ++i) {
-      uint32_t m = 0;
-#pragma unroll
-      for (int q = 0; q < S::RUNS; ++q) {
-        float v[S::W];
-        run_of<S>(acc[i], q, v);
-        m = max(m, amax_bits(v));
-      }
-      m = max(m, (uint32_t)__shfl_xor((int)m, 16));
-      m = max(m, (uint32_t)__shfl_xor((int)m, 32));
-      if (lane < 16) top[wn * S::BM + row(i)] = m;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < S::MT; ++i) {
-      const int r = row(i);
-      uint32_t m = 0;
-#pragma unroll
-      for (int w = 0; w < SHARE; ++w)
-        m = max(m, top[(wn / SHARE * SHARE + w) * S::BM + r]);
-      if (r >= rows || wave_n0 >= p.np) continue;
-      const float s = scale_of(m);
-#pragma unroll
-      for (int q = 0; q < S::RUNS; ++q) {
-        float v[S::W];
-        run_of<S>(acc[i], q, v);
-        uint32_t h[S::W / 4];
-        to_fp8(v, s, h);
-        uint8_t* to = (uint8_t*)p.H + (int64_t)(at0 + r) * p.np + column(q);
-        __builtin_memcpy(__builtin_assume_aligned(to, sizeof(h)), h,
-                         sizeof(h));
-      }
-      if (lane < 16 && wn % SHARE == 0)
-        p.SH[(int64_t)(wave_n0 / 128) * p.N + at0 + r] = s;
-    }
-  } else if constexpr (FIRST) {
-#pragma unroll
-    for (int q = 0; q < S::RUNS; ++q)
-#pragma unroll
-      for (int i = 0; i < S::MT; ++i) {
-        if (row(i) >= rows || column(q) >= p.np) continue;
-        float v[S::W];
-        run_of<S>(acc[i], q, v);
-        // rounded to bf16 here: the second product takes no wider operand
-        __bf16 t[S::W];
-#pragma unroll
-        for (int c = 0; c < S::W; ++c) t[c] = (__bf16)v[c];
-        __bf16* h =
-            (__bf16*)p.H + (int64_t)(at0 + row(i)) * p.np + column(q);
-        __builtin_memcpy(__builtin_assume_aligned(h, 16), t, sizeof(t));
-      }
-  } else {
-#pragma unroll
-    for (int i = 0; i < S::MT; ++i) {
-      if (row(i) >= rows) continue;
-      const int a = p.order[at0 + row(i)];
-      const float w = p.w[a];
-      uint32_t top = 0;
-      float v[S::RUNS][S::W];
-#pragma unroll
-      for (int q = 0; q < S::RUNS; ++q) {
-        float b[S::W];
-        load_bias(q, b);
-        run_of<S>(acc[i], q, v[q]);
-#pragma unroll
-        for (int c = 0; c < S::W; ++c)
-          v[q][c] = column(q) + c < p.n ? (v[q][c] + b[c]) * w : 0.f;
-        top = max(top, amax_bits(v[q]));
-      }
-      top = max(top, (uint32_t)__shfl_xor((int)top, 16));
-      top = max(top, (uint32_t)__shfl_xor((int)top, 32));
-      const int up = power_over(top);
-#pragma unroll
-      for (int q = 0; q < S::RUNS; ++q)
-        if (column(q) < p.np)
-          store_terms(p.Y + (int64_t)a * p.np + column(q), v[q], up);
-      if (lane < 16 && wave_n0 < p.np)
-        p.SY[(int64_t)a * (p.np / 64) + wave_n0 / 64] = power(up);
-    }
-  }
+  const int row0 = wm * S::MT * 16;
+  if (rows == S::BM && n0 + S::BN <= p.n)
+    finish_experts<S, FIRST, KIND, true>(p, e, at0, rows, row0, wave_n0, wn,
+                                         lane, smem, acc);
+  else
+    finish_experts<S, FIRST, KIND, false>(p, e, at0, rows, row0, wave_n0, wn,
+                                          lane, smem, acc);
 }
 
 // Without a plan, the first product: CW * 16 columns of an assignment a
@@ -927,7 +939,7 @@ __global__ __launch_bounds__(512, 4) void experts_hidden_kernel(Experts p) {
   load_run(p.bias + (int64_t)e * p.n + n, p.bias ? p.n - n : 0, b);
 #pragma unroll
   for (int c = 0; c < 4; ++c) v[c] += b[c];
-  activate_by(v, p.act);
+  activate(v, p.act);
 #pragma unroll
   for (int c = 0; c < 4; ++c)
     if (n + c >= p.n) v[c] = 0.f;
@@ -1049,11 +1061,23 @@ using Tile32 = Shape<FP8, 32, 128, 2, 2, 4, FIRST && FP8 ? 16 : 8>;
 template <bool FP8, bool FIRST>
 using Tile64 = Shape<FP8, 64, 128, 2, 2, 4, FIRST && FP8 ? 16 : 8>;
 
-template <class S, bool FIRST>
+template <class S, bool FIRST, int KIND>
 void run(Experts p, hipStream_t stream) {
   p.tiles_n = up(FIRST ? p.np : p.n, S::BN);
-  hipLaunchKernelGGL((experts_kernel<S, FIRST>), dim3(p.n_tiles * p.tiles_n),
+  hipLaunchKernelGGL((experts_kernel<S, FIRST, KIND>), dim3(p.n_tiles * p.tiles_n),
                      dim3(S::THREADS), S::LDS, stream, p);
+}
+
+template <class S>
+void run_first(Experts p, hipStream_t stream) {
+  switch (kind_of(p.act)) {
+    case PLAIN:
+      return run<S, true, PLAIN>(p, stream);
+    case CLAMP:
+      return run<S, true, CLAMP>(p, stream);
+    case GELU:
+      return run<S, true, GELU>(p, stream);
+  }
 }
 
 int64_t up256(int64_t bytes) { return (bytes + 255) & ~int64_t(255); }
@@ -1072,7 +1096,9 @@ Layout layout(const MoeMlp& m) {
   Layout l{};
   const int64_t N = (int64_t)m.T * m.k;
   l.direct = N <= 8 && N <= m.E;
-  l.BM = N <= 32 * (int64_t)m.E ? 32 : N <= 96 * (int64_t)m.E ? 64 : 128;
+  const int64_t tiles = (N / 128 + std::min<int64_t>(N, m.E)) *
+                        up(std::min(m.D, m.H), 128);
+  l.BM = N <= 32 * (int64_t)m.E ? 32 : tiles < 512 ? 64 : 128;
   l.n_tiles = (int)(N / l.BM + std::min<int64_t>(N, m.E));
   l.blocks = up(N, PLAN_ROWS);
   const int unit = m.fp8 ? 128 : 64, size = m.fp8 ? 1 : 2;
@@ -1153,11 +1179,11 @@ void run_mlp(const MoeMlp& m, const Layout& l, char* ws, hipStream_t stream) {
     hipLaunchKernelGGL((experts_hidden_kernel<FP8, CW, 8 / CW>),
                        dim3(N * p.tiles_n), dim3(512), 0, stream, p);
   } else if (l.BM == 32) {
-    run<Tile32<FP8, true>, true>(p, stream);
+    run_first<Tile32<FP8, true>>(p, stream);
   } else if (l.BM == 64) {
-    run<Tile64<FP8, true>, true>(p, stream);
+    run_first<Tile64<FP8, true>>(p, stream);
   } else {
-    run<Tile128<FP8, true>, true>(p, stream);
+    run_first<Tile128<FP8, true>>(p, stream);
   }
 
   p.A = (const uint8_t*)ws + l.h;
@@ -1182,11 +1208,11 @@ void run_mlp(const MoeMlp& m, const Layout& l, char* ws, hipStream_t stream) {
     return;
   }
   if (l.BM == 32)
-    run<Tile32<FP8, false>, false>(p, stream);
+    run<Tile32<FP8, false>, false, PLAIN>(p, stream);
   else if (l.BM == 64)
-    run<Tile64<FP8, false>, false>(p, stream);
+    run<Tile64<FP8, false>, false, PLAIN>(p, stream);
   else
-    run<Tile128<FP8, false>, false>(p, stream);
+    run<Tile128<FP8, false>, false, PLAIN>(p, stream);
 
   const int64_t work = (int64_t)m.T * up(m.D, 8);
   const bool vec = (uintptr_t)m.Y % 16 == 0 && m.ldy % 8 == 0 &&

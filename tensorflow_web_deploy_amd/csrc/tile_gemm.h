@@ -421,29 +421,34 @@ __device__ __forceinline__ float gelu(float v) {
   return v * (v < 0.f ? h : 1.f - h);
 }
 
-// 0 none, 1 relu, 2 relu6, 5 erf-GELU: the codes of the bf16 GEMM
-template <int ACT>
-__device__ __forceinline__ float activate(float v) {
-  if (ACT == 1) return v < 0.f ? 0.f : v;
-  if (ACT == 2) return v < 0.f ? 0.f : v > 6.f ? 6.f : v;
-  if (ACT == 5) return gelu(v);
-  return v;
+// What an activation's code comes to: nothing, a clamp, GELU. Kernels of many
+// rows are made for one of them.
+enum { PLAIN, CLAMP, GELU };
+
+inline int kind_of(int act) {
+  return act == 0 ? PLAIN : act == 5 ? GELU : CLAMP;
 }
 
-template <int ACT, int R>
-__device__ __forceinline__ void activate_all(float (&v)[R]) {
+template <int KIND, int R>
+__device__ __forceinline__ void activate_kind(float (&v)[R], int act) {
+  if constexpr (KIND == CLAMP) {
+    const float high = act == 2 ? 6.f : INFINITY;
 #pragma unroll
-  for (int e = 0; e < R; ++e) v[e] = activate<ACT>(v[e]);
+    for (int e = 0; e < R; ++e)  // NaN stays
+      v[e] = v[e] < 0.f ? 0.f : v[e] > high ? high : v[e];
+  } else if constexpr (KIND == GELU) {
+#pragma unroll
+    for (int e = 0; e < R; ++e) v[e] = gelu(v[e]);
+  }
 }
 
+// act: 0 none, 1 relu, 2 relu6, 5 erf-GELU, the codes of the bf16 GEMM
 template <int R>
-__device__ __forceinline__ void activate_by(float (&v)[R], int act) {
-  if (act == 1)
-    activate_all<1>(v);
-  else if (act == 2)
-    activate_all<2>(v);
-  else if (act == 5)
-    activate_all<5>(v);
+__device__ __forceinline__ void activate(float (&v)[R], int act) {
+  if (act == 5)
+    activate_kind<GELU>(v, act);
+  else if (act)
+    activate_kind<CLAMP>(v, act);
 }
 
 // Workgroups go round the 8 XCDs in turn. Give each XCD a contiguous run of
