@@ -268,6 +268,9 @@ __global__ __launch_bounds__(256) void gemm_fp8_join_kernel(Dense d,
 
 template <int W>
 using Tile128 = Shape<true, 128, 128, 2, 2, 2, W>;
+// the most rows of which two workgroups' steps fit into a CU's LDS
+template <int W>
+using Tile160 = Shape<true, 160, 128, 2, 2, 2, W>;
 template <int W>
 using Tile256 = Shape<true, 256, 256, 2, 4, 2, W>;
 // rows for half a tile: what counts is how much of the weights is on its way
@@ -315,7 +318,7 @@ void run(Dense d, int slices, hipStream_t stream) {
   }
 }
 
-enum class Way { FEW, TILE64, TILE128, TILE256 };
+enum class Way { FEW, TILE64, TILE128, TILE160, TILE256 };
 
 struct Plan {
   Way way;
@@ -325,12 +328,35 @@ struct Plan {
 Plan plan(int M, int N, int Kp) {
   const int all = Kp / STEP;
   if (M <= 16) return {Way::FEW, 1, all};
-  if ((int64_t)up(M, 256) * up(N, 256) >= 256) return {Way::TILE256, 1, all};
+  // Rounds of tiles over the chip times what a tile takes, in us: about 1.7 a
+  // step and 9 beside for 256 x 256, one a CU; 0.95 and 8 for 128 x 128 and
+  // 1.15 and 9 for 160 x 128, two a CU.
+  auto cost = [&](int m, int n, int at_once, double step, double fixed) {
+    const int64_t tiles = (int64_t)up(M, m) * up(N, n);
+    return up(tiles, at_once) * (all * step + fixed);
+  };
+  const double c128 = cost(128, 128, 512, 0.95, 8);
+  const double c160 = cost(160, 128, 512, 1.15, 9);
+  const double c256 = cost(256, 256, 256, 1.7, 9);
+  if ((int64_t)up(M, 128) * up(N, 128) >= 256) {
+    const Way way = c256 < c128 && c256 < c160 ? Way::TILE256
+                    : c160 < c128              ? Way::TILE160
+                                               : Way::TILE128;
+    return {way, 1, all};
+  }
+  // Few tiles: K may be cut. A tile alone on its CU takes about 0.6 us a step
+  // and 7 beside; the slices' f32 planes go out and come back at 4 TB/s, and
+  // adding them up is a launch more, 4 us.
   const Way way = M <= 64 ? Way::TILE64 : Way::TILE128;
   const int64_t tiles = (int64_t)up(M, 128) * up(N, 128);
-  int s = 1;
-  while (tiles * s < 256 && all / (s * 2) >= 4) s *= 2;
-  const int steps = up(all, s);
+  int best = 1;
+  double least = 1e30;
+  for (int s = 1; s <= 32 && s <= all; s *= 2) {
+    const double t = up(tiles * s, 256) * (up(all, s) * 0.6 + 7) +
+                     (s > 1 ? 4 + (double)s * M * N * 8 / 4e6 : 0);
+    if (t < least) least = t, best = s;
+  }
+  const int steps = up(all, best);
   return {way, up(all, steps), steps};
 }
 
@@ -395,6 +421,9 @@ void launch_gemm_fp8(const void* A, const float* SA, const void* B,
       break;
     case Way::TILE128:
       run<Tile128>(d, p.slices, stream);
+      break;
+    case Way::TILE160:
+      run<Tile160>(d, p.slices, stream);
       break;
     case Way::TILE256:
       run<Tile256>(d, p.slices, stream);
