@@ -215,19 +215,28 @@ __global__ __launch_bounds__(S::THREADS, 2) void gemm_fp8_slice_kernel(
   }
 }
 
-// 4 columns of a row, whatever the layer has
-__device__ __forceinline__ void finish4(const Dense& d, int64_t m, int n,
-                                        float (&v)[4]) {
+// 4 columns of a row, whatever the layer has: what it adds, loaded early, and
+// the rest of the way
+struct Added4 {
   float b[4];
-  load_run(d.bias + n, d.bias ? d.N - n : 0, b);
-  __bf16 res[4] = {};
-  if (d.residual) load_residual<false>(d, m, n, res);
+  __bf16 res[4];
+};
+
+__device__ __forceinline__ Added4 added4(const Dense& d, int64_t m, int n) {
+  Added4 x{};
+  load_run(d.bias + n, d.bias ? d.N - n : 0, x.b);
+  if (d.residual) load_residual<false>(d, m, n, x.res);
+  return x;
+}
+
+__device__ __forceinline__ void finish4(const Dense& d, int64_t m, int n,
+                                        float (&v)[4], const Added4& x) {
   if (d.act == 0)
-    finish<PLAIN, true, false>(d, m, n, v, b, res);
+    finish<PLAIN, true, false>(d, m, n, v, x.b, x.res);
   else if (d.act == 5)
-    finish<GELU, true, false>(d, m, n, v, b, res);
+    finish<GELU, true, false>(d, m, n, v, x.b, x.res);
   else
-    finish<CLAMP, true, false>(d, m, n, v, b, res);
+    finish<CLAMP, true, false>(d, m, n, v, x.b, x.res);
 }
 
 // up to 16 rows: 16 columns a workgroup, K cut into 8 parts, a wave each
@@ -237,15 +246,16 @@ __global__ __launch_bounds__(512, 4) void gemm_fp8_few_kernel(Dense d) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n0 = blockIdx.x * 16, all = d.Kp / STEP;
   const int row = min(lane & 15, d.M - 1), col = min(n0 + (lane & 15), d.N - 1);
+  const int n = n0 + (lane >> 4) * 4;
+  const Added4 x = added4(d, row, n);
   const f32x4 acc = few_product<true>(
       d.A + (int64_t)row * d.Kp + (lane >> 4) * 16,
       d.B + (int64_t)col * d.Kp + (lane >> 4) * 16, d.SA + row, d.M,
       d.SB + (int64_t)(n0 / 128) * all, all * wave / 8, all * (wave + 1) / 8);
   const f32x4 sum = few_join<8>(acc, part, 0, wave, lane);
-  const int m = lane & 15, n = n0 + (lane >> 4) * 4;
-  if (wave || m >= d.M || n >= d.N) return;
+  if (wave || (lane & 15) >= d.M || n >= d.N) return;
   float v[4] = {sum[0], sum[1], sum[2], sum[3]};
-  finish4(d, m, n, v);
+  finish4(d, row, n, v, x);
 }
 
 // split K: adds up the slices, in their order, and finishes the layer
@@ -257,43 +267,44 @@ __global__ __launch_bounds__(256) void gemm_fp8_join_kernel(Dense d,
   const int64_t m = t / per;
   const int n = (int)(t - m * per) * 4;
   float v[4] = {0.f, 0.f, 0.f, 0.f};
+  const Added4 x = added4(d, m, n);
   for (int s = 0; s < slices; ++s) {
     float w[4];
     load_run(d.part + ((int64_t)s * d.M + m) * d.N + n, d.N - n, w);
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] += w[e];
   }
-  finish4(d, m, n, v);
+  finish4(d, m, n, v, x);
 }
 
 template <int W>
 using Tile128 = Shape<true, 128, 128, 2, 2, 2, W>;
 // the most rows of which two workgroups' steps fit into a CU's LDS
-template <int W>
-using Tile160 = Shape<true, 160, 128, 2, 2, 2, W>;
-template <int W>
-using Tile256 = Shape<true, 256, 256, 2, 4, 2, W>;
+using Tile160 = Shape<true, 160, 128, 2, 2, 2, 8>;
+using Tile256 = Shape<true, 256, 256, 2, 4, 2, 8>;
 // rows for half a tile: what counts is how much of the weights is on its way
 template <int W>
 using Tile64 = Shape<true, 64, 128, 2, 2, 4, W>;
 
 int up(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
-template <template <int> class T>
-void run(Dense d, int slices, hipStream_t stream) {
-  using S = T<8>;   // bf16 results
-  using P = T<4>;   // f32 slices
+template <class S>  // its lanes hold 4 columns of f32
+void run_slices(Dense d, int slices, hipStream_t stream) {
   d.tiles_m = up(d.M, S::BM);
   d.tiles_n = up(d.N, S::BN);
-  const dim3 grid(d.tiles_m * d.tiles_n, slices);
-  if (slices > 1) {
-    hipLaunchKernelGGL((gemm_fp8_slice_kernel<P>), grid, dim3(P::THREADS),
-                       P::LDS, stream, d);
-    const int64_t work = (int64_t)d.M * ((d.N + 3) / 4);
-    hipLaunchKernelGGL(gemm_fp8_join_kernel, dim3(up(work, 256)), dim3(256),
-                       0, stream, d, slices);
-    return;
-  }
+  hipLaunchKernelGGL((gemm_fp8_slice_kernel<S>),
+                     dim3(d.tiles_m * d.tiles_n, slices), dim3(S::THREADS),
+                     S::LDS, stream, d);
+  const int64_t work = (int64_t)d.M * ((d.N + 3) / 4);
+  hipLaunchKernelGGL(gemm_fp8_join_kernel, dim3(up(work, 256)), dim3(256), 0,
+                     stream, d, slices);
+}
+
+template <class S>  // 8 columns of bf16
+void run(Dense d, hipStream_t stream) {
+  d.tiles_m = up(d.M, S::BM);
+  d.tiles_n = up(d.N, S::BN);
+  const dim3 grid(d.tiles_m * d.tiles_n);
   auto go = [&](auto kind, auto res) {
     hipLaunchKernelGGL(
         (gemm_fp8_kernel<S, decltype(kind)::value, decltype(res)::value>),
@@ -417,16 +428,22 @@ void launch_gemm_fp8(const void* A, const float* SA, const void* B,
                          stream, d);
       break;
     case Way::TILE64:
-      run<Tile64>(d, p.slices, stream);
+      if (p.slices > 1)
+        run_slices<Tile64<4>>(d, p.slices, stream);
+      else
+        run<Tile64<8>>(d, stream);
       break;
     case Way::TILE128:
-      run<Tile128>(d, p.slices, stream);
+      if (p.slices > 1)
+        run_slices<Tile128<4>>(d, p.slices, stream);
+      else
+        run<Tile128<8>>(d, stream);
       break;
     case Way::TILE160:
-      run<Tile160>(d, p.slices, stream);
+      run<Tile160>(d, stream);
       break;
     case Way::TILE256:
-      run<Tile256>(d, p.slices, stream);
+      run<Tile256>(d, stream);
       break;
   }
 }

@@ -925,7 +925,10 @@ __global__ __launch_bounds__(512, 4) void experts_hidden_kernel(Experts p) {
   if ((unsigned)e >= (unsigned)p.E) return;
   const int64_t row = a / p.k;
   const int col = min(n0 + (lane & 15), p.n - 1);
+  const int n = n0 + (lane >> 4) * 4;
   const int blocks_n = (p.n + 127) / 128;
+  float b[4];  // on its way with the weights
+  load_run(p.bias + (int64_t)e * p.n + n, p.bias ? p.n - n : 0, b);
   const f32x4 acc = few_product<FP8>(
       p.A + row * p.a_row + (lane >> 4) * 16,
       p.B + ((int64_t)e * p.n + col) * ((int64_t)p.steps * STEP) +
@@ -934,9 +937,7 @@ __global__ __launch_bounds__(512, 4) void experts_hidden_kernel(Experts p) {
       p.SB + ((int64_t)e * blocks_n + min(n0 / 128, blocks_n - 1)) * p.steps,
       p.steps * ks / KS, p.steps * (ks + 1) / KS);
   const f32x4 sum = few_join<KS>(acc, part, cw, ks, lane);
-  const int n = n0 + (lane >> 4) * 4;
-  float v[4] = {sum[0], sum[1], sum[2], sum[3]}, b[4];
-  load_run(p.bias + (int64_t)e * p.n + n, p.bias ? p.n - n : 0, b);
+  float v[4] = {sum[0], sum[1], sum[2], sum[3]};
 #pragma unroll
   for (int c = 0; c < 4; ++c) v[c] += b[c];
   activate(v, p.act);
@@ -969,7 +970,8 @@ __global__ __launch_bounds__(512, 4) void experts_hidden_kernel(Experts p) {
 }
 
 // Without a plan, the second product and the sum over a token's experts: 16
-// columns of a token a workgroup. Its 16 rows are all the same one.
+// columns of a token a workgroup, its waves share the experts and, if there
+// are fewer than 8, K. The 16 rows are all the same one.
 template <bool FP8>
 __global__ __launch_bounds__(512, 4) void experts_sum_kernel(
     Experts p, const __bf16* residual, int64_t ldr, __bf16* Y, int64_t ldy) {
@@ -982,21 +984,23 @@ __global__ __launch_bounds__(512, 4) void experts_sum_kernel(
   const int n = n0 + (lane >> 4) * 4;
   const int blocks_n = (p.n + 127) / 128;
   f32x4 total = {0.f, 0.f, 0.f, 0.f};
-  for (int j = 0; j < p.k; ++j) {
+  const int parts = max(1, 8 / p.k);
+  for (int u = wave; u < p.k * parts; u += 8) {
+    const int j = u / parts, ks = u - j * parts;
     const int64_t a = t * p.k + j;
     const int e = p.ids[a];
     if ((unsigned)e >= (unsigned)p.E) continue;
+    const float w = p.w[a];
+    float b[4];
+    load_run(p.bias + (int64_t)e * p.n + n, p.bias && ks == 0 ? p.n - n : 0,
+             b);
     const f32x4 acc = few_product<FP8>(
         p.A + a * p.a_row + (lane >> 4) * 16,
         p.B + ((int64_t)e * p.n + col) * ((int64_t)p.steps * STEP) +
             (lane >> 4) * 16,
         p.SA + a, p.sa_rows,
         p.SB + ((int64_t)e * blocks_n + n0 / 128) * p.steps,
-        p.steps * wave / 8, p.steps * (wave + 1) / 8);
-    const float w = p.w[a];
-    float b[4];
-    load_run(p.bias + (int64_t)e * p.n + n,
-             p.bias && wave == 0 ? p.n - n : 0, b);
+        p.steps * ks / parts, p.steps * (ks + 1) / parts);
 #pragma unroll
     for (int c = 0; c < 4; ++c)
       total[c] = __builtin_fmaf(acc[c] + b[c], w, total[c]);
