@@ -364,6 +364,10 @@ void check_devices(c10::ArrayRef<std::pair<const torch::Tensor*, const char*>>
   }
 }
 
+// a launch holds fewer than 2^32 threads along x: with 16 rows, or a tile of
+// 128 x 128, to a workgroup of 256
+constexpr int64_t kMaxRows = 1 << 27, kMaxTiles = 1 << 24;
+
 int64_t blocks128(int64_t n) { return (n + 127) / 128; }
 
 // X [M,K] bf16|f32 -> Q [M,Kp] e4m3, Kp = K up to whole blocks of 128 (the
@@ -377,7 +381,7 @@ void quant_fp8(torch::Tensor X, torch::Tensor Q, torch::Tensor S,
               "block_rows must be 1 or 128, got ", block_rows);
   const int64_t M = X.size(0), K = X.size(1), Kb = blocks128(K);
   TORCH_CHECK(K >= 1 && K <= 1 << 22, "K must be 1 to 2^22, got ", K);
-  TORCH_CHECK(M < 1 << 30 && blocks128(M) * Kb < 1 << 30,
+  TORCH_CHECK(M < kMaxRows && blocks128(M) * Kb < kMaxTiles,
               "X is too large: ", X.sizes());
   check_whole(Q, kFp8, {M, Kb * 128}, "Q");
   check_aligned(Q, "Q");
@@ -408,9 +412,9 @@ void gemm_fp8(torch::Tensor A, torch::Tensor SA, torch::Tensor B,
   TORCH_CHECK(Kp >= 128 && Kp % 128 == 0 && Kp <= 1 << 22,
               "A must hold whole blocks of 128 along K, 2^22 values at most, "
               "got ", Kp);
-  TORCH_CHECK(N >= 1 && N < 1 << 30 && M < 1 << 30, "C is too large or empty: ",
-              C.sizes());
-  TORCH_CHECK(blocks128(M) * blocks128(N) < 1 << 30, "C is too large");
+  TORCH_CHECK(N >= 1 && N < kMaxRows && M < kMaxRows &&
+                  blocks128(M) * blocks128(N) < kMaxTiles,
+              "C is too large or has no columns: ", C.sizes());
   TORCH_CHECK(M * (Kp / 128) < 1 << 30, "SA is too large");
   check_whole(A, kFp8, {M, Kp}, "A");
   check_whole(SA, torch::kFloat32, {Kp / 128, M}, "SA");
@@ -462,7 +466,7 @@ void moe_route(torch::Tensor logits, c10::optional<torch::Tensor> bias,
   check_rows(logits, "logits");
   const int64_t T = logits.size(0), E = logits.size(1);
   TORCH_CHECK(E >= 1 && E <= 512, "1 to 512 experts, got ", E);
-  TORCH_CHECK(T < 1 << 30, "too many rows: ", T);
+  TORCH_CHECK(T < kMaxRows, "too many rows: ", T);
   TORCH_CHECK(score == 0 || score == 1,
               "score must be 0 (softmax) or 1 (sigmoid), got ", score);
   TORCH_CHECK(groups >= 1 && groups <= 64 && E % groups == 0,
@@ -494,8 +498,8 @@ void moe_route(torch::Tensor logits, c10::optional<torch::Tensor> bias,
                    (int)best, renorm, (float)scale, cur_stream());
 }
 
-// A call's rows are taken so many at a time that its workspace stays within
-// some gigabytes and every offset within 32 bits.
+// A call's rows are taken so many at a time that each part of its workspace
+// stays within 4 GiB and every offset into the rows within 32 bits.
 constexpr int64_t kMoeRows = 1 << 17;
 
 void moe_mlp(const torch::Tensor& X, const torch::Tensor& ids,
@@ -557,9 +561,10 @@ void moe_mlp(const torch::Tensor& X, const torch::Tensor& ids,
   check_devices(all);
   if (T == 0) return;
   const c10::DeviceGuard guard(X.device());
-  const int64_t chunk =
-      std::min(T, std::max<int64_t>(1, std::min(kMoeRows / k,
-                                                (int64_t(1) << 31) / (Dp * 2))));
+  const int64_t chunk = std::min(
+      {T, std::max<int64_t>(
+              1, std::min(kMoeRows, (int64_t(1) << 31) / std::max(Dp, Hp)) / k),
+       (int64_t(1) << 30) / Dp});
   MoeMlp m{};
   m.W1 = W1.data_ptr();
   m.W2 = W2.data_ptr();

@@ -246,8 +246,8 @@ __device__ __forceinline__ int expert_at(int l, int v) {
   return V >= 4 ? v / 4 * 64 + l * 4 + v % 4 : l;
 }
 
-// 16 lanes a row, 4 rows a wave: the steps across lanes stay within rows of the register file, and one
-// instruction serves 4 rows. Everything is decided in f32; a row where
+// 16 lanes a row, 4 rows a wave: the steps across lanes stay within rows of
+// the register file, and one instruction serves 4 rows. Everything is decided in f32; a row where
 // rounding could change what is chosen or its order, or whose scores leave
 // the range of f32, is then done again in 64 bits, so that the choice is that
 // of the scores in 64 bits, the lower index first among equals. That is one
@@ -713,9 +713,11 @@ struct Experts {
 };
 
 // A row's 64 columns of a term share a power of two that brings the largest
-// under 2^15, and go out in 16 bits: 2^-12 of a value is lost where the sum's
-// own rounding to bf16 loses 2^-9, and the terms, the most that a layer of
-// many rows moves, take half the bytes.
+// finite one under 2^15, and go out in 16 bits: 2^-12 of a value is lost where the sum's
+// own rounding to bf16 loses 2^-9 (a value below 2^-29 of the largest loses
+// 2^-40 of that one), and the terms, the most that a layer of many rows moves,
+// take half the bytes.
+constexpr uint32_t INF_BITS = 0x7f800000;
 __device__ __forceinline__ int power_over(uint32_t top) {  // its biased form
   return max((int)(top >> 23), 15) - 14;
 }
@@ -840,6 +842,18 @@ __device__ __forceinline__ void finish_experts(
       }
       top = max(top, (uint32_t)__shfl_xor((int)top, 16));
       top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+      if (top >= INF_BITS) {  // the columns beside it are kept all the same
+        top = 0;
+#pragma unroll
+        for (int q = 0; q < S::RUNS; ++q)
+#pragma unroll
+          for (int c = 0; c < S::W; ++c) {
+            const uint32_t u = __builtin_bit_cast(uint32_t, v[q][c]) & ~(1u << 31);
+            top = max(top, u < INF_BITS ? u : 0);
+          }
+        top = max(top, (uint32_t)__shfl_xor((int)top, 16));
+        top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+      }
       const int up = power_over(top);
 #pragma unroll
       for (int q = 0; q < S::RUNS; ++q)
@@ -854,7 +868,8 @@ __device__ __forceinline__ void finish_experts(
 // The rows of one tile, all of one expert, times its weights. FIRST: rows are
 // gathered by token, the result is activated, rounded to the layer's type and
 // kept in the order of the experts. Otherwise: rows as they lie, the result
-// is weighted and goes to its assignment's place, in f32.
+// is weighted and goes to its assignment's place, in 16 bits over a power of
+// two.
 template <class S, bool FIRST, int KIND>
 __global__ __launch_bounds__(S::THREADS, 2) void experts_kernel(Experts p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];

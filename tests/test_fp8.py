@@ -97,6 +97,12 @@ def _gemm_args(m=4, n=5, k=128, **kw):
      "residual must be"),
     ({"act": 3}, "act must be"),
     ({"act": -1}, "act must be"),
+    ({"C": torch.empty(4, 1 << 27, dtype=torch.bfloat16, device="meta")},
+     "C is too large"),
+    ({"A": torch.zeros(4 * 128 + 4).to(E4M3)[4:].view(4, 128)},
+     "A must start at a multiple of 16"),
+    ({"B": torch.zeros(5 * 128 + 8).to(E4M3)[8:].view(5, 128)},
+     "B must start at a multiple of 16"),
     ({}, "A must be on GPU"),
 ])
 def test_gemm_refuses(E, kw, word):
@@ -114,6 +120,8 @@ def test_gemm_refuses(E, kw, word):
     (torch.zeros(4, 0), (4, 0), (0, 4), 1, "K must be"),
     (torch.zeros(130, 4).t(), (4, 256), (2, 4), 1, "contiguous rows"),
     (torch.zeros(130), (4, 256), (2, 4), 1, "2D"),
+    (torch.empty(1 << 27, 1, device="meta"), (4, 128), (1, 4), 1,
+     "X is too large"),
     (torch.zeros(4, 130), (4, 256), (2, 4), 1, "on GPU"),
 ])
 def test_quant_refuses(E, x, q, s, rows, word):

@@ -122,6 +122,7 @@ def test_reference_by_hand():
     ({"kept": 0}, "kept must"),
     ({"groups": 8, "kept": 1}, "k must be"),
     ({"best": 3}, "best must"),
+    ({"logits": torch.empty(1 << 27, 8, device="meta")}, "too many rows"),
     ({}, "logits must be on GPU"),
 ])
 def test_route_refuses(E, kw, word):
@@ -491,6 +492,31 @@ def test_mlp_nan_stays_in_its_row(E, fp8):
     keep = torch.ones(40, dtype=torch.bool)
     keep[11] = keep[12] = False
     assert torch.equal(y[keep], want[keep])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("t", [2, 40, 300])
+def test_mlp_infinity_stays_in_its_column(E, fp8, t):
+    """A term that is infinite takes nothing from the columns beside it."""
+    layer = Layer(E, fp8, 4, 200, 130)
+    x, ids, w = some_rows(t, 4, 2, 200)
+    ids[:, 0] = 1
+    ids[:, 1] = 2
+    spots = {5: math.inf, 70: -math.inf, 133: math.nan}
+    for c, v in spots.items():
+        layer.b2[1, c] = v
+    got = layer(x, ids, w)
+    for c, v in spots.items():
+        layer.b2[1, c] = 0
+    zero = layer(x, ids, w)
+    for c, v in spots.items():
+        if v == v:
+            assert (got[:, c] == v * w[:, 0].sign()).all()
+        else:
+            assert got[:, c].isnan().all()
+        got[:, c] = zero[:, c]
+    layer.check(got, x, ids, w)
 
 
 @pytest.mark.gpu
