@@ -336,39 +336,41 @@ struct Plan {
   int slices, steps;  // K is cut so often that the grid fills the 256 CUs
 };
 
+// What a way costs, in us: rounds of tiles over the chip times what a tile
+// takes, its steps and what lies before and behind them. Tiles of 64 x 128
+// and of 256 x 256 lie alone on a CU. Of 128 x 128 and 160 x 128 two share
+// one, where there are more than CUs. Cutting K fills the chip where tiles are
+// few; the slices' f32 planes go out and come back at 4 TB/s, and adding them
+// up is a launch more, 4 us. Measured (tiles of 64 / 128 / 160 / 256 rows, the
+// best number of slices for each): 64 x 25088 x 4096: 26.3 / 28.4, without
+// slices 95 / 126; 512 x 4096 x 4096: 20.5 / 24.6 / 28.3 / 52.7; 2048^3:
+// 22.2 / 16.1 / 19.1 / 31.0; 12544 x 768 x 768: - / 17.3 / 14.8 / 18.1;
+// 16200 x 4096 x 8192: - / 548 / 531 / 501.
 Plan plan(int M, int N, int Kp) {
   const int all = Kp / STEP;
+  // 16 x 4096 x 4096: 6.8 us, as the best tiles of 64 rows 10.5; for 17 rows
+  // the tiles take 10.6
   if (M <= 16) return {Way::FEW, 1, all};
-  // Rounds of tiles over the chip times what a tile takes, in us: about 1.7 a
-  // step and 9 beside for 256 x 256, one a CU; 0.95 and 8 for 128 x 128 and
-  // 1.15 and 9 for 160 x 128, two a CU.
-  auto cost = [&](int m, int n, int at_once, double step, double fixed) {
-    const int64_t tiles = (int64_t)up(M, m) * up(N, n);
-    return up(tiles, at_once) * (all * step + fixed);
-  };
-  const double c128 = cost(128, 128, 512, 0.95, 8);
-  const double c160 = cost(160, 128, 512, 1.15, 9);
-  const double c256 = cost(256, 256, 256, 1.7, 9);
-  if ((int64_t)up(M, 128) * up(N, 128) >= 256) {
-    const Way way = c256 < c128 && c256 < c160 ? Way::TILE256
-                    : c160 < c128              ? Way::TILE160
-                                               : Way::TILE128;
-    return {way, 1, all};
-  }
-  // Few tiles: K may be cut. A tile alone on its CU takes about 0.6 us a step
-  // and 7 beside; the slices' f32 planes go out and come back at 4 TB/s, and
-  // adding them up is a launch more, 4 us.
-  const Way way = M <= 64 ? Way::TILE64 : Way::TILE128;
-  const int64_t tiles = (int64_t)up(M, 128) * up(N, 128);
-  int best = 1;
+  Plan best{Way::TILE128, 1, all};
   double least = 1e30;
+  auto offer = [&](Way way, int slices, int steps, int m, int n, int at_once,
+                   double step, double fixed) {
+    const int64_t tiles = (int64_t)up(M, m) * up(N, n) * slices;
+    const double t = up(tiles, at_once) * (steps * step + fixed) +
+                     (slices > 1 ? 4 + (double)slices * M * N * 8 / 4e6 : 0);
+    if (t < least) least = t, best = {way, slices, steps};
+  };
   for (int s = 1; s <= 32 && s <= all; s *= 2) {
-    const double t = up(tiles * s, 256) * (up(all, s) * 0.6 + 7) +
-                     (s > 1 ? 4 + (double)s * M * N * 8 / 4e6 : 0);
-    if (t < least) least = t, best = s;
+    const int steps = up(all, s), slices = up(all, steps);
+    offer(Way::TILE64, slices, steps, 64, 128, 256, 0.47, 3.2);
+    if ((int64_t)up(M, 128) * up(N, 128) * slices <= 256)
+      offer(Way::TILE128, slices, steps, 128, 128, 256, 0.62, 5.5);
+    else
+      offer(Way::TILE128, slices, steps, 128, 128, 512, 0.95, 8);
   }
-  const int steps = up(all, best);
-  return {way, up(all, steps), steps};
+  offer(Way::TILE160, 1, all, 160, 128, 512, 1.15, 9);
+  offer(Way::TILE256, 1, all, 256, 256, 256, 1.7, 9);
+  return best;
 }
 
 }  // namespace
