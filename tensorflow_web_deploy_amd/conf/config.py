@@ -13,6 +13,9 @@ from typing import Optional
 import yaml
 
 
+DTYPES = ("bf16", "fp8")
+
+
 @dataclass(frozen=True)
 class Config:
     # model
@@ -27,7 +30,9 @@ class Config:
     normalize: str = "unit"              # 'unit' | 'inception' | 'raw'
     # engine
     device: str = "auto"                 # 'auto' | 'cpu' | 'cuda'
-    dtype: str = "bf16"                  # gpu compute dtype
+    dtype: str = "bf16"                  # gpu compute dtype; 'fp8': products
+                                         # with dense and experts' weights in
+                                         # e4m3 with block scales, rest bf16
     use_hip_graphs: bool = True
     batch_sizes: tuple = (1, 8, 32, 64)  # pre-compiled/captured batch sizes
     # serving
@@ -40,6 +45,11 @@ class Config:
     max_wait_ms: float = 2.0
     # data parallel
     gpus: int = 1
+
+    def __post_init__(self):
+        if self.dtype not in DTYPES:
+            raise ValueError(f"dtype must be one of {', '.join(DTYPES)}, "
+                             f"got {self.dtype}")
 
     def replace(self, **kw) -> "Config":
         return dataclasses.replace(self, **kw)
@@ -64,6 +74,7 @@ def add_config_args(p: argparse.ArgumentParser) -> None:
     p.add_argument("--host", default=None)
     p.add_argument("--gpus", type=int, default=None)
     p.add_argument("--device", default=None)
+    p.add_argument("--dtype", default=None, choices=DTYPES)
     p.add_argument("--max-batch", dest="max_batch", type=int, default=None)
     p.add_argument("--max-wait-ms", dest="max_wait_ms", type=float, default=None)
     p.add_argument("--labels", dest="labels_path", default=None)

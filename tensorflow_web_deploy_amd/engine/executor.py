@@ -152,6 +152,60 @@ def _dense_nd(node, ins, consts):
     return y
 
 
+def route_experts(logits, bias, k, score="softmax", groups=1, kept=1, best=1,
+                  renorm=True, scale=1.0):
+    """The k experts of each row, the lower index first among equals, and
+    their weights; places that no expert is left for get id -1 and weight 0
+    (moe_route's definition, in plain torch ops)."""
+    shut = ~(logits > -math.inf)
+    x = logits.masked_fill(shut, -math.inf)
+    if score == "sigmoid":
+        p = torch.sigmoid(x)
+    else:
+        # an infinite logit leaves nothing to the finite ones
+        most = x.amax(-1, keepdim=True) == math.inf
+        x = torch.where(most, torch.where(x == math.inf, 0.0, -math.inf), x)
+        p = torch.softmax(x, -1)
+    p = p.masked_fill(shut, 0.0)
+    key = p if bias is None else p + bias
+    key = key.masked_fill(shut | key.isnan(), -math.inf)
+    if groups > 1:
+        parts = key.unflatten(-1, (groups, -1))
+        top = parts.sort(-1, descending=True).values[..., :best]
+        # a group with one expert left counts that one alone
+        total = torch.where(top.isinf() & (top < 0), 0.0, top).sum(-1)
+        total = total.masked_fill(top[..., 0] == -math.inf, -math.inf)
+        order = total.sort(dim=-1, descending=True, stable=True).indices
+        keep = torch.zeros_like(total, dtype=torch.bool)
+        keep.scatter_(-1, order[..., :kept], True)
+        key = parts.masked_fill(~keep[..., None], -math.inf).flatten(-2)
+    chosen, ids = key.sort(dim=-1, descending=True, stable=True)
+    chosen, ids = chosen[..., :k], ids[..., :k]
+    none = chosen == -math.inf
+    w = p.gather(-1, ids).masked_fill(none, 0.0)
+    if renorm:
+        total = w.sum(-1, keepdim=True)
+        w = torch.where(total > 0, w / total, 0.0)
+    return ids.masked_fill(none, -1), w * scale
+
+
+@cpu_op("MoeMLP")
+def _moe_mlp(node, ins, consts):
+    a = node.attrs
+    x = ins[0].flatten(0, -2)
+    wr, w1, b1, w2, b2 = ins[1:6]
+    ids, w = route_experts(x @ wr, ins[6] if len(ins) > 6 else None, a["k"],
+                           a["score"], a["groups"], a["kept"], a["best"],
+                           a["renorm"], a["scale"])
+    act = {"none": lambda v: v, "relu": F.relu, "gelu": F.gelu}[a["act"]]
+    y = torch.zeros_like(x)
+    for e in range(w1.shape[0]):
+        rows, place = (ids == e).nonzero(as_tuple=True)
+        out = act(x[rows] @ w1[e] + b1[e]) @ w2[e] + b2[e]
+        y.index_add_(0, rows, out * w[rows, place, None])
+    return y.view(ins[0].shape)
+
+
 @cpu_op("Conv2D")
 def _conv_raw(node, ins, consts):
     return _conv2d(ins[0], ins[1], node.attrs["strides"],

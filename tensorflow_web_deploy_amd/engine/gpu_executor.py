@@ -52,7 +52,9 @@ def _pad64(n):
 # ops a side-stream chain may contain (pure native-kernel steps with no
 # torch temporaries — keeps graph capture and the caching allocator
 # trivially safe on side streams). MatMul-family included for ViT's
-# 3-way Q/K/V fork (each projection fills only ~0.6 blocks/CU alone).
+# 3-way Q/K/V fork (each projection fills only ~0.6 blocks/CU alone);
+# what gemm_fp8 may need for its slices it takes from the allocator's
+# pool of the stream that it runs on.
 _CHAIN_OPS = ("ConvBlock", "DepthwiseConvBlock", "MaxPool", "AvgPool",
               "MatMul", "Dense", "DenseND")
 
@@ -116,6 +118,7 @@ class GpuExecutor:
         self.device = torch.device(device)
         self.cfg = cfg
         self.use_graphs = bool(getattr(cfg, "use_hip_graphs", True))
+        self.fp8 = getattr(cfg, "dtype", "bf16") == "fp8"
         self._weights: Dict[str, tuple] = {}
         self._plans: Dict[int, "_Plan"] = {}
         self.consts = graph.consts
@@ -169,6 +172,53 @@ class GpuExecutor:
         t = torch.from_numpy(wt).to(self.device, torch.bfloat16).contiguous()
         self._weights[key] = (t, K, N, Kp, Np)
         return self._weights[key]
+
+    def _quant_weight(self, w: torch.Tensor):
+        """[N, K] -> e4m3 [N, K up to whole blocks of 128] and its scales"""
+        N, K = w.shape
+        kb = _ceil_div(K, 128)
+        q = torch.empty(N, kb * 128, dtype=torch.float8_e4m3fn,
+                        device=self.device)
+        s = torch.empty(_ceil_div(N, 128), kb, device=self.device)
+        ext().quant_fp8(w.to(self.device).contiguous(), q, s, 128)
+        return q, s
+
+    def _prep_dense_weight_fp8(self, wname: str, transpose_b: bool):
+        key = wname + ("/T" if transpose_b else "") + "/fp8"
+        if key not in self._weights:
+            w = torch.from_numpy(np.ascontiguousarray(
+                self.consts[wname], np.float32))
+            self._weights[key] = self._quant_weight(w if transpose_b
+                                                    else w.t())
+        return self._weights[key]
+
+    def _prep_expert_weight(self, wname: str):
+        """[E, K, N] -> [E, N, K filled up with zeros] and, in e4m3, the
+        scales of each expert"""
+        key = wname + "/experts"
+        if key in self._weights:
+            return self._weights[key]
+        w = torch.from_numpy(np.ascontiguousarray(
+            self.consts[wname], np.float32)).transpose(1, 2)
+        if self.fp8:
+            q, s = zip(*(self._quant_weight(e) for e in w))
+            self._weights[key] = torch.stack(q), torch.stack(s)
+        else:
+            E_, N, K = w.shape
+            t = torch.zeros(E_, N, _pad64(K), dtype=torch.bfloat16,
+                            device=self.device)
+            t[..., :K] = w.to(self.device)
+            self._weights[key] = t, None
+        return self._weights[key]
+
+    def _is_dense(self, node: Node) -> bool:
+        """rows times a weight that is known now"""
+        if node.op in ("BatchMatMul", "BatchMatMulV2"):
+            w = self.consts.get(node.inputs[1])
+            return (w is not None and w.ndim == 2
+                    and not node.attrs.get("adj_x")
+                    and not node.attrs.get("adj_y"))
+        return node.op in ("Dense", "DenseND")
 
     def _bias(self, bname: Optional[str], n: int):
         if not bname:
@@ -261,14 +311,54 @@ class GpuExecutor:
                 c0 += w
             concat_fused[n.name] = c0
 
+        # fp8: rows that dense layers read are rounded once for all of
+        # them, in a step of the node that made them
+        rounded: Dict[str, tuple] = {}
+
+        def round_rows(name):
+            if not self.fp8 or name not in bufs or not any(
+                    self._is_dense(c) and c.inputs[0] == name
+                    for c in consumer_nodes.get(name, [])):
+                return
+            K = shapes[name][-1]
+            X = bufs[name].view(-1, K)
+            M, kb = X.shape[0], _ceil_div(K, 128)
+            q = torch.zeros((M, kb * 128), dtype=torch.float8_e4m3fn,
+                            device=dev)
+            s = torch.zeros((kb, M), device=dev)
+            rounded[name] = q, s
+            steps.append(lambda: E.quant_fp8(X, q, s, 1))
+
+        round_rows(inp)
+        made = None
         fused_skip: set = set()
         pending_attn: Dict[str, tuple] = {}
         spans: List[tuple] = []  # (node name, first step idx) per node
         for node in g.nodes:
             op = node.op
+            if made is not None:
+                round_rows(made)
+            made = node.name
             spans.append((node.name, len(steps)))
             if node.name in fused_skip:
                 # consumed by the fused-attention step
+                continue
+            if self.fp8 and self._is_dense(node):
+                q, qs = rounded[node.inputs[0]]
+                wt, ws = self._prep_dense_weight_fp8(
+                    node.inputs[1], bool(node.attrs.get("transpose_b")))
+                N = wt.shape[0]
+                assert q.shape[1] == wt.shape[1], \
+                    f"dense K mismatch {node.name}"
+                bias = self._bias(node.attrs.get("bias"), N)
+                act = (2 if node.attrs.get("relu6") else
+                       1 if node.attrs.get("relu") else
+                       {None: 0, "relu": ACT_RELU, "gelu": ACT_GELU}[
+                           node.attrs.get("act")])
+                Y = alloc(node.name, (*shapes[node.inputs[0]][:-1], N))
+                steps.append(lambda q=q, qs=qs, wt=wt, ws=ws,
+                             Y2=Y.view(-1, N), bias=bias, act=act:
+                             E.gemm_fp8(q, qs, wt, ws, Y2, bias, None, act))
                 continue
             if op in ("ConvBlock",):
                 xn = node.inputs[0]
@@ -451,6 +541,40 @@ class GpuExecutor:
                 steps.append(lambda A2=A2, wt=wt, Y2=Y2, bias=bias, K=K,
                              act=act:
                              E.gemm_bf16(A2, wt, Y2, bias, None, K, act))
+            elif op == "MoeMLP":
+                xn, rn, w1n, b1n, w2n, b2n = node.inputs[:6]
+                at = node.attrs
+                wr, K, NE, _, Ep = self._prep_dense_weight(rn, False)
+                A2 = bufs[xn].view(-1, K)
+                M = A2.shape[0]
+                w1, s1 = self._prep_expert_weight(w1n)
+                w2, s2 = self._prep_expert_weight(w2n)
+                b1 = self._bias(b1n, 0).view(NE, -1)
+                b2 = self._bias(b2n, 0).view(NE, -1)
+                rb = self._bias(node.inputs[6] if len(node.inputs) > 6
+                                else None, NE)
+                lg = torch.zeros((M, Ep), dtype=torch.bfloat16, device=dev)
+                ids = torch.zeros((M, int(at["k"])), dtype=torch.int32,
+                                  device=dev)
+                pw = torch.zeros(ids.shape, device=dev)
+                steps.append(lambda A2=A2, wr=wr, lg=lg, K=K:
+                             E.gemm_bf16(A2, wr, lg, None, None, K, 0))
+                how = (("softmax", "sigmoid").index(at["score"]),
+                       int(at["groups"]), int(at["kept"]), int(at["best"]),
+                       bool(at["renorm"]), float(at["scale"]))
+                steps.append(lambda lg=lg[:, :NE], rb=rb, ids=ids, pw=pw,
+                             how=how: E.moe_route(lg, rb, ids, pw, *how))
+                Y2 = alloc(node.name, shapes[xn]).view(M, K)
+                act = {"none": 0, "relu": ACT_RELU, "gelu": ACT_GELU}[
+                    at["act"]]
+                if self.fp8:
+                    steps.append(lambda a=(A2, ids, pw, w1, s1, b1, w2, s2,
+                                           b2, Y2, None, act):
+                                 E.moe_mlp_fp8(*a))
+                else:
+                    steps.append(lambda a=(A2, ids, pw, w1, b1, w2, b2, Y2,
+                                           None, act):
+                                 E.moe_mlp_bf16(*a))
             elif op in ("BatchMatMul", "BatchMatMulV2") \
                     and node.name in pending_attn:
                 At, Bk, b1v, b2v, Sv = pending_attn.pop(node.name)

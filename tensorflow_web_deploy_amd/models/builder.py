@@ -162,6 +162,32 @@ class GraphBuilder:
             y = self.bias_add(y, f"{name}/bias_add", cout)
         return y
 
+    def moe(self, x: str, name: str, dim: int, hidden: int, experts: int,
+            k: int, score: str = "softmax", groups: int = 1, kept: int = 1,
+            best: int = 1, renorm: bool = True, scale: float = 1.0,
+            act: str = "gelu", router_bias: bool = False) -> str:
+        """Mixture of experts over the last axis: a router without a bias of
+        its own scores the experts, the k best ones (router_bias added for
+        the choice alone; out of the `kept` groups of experts whose `best`
+        largest add up to the most) each run act(x W1 + b1) W2 + b2, and
+        their scores weight the sum."""
+        ins = [x,
+               self.weight(f"{name}/router/w", (dim, experts),
+                           scale=float(np.sqrt(1.0 / dim)))]
+        for part, i, o in (("fc1", dim, hidden), ("fc2", hidden, dim)):
+            ins.append(self.weight(f"{name}/{part}/w", (experts, i, o),
+                                   scale=float(np.sqrt(1.0 / i))))
+            ins.append(self.const(
+                f"{name}/{part}/b", (0.01 * self.rng.standard_normal(
+                    (experts, o))).astype(np.float32)))
+        if router_bias:
+            ins.append(self.const(
+                f"{name}/router/bias", (0.01 * self.rng.standard_normal(
+                    experts)).astype(np.float32)))
+        return self.node("MoeMLP", name, ins, k=k, score=score, groups=groups,
+                         kept=kept, best=best, renorm=renorm,
+                         scale=float(scale), act=act)
+
     def softmax(self, x: str, name: str = "softmax") -> str:
         return self.node("Softmax", name, [x])
 

@@ -111,7 +111,9 @@ def _mlp(b: GraphBuilder, x: str, name: str) -> str:
     return b.node("AddV2", f"{name}/fc2/bias", [y, b2])
 
 
-def build_vit_b16(seed: int = 0, num_classes: int = NUM_CLASSES):
+def build_vit_b16(seed: int = 0, num_classes: int = NUM_CLASSES,
+                  experts: int = 0, experts_per_token: int = 2):
+    """experts > 0: every second layer's MLP is a mixture of that many."""
     b = GraphBuilder(seed=seed)
     x = b.placeholder(INPUT_NAME, [-1, 224, 224, 3])
     y = b.conv2d(x, "patch_embed", 16, 16, 3, DIM, 16, "VALID")
@@ -126,7 +128,11 @@ def build_vit_b16(seed: int = 0, num_classes: int = NUM_CLASSES):
         att = _attention(b, ln1, f"layer{i}/attn")
         y = b.node("AddV2", f"layer{i}/res1", [att, y])
         ln2 = _layernorm(b, y, f"layer{i}/ln2", DIM)
-        mlp = _mlp(b, ln2, f"layer{i}/mlp")
+        if experts and i % 2:
+            mlp = b.moe(ln2, f"layer{i}/moe", DIM, MLP, experts,
+                        experts_per_token)
+        else:
+            mlp = _mlp(b, ln2, f"layer{i}/mlp")
         y = b.node("AddV2", f"layer{i}/res2", [mlp, y])
     y = _layernorm(b, y, "final_ln", DIM)
     ax = b.const("gap/axis", np.array([1], np.int32))

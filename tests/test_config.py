@@ -36,3 +36,17 @@ def test_labels_default_and_file(tmp_path):
     labs = load_labels(str(f), 5)
     assert labs[0] == "cat" and labs[2] == "fish"
     assert len(labs) == 5  # padded to num_classes
+
+
+def test_dtype():
+    assert Config().dtype == "bf16"
+    p = argparse.ArgumentParser()
+    add_config_args(p)
+    assert config_from_args(p.parse_args(["--dtype", "fp8"])).dtype == "fp8"
+    assert config_from_args(p.parse_args([])).dtype == "bf16"
+    with pytest.raises(SystemExit):
+        p.parse_args(["--dtype", "fp4"])
+    with pytest.raises(ValueError, match="dtype must be one of"):
+        Config(dtype="int8")
+    with pytest.raises(ValueError, match="dtype must be one of"):
+        Config().replace(dtype="fp32")

@@ -266,6 +266,26 @@ def test_gemm(E, m, n, k):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("act,residual", [(0, True), (5, False), (2, True)])
+@pytest.mark.parametrize("m,n,k", [(12500, 761, 128), (4000, 4055, 4096),
+                                   (6200, 768, 256), (500, 2000, 1024)])
+def test_gemm_many_tiles(E, m, n, k, act, residual):
+    """Some of the rows, among them each tile's first and last ones."""
+    qa, sa, qb, sb = operands(E, m, n, k, seed=m)
+    bias = torch.randn(n, device="cuda")
+    res = (torch.randn(m, n, device="cuda").to(torch.bfloat16) if residual
+           else None)
+    c = torch.full((m, n), math.nan, dtype=torch.bfloat16, device="cuda")
+    E.gemm_fp8(qa, sa, qb, sb, c, bias, res, act)
+    assert not c.isnan().any()
+    rows = sorted({0, 1, 63, 64, 127, 128, 159, 160, 255, 256, m - 130, m - 2,
+                   m - 1, *range(5, m, m // 10)})
+    check_gemm(c[rows], qa.view(torch.uint8)[rows].view(E4M3),
+               sa[:, rows], qb, sb, bias, None if res is None else res[rows],
+               act)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("act", [0, 1, 2, 5])
 @pytest.mark.parametrize("m,n,k", [(3, 40, 256), (64, 96, 4096),
                                    (200, 250, 384)])

@@ -417,6 +417,20 @@ def test_mlp(E, t, e, k, d, h, fp8):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("t,e,k,d,h", [
+    (16, 20, 1, 200, 136), (8, 70, 4, 72, 200), (3, 40, 5, 100, 100),
+    (2000, 5, 1, 490, 700), (1000, 5, 2, 1000, 990)])
+def test_mlp_every_way(E, t, e, k, d, h, fp8):
+    """Without a plan for up to 32 assignments, tiles of 64 and 128 rows."""
+    layer = Layer(E, fp8, e, d, h)
+    x, ids, w = some_rows(t, e, k, d)
+    res = torch.randn(t, d, device="cuda").to(torch.bfloat16)
+    for act in (0, 1, 5):
+        layer.check(layer(x, ids, w, res, act), x, ids, w, res, act)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fp8", [False, True])
 @pytest.mark.parametrize("act", [0, 1, 2, 5])
 @pytest.mark.parametrize("t", [3, 150])
 def test_mlp_epilogue(E, fp8, act, t):
