@@ -737,6 +737,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("host_register", [](int64_t ptr, int64_t bytes) {
     hipError_t e = hipHostRegister(reinterpret_cast<void*>(ptr),
                                    (size_t)bytes, hipHostRegisterDefault);
+    // a refusal is the answer, not an error for the next call to report
+    if (e != hipSuccess) (void)hipGetLastError();
     return e == hipSuccess;
   });
   m.def("host_unregister", [](int64_t ptr) {
