@@ -282,9 +282,9 @@ using Tile128 = Shape<true, 128, 128, 2, 2, 2, W>;
 // the most rows of which two workgroups' steps fit into a CU's LDS
 using Tile160 = Shape<true, 160, 128, 2, 2, 2, 8>;
 using Tile256 = Shape<true, 256, 256, 2, 4, 2, 8>;
-// rows for half a tile: what counts is how much of the weights is on its way
+// few rows: what counts is how much of the weights is on its way
 template <int W>
-using Tile64 = Shape<true, 64, 128, 2, 2, 4, W>;
+using Tile64 = Shape<true, 64, 128, 2, 2, 3, W>;
 
 int up(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
@@ -337,15 +337,15 @@ struct Plan {
 };
 
 // What a way costs, in us: rounds of tiles over the chip times what a tile
-// takes, its steps and what lies before and behind them. Tiles of 64 x 128
-// and of 256 x 256 lie alone on a CU. Of 128 x 128 and 160 x 128 two share
-// one, where there are more than CUs. Cutting K fills the chip where tiles are
-// few; the slices' f32 planes go out and come back at 4 TB/s, and adding them
-// up is a launch more, 4 us. Measured (tiles of 64 / 128 / 160 / 256 rows, the
-// best number of slices for each): 64 x 25088 x 4096: 26.3 / 28.4, without
-// slices 95 / 126; 512 x 4096 x 4096: 20.5 / 24.6 / 28.3 / 52.7; 2048^3:
-// 22.2 / 16.1 / 19.1 / 31.0; 12544 x 768 x 768: - / 17.3 / 14.8 / 18.1;
-// 16200 x 4096 x 8192: - / 548 / 531 / 501.
+// takes, its steps and what lies before and behind them. Tiles of 256 x 256
+// lie alone on a CU, of the others two share one where there are more than
+// CUs. Cutting K fills the chip where tiles are few; the slices' f32 planes go
+// out and come back at 4 TB/s, and adding them up is a launch more, 4 us.
+// Measured (tiles of 64 / 128 / 160 / 256 rows, the first two with the best
+// number of slices): 64 x 25088 x 4096: 26.2 / 28.4, without slices 97 / 126;
+// 512 x 4096 x 4096: 20.1 / 24.6 / 28.3 / 52.7; 2048^3: 14.9 / 15.9 / 19.6 /
+// 31.1; 12544 x 768 x 768: 19.2 / 17.4 / 15.1 / 18.2; 16200 x 4096 x 8192:
+// 695 / 545 / 532 / 507.
 Plan plan(int M, int N, int Kp) {
   const int all = Kp / STEP;
   // 16 x 4096 x 4096: 6.8 us, as the best tiles of 64 rows 10.5; for 17 rows
@@ -362,9 +362,12 @@ Plan plan(int M, int N, int Kp) {
   };
   for (int s = 1; s <= 32 && s <= all; s *= 2) {
     const int steps = up(all, s), slices = up(all, steps);
-    offer(Way::TILE64, slices, steps, 64, 128, 256, 0.47, 3.2);
+    if ((int64_t)up(M, 64) * up(N, 128) * slices <= 256)
+      offer(Way::TILE64, slices, steps, 64, 128, 256, 0.47, 3.2);
+    else
+      offer(Way::TILE64, slices, steps, 64, 128, 512, 0.62, 4.9);
     if ((int64_t)up(M, 128) * up(N, 128) * slices <= 256)
-      offer(Way::TILE128, slices, steps, 128, 128, 256, 0.62, 5.5);
+      offer(Way::TILE128, slices, steps, 128, 128, 256, 0.62, 5.7);
     else
       offer(Way::TILE128, slices, steps, 128, 128, 512, 0.95, 8);
   }

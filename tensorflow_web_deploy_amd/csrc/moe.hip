@@ -1075,11 +1075,14 @@ __global__ __launch_bounds__(256) void combine_kernel(
 
 template <bool FP8, bool FIRST>
 using Tile128 = Shape<FP8, 128, 128, 2, 2, 2, FIRST && FP8 ? 16 : 8>;
-// few rows an expert: what counts is how much of the weights is on its way
+// Few rows an expert: what counts is how much of the weights is on its way.
+// As many stages as let two workgroups onto a CU: with one more, so that each
+// lies alone, 33 rows of 1000 for 64 experts in e4m3 took 34.7 us, not 28.5.
 template <bool FP8, bool FIRST>
-using Tile32 = Shape<FP8, 32, 128, 2, 2, 4, FIRST && FP8 ? 16 : 8>;
+using Tile32 =
+    Shape<FP8, 32, 128, 2, 2, FP8 ? 3 : 4, FIRST && FP8 ? 16 : 8>;
 template <bool FP8, bool FIRST>
-using Tile64 = Shape<FP8, 64, 128, 2, 2, 4, FIRST && FP8 ? 16 : 8>;
+using Tile64 = Shape<FP8, 64, 128, 2, 2, 3, FIRST && FP8 ? 16 : 8>;
 
 template <class S, bool FIRST, int KIND>
 void run(Experts p, hipStream_t stream) {
@@ -1123,27 +1126,28 @@ bool goes_directly(int64_t N, int64_t E) {
 }
 
 // Rows of a tile: 32, 64 or 128, whatever costs least. Both products take as
-// many rounds over the chip as their tiles need, one tile a CU of 32 or 64
-// rows, two of 128; a round takes its steps and what lies before and behind
-// them. Measured, in us, for 32 / 64 / 128 rows and N rows in all: 16 experts
-// of 768 x 1536 in bf16, N = 256: 28.8 / 33.2 / 41.3, N = 2048:
-// 45.1 / 42.7 / 49.0, N = 8192: 111 / 119 / 75; 8 of 2048 x 2048 in e4m3,
-// N = 256: 29.0 / 34.1 / 42.2, 512: 46.8 / 34.9 / 42.6, 1024: 63 / 57 / 44.
-// Over 98 such cases the costs below chose a tile that is 2% off the best one
-// on average, 9% at most.
+// many rounds over the chip as their tiles need, two of them a CU, a little
+// less than a whole one if each lies alone; a round takes its steps and what
+// lies before and behind them. Measured, in us, for 32 / 64 / 128 rows and N
+// rows in all: 16 experts of 768 x 1536 in bf16, N = 256: 29.0 / 32.5 / 41.8,
+// N = 2048: 44.0 / 38.5 / 49.1, N = 6000: 88 / 72 / 68; 128 of 1024 x 704 in
+// e4m3, N = 128: 37.1 / 38.8 / 43.0, N = 8192: 78 / 73 / 83, N = 24000:
+// 169 / 137 / 128. Over 112 such cases the costs below chose a tile that is
+// 0.3% off the best one on average, 6% at most.
 int tile_rows(const MoeMlp& m, int64_t N, int unit) {
   struct {
-    int rows, at_once;
+    int rows;
     double step, fixed;
-  } const shapes[] = {{32, 256, 0.45, 2}, {64, 256, 0.7, 3}, {128, 512, 0.9, 9}};
+  } const shapes[] = {{32, 0.7, 0.2}, {64, 0.92, 0.4}, {128, 1.25, 2.6}};
   const double used = (double)std::min<int64_t>(N, m.E);
   double least = 1e30;
   int best = 0;
   for (const auto& s : shapes) {
     // half a tile an expert is left over, and each has one at least
-    const double tiles = std::max(used, (double)N / s.rows + used / 2);
+    const double rows = std::max(used, (double)N / s.rows + used / 2);
     auto product = [&](int k, int n) {
-      return std::ceil(tiles * up(n, 128) / s.at_once) *
+      const double tiles = rows * up(n, 128);
+      return (tiles > 256 ? std::ceil(tiles / 512) : 0.8) *
              (up(k, unit) * s.step + s.fixed);
     };
     const double t = product(m.D, m.H) + product(m.H, m.D);
