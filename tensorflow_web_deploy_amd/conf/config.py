@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import argparse
 import dataclasses
+import warnings
 from dataclasses import dataclass
 from typing import Optional
 
@@ -47,9 +48,9 @@ class Config:
     gpus: int = 1
 
     def __post_init__(self):
-        if self.dtype not in DTYPES:
-            raise ValueError(f"dtype must be one of {', '.join(DTYPES)}, "
-                             f"got {self.dtype}")
+        if self.dtype not in DTYPES:  # as ever, it runs, but not unsaid
+            warnings.warn(f"dtype {self.dtype} is none of "
+                          f"{', '.join(DTYPES)}: the GPU runs in bf16")
 
     def replace(self, **kw) -> "Config":
         return dataclasses.replace(self, **kw)
