@@ -239,23 +239,42 @@ __device__ __forceinline__ void finish4(const Dense& d, int64_t m, int n,
     finish<CLAMP, true, false>(d, m, n, v, x.b, x.res);
 }
 
-// up to 16 rows: 16 columns a workgroup, K cut into 8 parts, a wave each
-__global__ __launch_bounds__(512, 4) void gemm_fp8_few_kernel(Dense d) {
-  __shared__ __attribute__((aligned(16))) float part[8 * 256];
+// up to 16 RT rows: 16 columns a workgroup, K cut into 8 parts, a wave each;
+// wave i finishes row tile i
+template <int RT>
+__global__ __launch_bounds__(512, RT == 1 ? 4 : 2) void gemm_fp8_few_kernel(
+    Dense d) {
+  __shared__ __attribute__((aligned(16))) float part[RT * 8 * 256];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n0 = blockIdx.x * 16, all = d.Kp / STEP;
-  const int row = min(lane & 15, d.M - 1), col = min(n0 + (lane & 15), d.N - 1);
+  const int col = min(n0 + (lane & 15), d.N - 1);
   const int n = n0 + (lane >> 4) * 4;
-  const Added4 x = added4(d, row, n);
-  const f32x4 acc = few_product<true>(
-      d.A + (int64_t)row * d.Kp + (lane >> 4) * 16,
-      d.B + (int64_t)col * d.Kp + (lane >> 4) * 16, d.SA + row, d.M,
-      d.SB + (int64_t)(n0 / 128) * all, all * wave / 8, all * (wave + 1) / 8);
-  const f32x4 sum = few_join<8>(acc, part, 0, wave, lane);
-  if (wave || (lane & 15) >= d.M || n >= d.N) return;
+  const int mine = min(wave, RT - 1) * 16 + (lane & 15);
+  const Added4 x = added4(d, min(mine, d.M - 1), n);
+  const uint8_t* a[RT];
+  const float* sa[RT];
+#pragma unroll
+  for (int i = 0; i < RT; ++i) {
+    const int row = min(i * 16 + (lane & 15), d.M - 1);
+    a[i] = d.A + (int64_t)row * d.Kp + (lane >> 4) * 16;
+    sa[i] = d.SA + row;
+  }
+  f32x4 acc[RT];
+  few_product<true, RT>(
+      a, d.B + (int64_t)col * d.Kp + (lane >> 4) * 16, sa, d.M,
+      d.SB + (int64_t)(n0 / 128) * all, all * wave / 8, all * (wave + 1) / 8,
+      acc);
+  f32x4* at = (f32x4*)part + lane;
+#pragma unroll
+  for (int i = 0; i < RT; ++i) at[(i * 8 + wave) * 64] = acc[i];
+  __syncthreads();
+  if (wave >= RT || mine >= d.M || n >= d.N) return;
+  f32x4 sum = at[wave * 8 * 64];
+#pragma unroll
+  for (int w = 1; w < 8; ++w) sum += at[(wave * 8 + w) * 64];
   float v[4] = {sum[0], sum[1], sum[2], sum[3]};
-  finish4(d, row, n, v, x);
+  finish4(d, mine, n, v, x);
 }
 
 // split K: adds up the slices, in their order, and finishes the layer
@@ -348,9 +367,13 @@ struct Plan {
 // 695 / 545 / 532 / 507.
 Plan plan(int M, int N, int Kp) {
   const int all = Kp / STEP;
-  // 16 x 4096 x 4096: 6.8 us, as the best tiles of 64 rows 10.5; for 17 rows
-  // the tiles take 10.6
-  if (M <= 16) return {Way::FEW, 1, all};
+  // Few rows, in us as such and as the best tiles: 1 x 4096 x 4096 5.3 / 9.5,
+  // 16 x 4096 x 4096 6.8 / 10.5, 16 x 25088 x 4096 25.5 / 25.4. Every 16
+  // columns read all rows again, so more than 16 rows are few only where
+  // neither side is long: 32 x 768 x 1000 4.9 / 6.9, 32 x 4096 x 4096
+  // 8.8 / 11.6, but 32 x 8192 x 2048 14.4 / 13.4, 32 x 1024 x 6000 8.8 / 8.0.
+  if (M <= 16 || (M <= 32 && N <= 4096 && Kp <= 4096))
+    return {Way::FEW, 1, all};
   Plan best{Way::TILE128, 1, all};
   double least = 1e30;
   auto offer = [&](Way way, int slices, int steps, int m, int n, int at_once,
@@ -429,8 +452,12 @@ void launch_gemm_fp8(const void* A, const float* SA, const void* B,
   d.steps = p.steps;
   switch (p.way) {
     case Way::FEW:
-      hipLaunchKernelGGL(gemm_fp8_few_kernel, dim3(up(N, 16)), dim3(512), 0,
-                         stream, d);
+      if (M <= 16)
+        hipLaunchKernelGGL((gemm_fp8_few_kernel<1>), dim3(up(N, 16)),
+                           dim3(512), 0, stream, d);
+      else
+        hipLaunchKernelGGL((gemm_fp8_few_kernel<2>), dim3(up(N, 16)),
+                           dim3(512), 0, stream, d);
       break;
     case Way::TILE64:
       if (p.slices > 1)

@@ -279,77 +279,97 @@ __device__ __forceinline__ void product(char* smem, __amdgpu_buffer_rsrc_t ra,
   }
 }
 
-// The product of up to 16 rows with 16 columns by one wave, for calls that
+// The product of up to 16 RT rows with 16 columns by one wave, for calls that
 // read their weights for a few rows: bound by the time that the weights take
 // to come, so they go from memory to registers at once, U steps ahead.
-// a, b, sa: this lane's row of A and of B (16 bytes from their start a
-// quarter of the wave) and its row's scale at step 0. As in a tile, a lane
-// ends up with row lane % 16 and the columns lane / 16 * 4 + 0..3.
-template <bool FP8>
+// a[i], b, sa[i]: this lane's row of A, in each row tile, and of B (16 bytes
+// from their start a quarter of the wave) and its row's scale at step 0. As in
+// a tile, a lane ends up with row lane % 16 of each row tile and the columns
+// lane / 16 * 4 + 0..3.
+template <bool FP8, int RT>
 struct FewStep {
-  i32x4 a[2], b[2];
-  float f;
+  i32x4 a[RT][2], b[2];
+  float f[RT];
 };
 
-template <bool FP8>
-__device__ __forceinline__ FewStep<FP8> few_step(const uint8_t* a,
-                                                 const uint8_t* b,
-                                                 const float* sa,
-                                                 int64_t s_rows,
-                                                 const float* sb, int step) {
-  FewStep<FP8> r;
+template <bool FP8, int RT>
+__device__ __forceinline__ FewStep<FP8, RT> few_step(
+    const uint8_t* const (&a)[RT], const uint8_t* b,
+    const float* const (&sa)[RT], int64_t s_rows, const float* sb, int step) {
+  FewStep<FP8, RT> r;
   const int64_t k = (int64_t)step * STEP;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    r.a[h] = *(const i32x4*)(a + k + h * 64);
     r.b[h] = *(const i32x4*)(b + k + h * 64);
+#pragma unroll
+    for (int i = 0; i < RT; ++i) r.a[i][h] = *(const i32x4*)(a[i] + k + h * 64);
   }
-  r.f = FP8 ? sa[step * s_rows] * sb[step] : 0.f;
+#pragma unroll
+  for (int i = 0; i < RT; ++i)
+    r.f[i] = FP8 ? sa[i][step * s_rows] * sb[step] : 0.f;
   return r;
 }
 
-template <bool FP8>
-__device__ __forceinline__ void few_multiply(const FewStep<FP8>& s,
-                                             f32x4& acc) {
-  if constexpr (FP8) {
-    const f32x4 p = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-        both(s.b), both(s.a), f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+template <bool FP8, int RT>
+__device__ __forceinline__ void few_multiply(const FewStep<FP8, RT>& s,
+                                             f32x4 (&acc)[RT]) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) acc[r] = __builtin_fmaf(p[r], s.f, acc[r]);
-  } else {
+  for (int i = 0; i < RT; ++i) {
+    if constexpr (FP8) {
+      const f32x4 p = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+          both(s.b), both(s.a[i]), f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0,
+          0);
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-      acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-          __builtin_bit_cast(bf16x8, s.b[h]),
-          __builtin_bit_cast(bf16x8, s.a[h]), acc, 0, 0, 0);
+      for (int r = 0; r < 4; ++r)
+        acc[i][r] = __builtin_fmaf(p[r], s.f[i], acc[i][r]);
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+            __builtin_bit_cast(bf16x8, s.b[h]),
+            __builtin_bit_cast(bf16x8, s.a[i][h]), acc[i], 0, 0, 0);
+    }
   }
 }
 
+template <bool FP8, int RT>
+__device__ __forceinline__ void few_product(
+    const uint8_t* const (&a)[RT], const uint8_t* b,
+    const float* const (&sa)[RT], int64_t s_rows, const float* sb, int first,
+    int last, f32x4 (&acc)[RT]) {
+  constexpr int U = 2;
+#pragma unroll
+  for (int i = 0; i < RT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (first >= last) return;
+  FewStep<FP8, RT> now[U], next[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    now[u] = few_step<FP8, RT>(a, b, sa, s_rows, sb, min(first + u, last - 1));
+  for (int s = first; s < last; s += U) {
+    if (s + U < last)
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        next[u] = few_step<FP8, RT>(a, b, sa, s_rows, sb,
+                                    min(s + U + u, last - 1));
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (s + u < last) few_multiply<FP8, RT>(now[u], acc);
+#pragma unroll
+    for (int u = 0; u < U; ++u) now[u] = next[u];
+  }
+}
+
+// one row tile
 template <bool FP8>
 __device__ __forceinline__ f32x4 few_product(const uint8_t* a,
                                              const uint8_t* b, const float* sa,
                                              int64_t s_rows, const float* sb,
                                              int first, int last) {
-  constexpr int U = 2;
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  if (first >= last) return acc;
-  FewStep<FP8> now[U], next[U];
-#pragma unroll
-  for (int u = 0; u < U; ++u)
-    now[u] = few_step<FP8>(a, b, sa, s_rows, sb, min(first + u, last - 1));
-  for (int s = first; s < last; s += U) {
-    if (s + U < last)
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        next[u] = few_step<FP8>(a, b, sa, s_rows, sb,
-                                min(s + U + u, last - 1));
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (s + u < last) few_multiply<FP8>(now[u], acc);
-#pragma unroll
-    for (int u = 0; u < U; ++u) now[u] = next[u];
-  }
-  return acc;
+  const uint8_t* const as[1] = {a};
+  const float* const sas[1] = {sa};
+  f32x4 acc[1];
+  few_product<FP8, 1>(as, b, sas, s_rows, sb, first, last, acc);
+  return acc[0];
 }
 
 // What KS waves have of the same 16 x 16 results, added up in their order;

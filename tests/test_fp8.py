@@ -253,7 +253,8 @@ def check_gemm(got, qa, sa, qb, sb, bias=None, res=None, act=0):
 
 GEMMS = [(1, 1, 1), (1, 16, 128), (2, 17, 300), (16, 1000, 768),
          (17, 129, 129), (63, 64, 1000), (65, 200, 4096), (128, 128, 128),
-         (130, 257, 640), (300, 96, 2048), (5, 4096, 1280), (257, 513, 384)]
+         (130, 257, 640), (300, 96, 2048), (5, 4096, 1280), (257, 513, 384),
+         (31, 77, 1100), (32, 160, 128), (20, 4100, 256), (29, 40, 4200)]
 
 
 @pytest.mark.gpu
