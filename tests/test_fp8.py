@@ -381,3 +381,58 @@ def test_layer_on_a_stream_and_in_a_graph(E):
         torch.cuda.synchronize()
         assert torch.equal(got, eager)
         check_gemm(got, q, s, qb, sb, None, None, 5)
+
+
+# ------------------------------------------------- offsets past 32 bits
+
+
+def far_rows(m, n, apart, dtype=torch.bfloat16):
+    """Rows of n values that lie `apart` from each other."""
+    return torch.empty((m - 1) * apart + n, dtype=dtype,
+                       device="cuda").as_strided((m, n), (apart, 1))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("block_rows", [1, 128])
+def test_quant_far_rows(E, block_rows):
+    x = far_rows(20, 200, 2 ** 28 + 3)
+    x.copy_(torch.randn(20, 200, device="cuda"))
+    check_quant(x.clone(), *run_quant(E, x, block_rows), block_rows)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,k", [(12, 256), (40, 256), (40, 8192)])
+def test_gemm_far_rows(E, m, k):
+    ops = operands(E, m, 70, k)
+    c, res = (far_rows(m, 70, 2 ** 28 + 5) for _ in range(2))
+    res.copy_(torch.randn(m, 70, device="cuda"))
+    E.gemm_fp8(*ops, c, None, res, 0)
+    check_gemm(c.clone(), *ops, None, res.clone(), 0)
+
+
+@pytest.mark.gpu
+def test_gemm_operands_past_4_gb(E):
+    n = 2 ** 25 + 5
+    g = torch.Generator("cuda").manual_seed(1)
+    long = torch.randint(0, 256, (n, 128), generator=g, device="cuda",
+                         dtype=torch.uint8)
+    long[long & 127 == 127] = 0  # no NaN
+    long = long.view(E4M3)
+    some = [0, 1, 2 ** 24 - 1, 2 ** 25 - 1, 2 ** 25, n - 2, n - 1]
+    part = long.view(torch.uint8)[some].view(E4M3)
+    for m in (2, 40):  # as weights
+        qa, sa, _, _ = operands(E, m, 8, 128, seed=m)
+        sb = torch.rand(up128(n) // 128, 1, generator=g, device="cuda")
+        c = torch.empty(m, n, dtype=torch.bfloat16, device="cuda")
+        E.gemm_fp8(qa, sa, long, sb, c)
+        # one at a time: each has a block's scale of its own
+        for i, at in enumerate(some):
+            check_gemm(c[:, at:at + 1], qa, sa,
+                       part.view(torch.uint8)[i:i + 1].view(E4M3),
+                       sb[at // 128][None])
+    del c
+    _, _, qb, sb = operands(E, 8, 16, 128)  # as rows
+    sa = torch.rand(1, n, generator=g, device="cuda")
+    c = torch.empty(n, 16, dtype=torch.bfloat16, device="cuda")
+    E.gemm_fp8(long, sa, qb, sb, c)
+    check_gemm(c[some], part, sa[:, some], qb, sb)

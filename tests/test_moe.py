@@ -12,7 +12,7 @@ import math
 import pytest
 import torch
 
-from test_fp8 import act_ref, quant_ref, up128, values64
+from test_fp8 import act_ref, far_rows, quant_ref, up128, values64
 
 E4M3 = torch.float8_e4m3fn
 
@@ -616,3 +616,71 @@ def test_two_streams_at_once(E, fp8):
     torch.cuda.synchronize()
     for o, y in zip(got, want):
         assert all(torch.equal(z, y) for z in o)
+
+
+# ------------------------------------------------- offsets past 32 bits
+
+
+@pytest.mark.gpu
+def test_route_far_rows(E):
+    x = far_rows(20, 70, 2 ** 28 + 3)
+    x.copy_(torch.randn(20, 70, device="cuda"))
+    ids, w = route(E, x, None, 5, 1)
+    again = route(E, x.clone(), None, 5, 1)
+    assert torch.equal(ids, again[0]) and torch.equal(w, again[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("t", [4, 40])
+def test_mlp_far_rows(E, fp8, t):
+    layer = Layer(E, fp8, 12, 64, 72)
+    x, ids, w = some_rows(t, 12, 2, 64)
+    apart = (2 ** 33 if t < 10 else 2 ** 29) + 8
+    v, res, y = (far_rows(t, 64, apart // 4) for _ in range(3))
+    v.copy_(x)
+    res.copy_(torch.randn(t, 64, device="cuda"))
+    layer(v, ids, w, res, 1, y)
+    layer.check(y.clone(), x, ids, w, res.clone(), 1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("t", [3, 40])
+def test_mlp_experts_past_4_gb(E, fp8, t):
+    """The last 8 of many large experts, and the same 8 alone."""
+    e, d, h = (70, 8192, 8192) if fp8 else (70, 4096, 8192)
+    g = torch.Generator("cuda").manual_seed(t)
+    w, s = [], []
+    for n, k in ((h, d), (d, h)):
+        if fp8:
+            q = torch.zeros(e, n, k, dtype=torch.uint8, device="cuda")
+            q[-8:] = torch.randint(0, 120, (8, n, k), generator=g,
+                                   device="cuda", dtype=torch.uint8)
+            w.append(q.view(E4M3))
+            s.append(torch.rand(e, n // 128, k // 128, generator=g,
+                                device="cuda") * 1e-4)
+        else:
+            q = torch.zeros(e, n, k, dtype=torch.bfloat16, device="cuda")
+            q[-8:] = torch.randn(8, n, k, generator=g, device="cuda") * k ** -.5
+            w.append(q)
+    b1, b2 = (torch.randn(e, n, generator=g, device="cuda") for n in (h, d))
+    x = torch.randn(t, d, generator=g, device="cuda").to(torch.bfloat16)
+    ids = torch.randint(0, 8, (t, 1), generator=g, device="cuda",
+                        dtype=torch.int32)
+    pw = torch.rand(t, 1, generator=g, device="cuda")
+
+    def run(first):
+        y = torch.full_like(x, math.nan)
+        a = [x, ids + (62 - first), pw]
+        for j, b in ((0, b1), (1, b2)):
+            a.append(w[j].view(torch.uint8)[first:].view(E4M3) if fp8
+                     else w[j][first:])
+            a += [s[j][first:]] if fp8 else []
+            a.append(b[first:])
+        (E.moe_mlp_fp8 if fp8 else E.moe_mlp_bf16)(*a, y, None, 1)
+        return y
+
+    y = run(0)
+    assert not y.isnan().any() and (y != 0).any(1).all()
+    assert torch.equal(y, run(62))
