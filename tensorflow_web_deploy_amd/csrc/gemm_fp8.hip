@@ -50,7 +50,8 @@ __global__ __launch_bounds__(256) void quant_tiles_kernel(
     top = max(top, amax_bits(v[i]));
   }
 #pragma unroll
-  for (int d = 32; d; d >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
+  for (int d = 32; d; d >>= 1)
+    top = max(top, (uint32_t)__shfl_xor((int)top, d));
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
   __syncthreads();
   top = max(max(part[0], part[1]), max(part[2], part[3]));
@@ -165,14 +166,15 @@ __device__ __forceinline__ DenseTile dense_tile(
   const auto ra = buffer(d.A + m0 * d.Kp, (uint32_t)rows * d.Kp);
   const auto rb = buffer(d.B + (int64_t)n0 * d.Kp, (uint32_t)cols * d.Kp);
   const auto rs = buffer(d.SA, (uint32_t)all * d.M * 4);
-  const Rows<S> at = rows_of<S>(
-      wave, lane,
-      [&](int r) { return (uint32_t)min(r, rows - 1) * d.Kp; },
-      [&](int r) { return (uint32_t)min(r, cols - 1) * d.Kp; },
-      [&](int r) { return (uint32_t)(m0 + min(r, rows - 1)) * 4; });
+  Rows<S> at;
+  rows_of_a<S>(at, wave, lane,
+               [&](int r) { return (uint32_t)min(r, rows - 1) * d.Kp; });
+  rows_of_b<S>(at, wave, lane,
+               [&](int r) { return (uint32_t)min(r, cols - 1) * d.Kp; });
+  at.s = (uint32_t)(m0 + min(scale_row<S>(wave, lane), rows - 1)) * 4;
   const int wave_m = wave / S::WN * S::MT * 16;
   const int wave_n = wave % S::WN * S::NT * 16;
-  product<S>(smem, ra, rb, rs, at, first, count, (uint32_t)d.M * 4,
+  product<S, false>(smem, ra, rb, rs, at, first, count, (uint32_t)d.M * 4,
              d.SB + (int64_t)min((n0 + wave_n) / 128, (d.N - 1) / 128) * all,
              wave, lane, acc);
   return {m0, n0, wave_m, wave_n};

@@ -113,7 +113,8 @@ void launch_quant_fp8(const void* X, bool f32, int64_t ldx, int64_t M, int K,
                       hipStream_t stream);
 // floats that launch_gemm_fp8 needs at `part`
 int64_t gemm_fp8_workspace(int M, int N, int Kp);
-// C = act(A @ B^T + bias + residual), C bf16 with row stride ldc; act: 0 none, 1 relu, 2 relu6, 5 gelu
+// C = act(A @ B^T + bias + residual), C bf16 with row stride ldc; act: 0 none,
+// 1 relu, 2 relu6, 5 gelu
 void launch_gemm_fp8(const void* A, const float* SA, const void* B,
                      const float* SB, void* C, int64_t ldc,
                      const float* bias, const void* residual, int64_t ldr,

@@ -722,10 +722,10 @@ struct Experts {
 };
 
 // A row's 64 columns of a term share a power of two that brings the largest
-// finite one under 2^15, and go out in 16 bits: 2^-12 of a value is lost where the sum's
-// own rounding to bf16 loses 2^-9 (a value below 2^-29 of the largest loses
-// 2^-40 of that one), and the terms, the most that a layer of many rows moves,
-// take half the bytes.
+// finite one under 2^15, and go out in 16 bits: 2^-12 of a value is lost where
+// the sum's own rounding to bf16 loses 2^-9 (a value below 2^-29 of the largest
+// loses 2^-40 of that one), and the terms, the most that a layer of many rows
+// moves, take half the bytes.
 constexpr uint32_t INF_BITS = 0x7f800000;
 __device__ __forceinline__ int power_over(uint32_t top) {  // its biased form
   return max((int)(top >> 23), 15) - 14;
@@ -857,7 +857,8 @@ __device__ __forceinline__ void finish_experts(
         for (int q = 0; q < S::RUNS; ++q)
 #pragma unroll
           for (int c = 0; c < S::W; ++c) {
-            const uint32_t u = __builtin_bit_cast(uint32_t, v[q][c]) & ~(1u << 31);
+            const uint32_t u =
+                __builtin_bit_cast(uint32_t, v[q][c]) & ~(1u << 31);
             top = max(top, u < INF_BITS ? u : 0);
           }
         top = max(top, (uint32_t)__shfl_xor((int)top, 16));
@@ -910,19 +911,33 @@ __global__ __launch_bounds__(S::THREADS, 2) void experts_kernel(Experts p) {
                         : buffer(p.A + at0 * p.a_row,
                                  (uint32_t)(rows * p.a_row));
   const auto rs = buffer(p.SA, p.sa_rows * 4 * p.steps);
-  // the row of A and SA behind row r of the tile
-  auto place = [&](int r) {
-    r = min(r, rows - 1);
-    return FIRST ? p.order[at0 + r] / p.k : r;
-  };
-  const Rows<S> at = rows_of<S>(
-      wave, lane, [&](int r) { return (uint32_t)(place(r) * p.a_row); },
-      [&](int r) { return (uint32_t)(min(r, cols - 1) * b_row); },
-      [&](int r) { return (uint32_t)(place(r) + (FIRST ? 0 : at0)) * 4; });
+  Rows<S> at;
+  rows_of_b<S>(at, wave, lane, [&](int r) {
+    return (uint32_t)(min(r, cols - 1) * b_row);
+  });
+  // The weights go ahead, as where the tile's rows lie is still to come: 33
+  // rows of 1000 for 64 experts in e4m3 10.5 -> 9.4 us.
+  int row[S::CA], scale = min(scale_row<S>(wave, lane), rows - 1);
+#pragma unroll
+  for (int i = 0; i < S::CA; ++i) {
+    row[i] = min(staged_row(wave, S::CA, i, lane), rows - 1);
+    if (FIRST) row[i] = p.order[at0 + row[i]];
+  }
+  scale = FIRST ? S::FP8 ? p.order[at0 + scale] : 0 : at0 + scale;
+  send_b<S>(smem, rb, at, 0, p.steps, wave);
+  if (FIRST) {
+#pragma unroll
+    for (int i = 0; i < S::CA; ++i) row[i] /= p.k;
+    scale /= p.k;
+  }
+#pragma unroll
+  for (int i = 0; i < S::CA; ++i)
+    at.a[i] = (uint32_t)(row[i] * p.a_row) + chunk_a(wave, S::CA, i, lane);
+  at.s = (uint32_t)scale * 4;
   const int wm = wave / S::WN, wn = wave % S::WN;
   const int wave_n0 = n0 + wn * S::NT * 16;
   f32x4 acc[S::MT][S::NT];
-  product<S>(smem, ra, rb, rs, at, 0, p.steps, p.sa_rows * 4,
+  product<S, true>(smem, ra, rb, rs, at, 0, p.steps, p.sa_rows * 4,
              S::FP8 ? p.SB + ((int64_t)e * blocks_n +
                               min(wave_n0 / 128, blocks_n - 1)) * p.steps
                     : nullptr,
@@ -1042,8 +1057,8 @@ __global__ __launch_bounds__(512, 4) void experts_sum_kernel(
 #pragma unroll
   for (int c = 0; c < 4; ++c)
     if (n + c < p.n)
-      Y[t * ldy + n + c] =
-          (__bf16)(sum[c] + (residual ? (float)residual[t * ldr + n + c] : 0.f));
+      Y[t * ldy + n + c] = (__bf16)(
+          sum[c] + (residual ? (float)residual[t * ldr + n + c] : 0.f));
 }
 
 // Each token adds up its experts' rows, in the order of its list: 8 columns a
@@ -1104,8 +1119,9 @@ using Tile64 = Shape<FP8, 64, 128, 2, 2, 3, FIRST && FP8 ? 16 : 8>;
 template <class S, bool FIRST, int KIND>
 void run(Experts p, hipStream_t stream) {
   p.tiles_n = up(FIRST ? p.np : p.n, S::BN);
-  hipLaunchKernelGGL((experts_kernel<S, FIRST, KIND>), dim3(p.n_tiles * p.tiles_n),
-                     dim3(S::THREADS), S::LDS, stream, p);
+  hipLaunchKernelGGL((experts_kernel<S, FIRST, KIND>),
+                     dim3(p.n_tiles * p.tiles_n), dim3(S::THREADS), S::LDS,
+                     stream, p);
 }
 
 template <class S>

@@ -94,46 +94,77 @@ __device__ __forceinline__ int staged_row(int wave, int count, int i,
   return (wave * count + i) * 8 + (lane >> 3);
 }
 
-// row_a(r), row_b(r), row_s(r): byte offset of row r of the tile, for r below
-// the tile's BM or BN
-template <class S, class A, class B, class C>
-__device__ __forceinline__ Rows<S> rows_of(int wave, int lane, A row_a,
-                                           B row_b, C row_s) {
-  Rows<S> at;
+__device__ __forceinline__ uint32_t chunk_a(int wave, int count, int i,
+                                            int lane) {
+  const int r = staged_row(wave, count, i, lane);
+  return ((lane & 7) ^ (r & 7)) << 4;
+}
+
+// row(r): byte offset of row r of the tile, for r below its BM or BN
+template <class S, class A>
+__device__ __forceinline__ void rows_of_a(Rows<S>& at, int wave, int lane,
+                                          A row) {
 #pragma unroll
   for (int i = 0; i < S::CA; ++i) {
     const int r = staged_row(wave, S::CA, i, lane);
-    at.a[i] = row_a(r) + (((lane & 7) ^ (r & 7)) << 4);
+    at.a[i] = row(r) + chunk_a(wave, S::CA, i, lane);
   }
+}
+
+template <class S, class B>
+__device__ __forceinline__ void rows_of_b(Rows<S>& at, int wave, int lane,
+                                          B row) {
 #pragma unroll
   for (int i = 0; i < S::CB; ++i) {
     const int r = staged_row(wave, S::CB, i, lane);
-    at.b[i] = row_b(r) + (((lane & 7) ^ key_b<S>(r)) << 4);
+    at.b[i] = row(r) + (((lane & 7) ^ key_b<S>(r)) << 4);
   }
-  // wave w brings the scales from row w*BM/WAVES on, 64 of them: where two
-  // waves overlap they write the same values, and what lies behind BM isn't
-  // read
-  at.s = S::FP8 ? row_s(min(wave * (S::BM / S::WAVES) + lane, S::BM - 1)) : 0;
-  return at;
 }
 
+// wave w brings the scales from row w*BM/WAVES on, 64 of them: where two waves
+// overlap they write the same values, and what lies behind BM isn't read
 template <class S>
-__device__ __forceinline__ void stage(char* lds, __amdgpu_buffer_rsrc_t ra,
-                                      __amdgpu_buffer_rsrc_t rb,
-                                      __amdgpu_buffer_rsrc_t rs,
-                                      const Rows<S>& at, int step,
-                                      uint32_t s_stride, int wave) {
+__device__ __forceinline__ int scale_row(int wave, int lane) {
+  return min(wave * (S::BM / S::WAVES) + lane, S::BM - 1);
+}
+
+// a step's rows of A and their scales
+template <class S>
+__device__ __forceinline__ void stage_a(char* lds, __amdgpu_buffer_rsrc_t ra,
+                                        __amdgpu_buffer_rsrc_t rs,
+                                        const Rows<S>& at, int step,
+                                        uint32_t s_stride, int wave) {
 #pragma unroll
   for (int i = 0; i < S::CA; ++i)
     load_lds<16>(ra, lds + (wave * S::CA + i) * 1024, at.a[i], step * STEP);
-#pragma unroll
-  for (int i = 0; i < S::CB; ++i)
-    load_lds<16>(rb, lds + S::BM * STEP + (wave * S::CB + i) * 1024, at.b[i],
-                 step * STEP);
   if (S::FP8)
     load_lds<4>(rs,
                 lds + (S::BM + S::BN) * STEP + wave * (S::BM / S::WAVES) * 4,
                 at.s, step * s_stride);
+}
+
+template <class S>
+__device__ __forceinline__ void stage_b(char* lds, __amdgpu_buffer_rsrc_t rb,
+                                        const Rows<S>& at, int step,
+                                        int wave) {
+#pragma unroll
+  for (int i = 0; i < S::CB; ++i)
+    load_lds<16>(rb, lds + S::BM * STEP + (wave * S::CB + i) * 1024, at.b[i],
+                 step * STEP);
+}
+
+// B's part of the steps that are on their way before the first is multiplied,
+// for a caller that still waits to learn which rows of A it needs. Always as
+// many, of a step that is there, so that the wait for something older needn't
+// be one for these too.
+template <class S>
+__device__ __forceinline__ void send_b(char* smem, __amdgpu_buffer_rsrc_t rb,
+                                       const Rows<S>& at, int first, int count,
+                                       int wave) {
+#pragma unroll
+  for (int j = 0; j < S::DEPTH - 1; ++j)
+    stage_b<S>(smem + j * S::STAGE, rb, at, first + min(j, count - 1), wave);
+  asm volatile("" ::: "memory");  // the waits count on this order
 }
 
 template <class S>
@@ -229,8 +260,8 @@ __device__ __forceinline__ void compute(const char* lds, float sb, int wm,
 }
 
 // Steps [first, first + count) of the product. sb: the scales of the wave's
-// columns, one a step.
-template <class S>
+// columns, one a step. B_SENT: send_b has been called.
+template <class S, bool B_SENT>
 __device__ __forceinline__ void product(char* smem, __amdgpu_buffer_rsrc_t ra,
                                         __amdgpu_buffer_rsrc_t rb,
                                         __amdgpu_buffer_rsrc_t rs,
@@ -247,9 +278,11 @@ __device__ __forceinline__ void product(char* smem, __amdgpu_buffer_rsrc_t ra,
   constexpr int AHEAD = S::DEPTH - 1;
 #pragma unroll
   for (int j = 0; j < AHEAD; ++j)
-    if (j < count)
-      stage<S>(smem + j * S::STAGE, ra, rb, rs, at, first + j,
-                     s_stride, wave);
+    if (j < count) {
+      if (!B_SENT) stage_b<S>(smem + j * S::STAGE, rb, at, first + j, wave);
+      stage_a<S>(smem + j * S::STAGE, ra, rs, at, first + j, s_stride, wave);
+      asm volatile("" ::: "memory");  // the waits count on this order
+    }
   // constant memory, so that the scale comes by a scalar load: a vector load
   // here would wait for every stage that is on its way
   const auto sbc =
@@ -259,7 +292,13 @@ __device__ __forceinline__ void product(char* smem, __amdgpu_buffer_rsrc_t ra,
   for (int j = 0; j < count; ++j) {
     // step j has landed once only the later ones are still on their way
     const int later = min(count - 1 - j, AHEAD - 1);
-    if (later >= 2)
+    // of those that send_b began, A's part alone is behind this one's
+    constexpr int PART = S::LOADS - S::CB;
+    if (B_SENT && j < AHEAD - 1 && later >= 2)
+      asm volatile("s_waitcnt vmcnt(%0)" ::"i"(2 * PART) : "memory");
+    else if (B_SENT && j < AHEAD - 1 && later == 1)
+      asm volatile("s_waitcnt vmcnt(%0)" ::"i"(PART) : "memory");
+    else if (later >= 2)
       asm volatile("s_waitcnt vmcnt(%0)" ::"i"(2 * S::LOADS) : "memory");
     else if (later == 1)
       asm volatile("s_waitcnt vmcnt(%0)" ::"i"(S::LOADS) : "memory");
@@ -267,9 +306,11 @@ __device__ __forceinline__ void product(char* smem, __amdgpu_buffer_rsrc_t ra,
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::"s"(fb) : "memory");  // here, not among the LDS reads
-    if (j + AHEAD < count)
-      stage<S>(smem + next * S::STAGE, ra, rb, rs, at, first + j + AHEAD,
-                     s_stride, wave);
+    if (j + AHEAD < count) {
+      char* to = smem + next * S::STAGE;
+      stage_a<S>(to, ra, rs, at, first + j + AHEAD, s_stride, wave);
+      stage_b<S>(to, rb, at, first + j + AHEAD, wave);
+    }
     compute<S>(smem + now * S::STAGE, fb, wm, wn, lane, acc);
     // the stage is free for the load behind the next barrier
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");

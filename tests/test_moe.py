@@ -198,7 +198,9 @@ def test_mlp_fp8_refuses_scales(E, kw):
     (70, 64, 2, 1, 1, 1), (33, 65, 6, 1, 1, 2), (17, 100, 8, 4, 2, 1),
     (40, 128, 4, 8, 3, 2), (23, 256, 8, 8, 4, 2), (11, 257, 9, 1, 1, 1),
     (13, 512, 33, 64, 20, 2), (7, 511, 64, 7, 7, 2), (6, 96, 5, 32, 5, 2),
-    (4, 6, 3, 6, 3, 2)])
+    (4, 6, 3, 6, 3, 2), (30, 256, 2, 1, 1, 1), (31, 250, 3, 10, 4, 2),
+    (50, 256, 13, 1, 1, 1), (50, 256, 14, 8, 4, 1), (19, 64, 16, 1, 1, 1),
+    (12, 300, 31, 1, 1, 1), (12, 300, 32, 3, 2, 2), (18, 14, 13, 1, 1, 1)])
 @pytest.mark.parametrize("bias", [False, True])
 def test_route(E, t, e, k, groups, kept, best, score, dtype, bias):
     g = torch.Generator().manual_seed(t * e + k)
@@ -298,7 +300,7 @@ class Layer:
 
     def __call__(self, x, ids, w, residual=None, act=0, y=None):
         if y is None:
-            y = torch.full_like(x, math.nan, memory_format=torch.contiguous_format)
+            y = torch.full(x.shape, math.nan, dtype=x.dtype, device="cuda")
         if self.fp8:
             self.E.moe_mlp_fp8(x, ids, w, self.w[0], self.s[0], self.b1,
                                self.w[1], self.s[1], self.b2, y, residual, act)
