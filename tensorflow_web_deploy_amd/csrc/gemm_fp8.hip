@@ -314,7 +314,10 @@ using Tile128 = Shape<true, 128, 128, 2, 2, 2, W>;
 // the most rows of which two workgroups' steps fit into a CU's LDS
 using Tile160 = Shape<true, 160, 128, 2, 2, 2, 8>;
 using Tile256 = Shape<true, 256, 256, 2, 4, 2, 8>;
-// few rows: what counts is how much of the weights is on its way
+// Few rows: what counts is how much of the weights is on its way. With 2
+// stages three workgroups fit on a CU instead of two, 2048^3 takes 13.8 us
+// instead of 14.7, but weights that come from HBM for one to a CU,
+// 64 x 25088 x 4096, 32.5 instead of 26.5.
 template <int W>
 using Tile64 = Shape<true, 64, 128, 2, 2, 3, W>;
 

@@ -1110,11 +1110,14 @@ using Tile128 = Shape<FP8, 128, 128, 2, 2, 2, FIRST && FP8 ? 16 : 8>;
 // Few rows an expert: what counts is how much of the weights is on its way.
 // As many stages as let two workgroups onto a CU: with one more, so that each
 // lies alone, 33 rows of 1000 for 64 experts in e4m3 took 34.7 us, not 28.5.
+// Tiles of 64 rows in e4m3 go three to a CU with 2 stages: 3000 rows of 1024,
+// 8 of 128 experts, 127 us, with 3 stages 137; in bf16 it is 186 and 189, but
+// 52 and 44 where each lies alone (256 rows of 2048, 2 of 8).
 template <bool FP8, bool FIRST>
 using Tile32 =
     Shape<FP8, 32, 128, 2, 2, FP8 ? 3 : 4, FIRST && FP8 ? 16 : 8>;
 template <bool FP8, bool FIRST>
-using Tile64 = Shape<FP8, 64, 128, 2, 2, 3, FIRST && FP8 ? 16 : 8>;
+using Tile64 = Shape<FP8, 64, 128, 2, 2, FP8 ? 2 : 3, FIRST && FP8 ? 16 : 8>;
 
 template <class S, bool FIRST, int KIND>
 void run(Experts p, hipStream_t stream) {
@@ -1159,14 +1162,15 @@ bool goes_directly(int64_t N, int64_t E) {
 }
 
 // Rows of a tile: 32, 64 or 128, whatever costs least. Both products take as
-// many rounds over the chip as their tiles need, two of them a CU, a little
-// less than a whole one if each lies alone; a round takes its steps and what
-// lies before and behind them. Measured, in us, for 32 / 64 / 128 rows and N
-// rows in all: 16 experts of 768 x 1536 in bf16, N = 256: 29.0 / 32.5 / 41.8,
-// N = 2048: 44.0 / 38.5 / 49.1, N = 6000: 88 / 72 / 68; 128 of 1024 x 704 in
-// e4m3, N = 128: 37.1 / 38.8 / 43.0, N = 8192: 78 / 73 / 83, N = 24000:
-// 169 / 137 / 128. Over 112 such cases the costs below chose a tile that is
-// 0.3% off the best one on average, 6% at most.
+// many rounds over the chip as their tiles need, two of them a CU (of 64 rows
+// in e4m3 three, which then take 1.27 times as long), a little less than a whole
+// one if each lies alone; a round takes its steps and what lies before and
+// behind them. Measured, in us, for 32 / 64 / 128 rows and N rows in all: 16
+// experts of 768 x 1536 in bf16, N = 256: 29.4 / 33.3 / 41.9, N = 2048:
+// 44.7 / 39.1 / 49.6, N = 6000: 88 / 72 / 67; 128 of 1024 x 704 in e4m3,
+// N = 128: 36.7 / 35.5 / 43.3, N = 8192: 79 / 70 / 82, N = 48000:
+// 302 / 211 / 207. Over 124 such cases the costs below chose a tile that is
+// 0.2% off the best one on average, 5% at most.
 int tile_rows(const MoeMlp& m, int64_t N, int unit) {
   struct {
     int rows;
@@ -1180,8 +1184,11 @@ int tile_rows(const MoeMlp& m, int64_t N, int unit) {
     const double rows = std::max(used, (double)N / s.rows + used / 2);
     auto product = [&](int k, int n) {
       const double tiles = rows * up(n, 128);
-      return (tiles > 256 ? std::ceil(tiles / 512) : 0.8) *
-             (up(k, unit) * s.step + s.fixed);
+      const double rounds = tiles <= 256 ? 0.8
+                            : tiles > 512 && s.rows == 64 && m.fp8
+                                ? std::ceil(tiles / 768) * 1.27
+                                : std::ceil(tiles / 512);
+      return rounds * (up(k, unit) * s.step + s.fixed);
     };
     const double t = product(m.D, m.H) + product(m.H, m.D);
     if (t < least) least = t, best = s.rows;
