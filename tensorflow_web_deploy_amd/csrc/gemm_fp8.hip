@@ -174,7 +174,7 @@ __device__ __forceinline__ DenseTile dense_tile(
   at.s = (uint32_t)(m0 + min(scale_row<S>(wave, lane), rows - 1)) * 4;
   const int wave_m = wave / S::WN * S::MT * 16;
   const int wave_n = wave % S::WN * S::NT * 16;
-  product<S, false>(smem, ra, rb, rs, at, first, count, (uint32_t)d.M * 4,
+  product<S, false, false>(smem, ra, rb, rs, at, first, count, (uint32_t)d.M * 4,
              d.SB + (int64_t)min((n0 + wave_n) / 128, (d.N - 1) / 128) * all,
              wave, lane, acc);
   return {m0, n0, wave_m, wave_n};
@@ -273,7 +273,7 @@ __global__ __launch_bounds__(512, RT == 1 ? 4 : 2) void gemm_fp8_few_kernel(
     sa[i] = d.SA + row;
   }
   f32x4 acc[RT];
-  few_product<true, RT>(
+  few_product<true, false>(
       a, d.B + (int64_t)col * d.Kp + (lane >> 4) * 16, sa, d.M,
       d.SB + (int64_t)(n0 / 128) * all, all * wave / 8, all * (wave + 1) / 8,
       acc);

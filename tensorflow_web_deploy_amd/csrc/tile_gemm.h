@@ -167,6 +167,33 @@ __device__ __forceinline__ void send_b(char* smem, __amdgpu_buffer_rsrc_t rb,
   asm volatile("" ::: "memory");  // the waits count on this order
 }
 
+// The product of two e4m3 tiles by the f16 instruction, whose sums keep what
+// f32 holds, where the 8-bit one drops what lies 2^13 under the largest of 8
+// neighbours. Half as fast, and 16 conversions a fragment.
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ f16x8 wider(int lo, int hi) {
+  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+  const f16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, false);
+  const f16x2 b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, true);
+  const f16x2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, false);
+  const f16x2 d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, true);
+  return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+__device__ __forceinline__ f32x4 exact_product(const i32x4 (&b)[2],
+                                               const i32x4 (&a)[2]) {
+  f32x4 p = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int i = 0; i < 4; i += 2)
+      p = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+          wider(b[h][i], b[h][i + 1]), wider(a[h][i], a[h][i + 1]), p, 0, 0,
+          0);
+  return p;
+}
+
 template <class S>
 struct FragA {
   i32x4 v[2];
@@ -189,7 +216,7 @@ __device__ __forceinline__ i32x8 both(const i32x4 (&v)[2]) {
   return __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-template <class S>
+template <class S, bool EXACT>
 __device__ __forceinline__ void compute(const char* lds, float sb, int wm,
                                         int wn, int lane,
                                         f32x4 (&acc)[S::MT][S::NT]) {
@@ -206,7 +233,20 @@ __device__ __forceinline__ void compute(const char* lds, float sb, int wm,
     b[t][0] = *(const i32x4*)(row + ((g ^ key) << 4));
     b[t][1] = *(const i32x4*)(row + (((g + 4) ^ key) << 4));
   }
-  if constexpr (S::FP8) {
+  if constexpr (EXACT) {
+#pragma unroll
+    for (int i = 0; i < S::MT; ++i) {
+      const FragA<S> a = read_a<S>(lds, wm, i, lane);
+      const float f = a.f * sb;
+#pragma unroll
+      for (int t = 0; t < S::NT; ++t) {
+        const f32x4 p = exact_product(b[t], a.v);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          acc[i][t][r] = __builtin_fmaf(p[r], f, acc[i][t][r]);
+      }
+    }
+  } else if constexpr (S::FP8) {
     // Three things at a time: rows i + 2 are read, rows i multiplied, and the
     // products of rows i - 1 scaled and added, 4 additions behind each
     // matrix instruction, which takes 8 times the time of one. The order is
@@ -260,8 +300,9 @@ __device__ __forceinline__ void compute(const char* lds, float sb, int wm,
 }
 
 // Steps [first, first + count) of the product. sb: the scales of the wave's
-// columns, one a step. B_SENT: send_b has been called.
-template <class S, bool B_SENT>
+// columns, one a step. B_SENT: send_b has been called. EXACT: e4m3 by the f16
+// instruction.
+template <class S, bool B_SENT, bool EXACT>
 __device__ __forceinline__ void product(char* smem, __amdgpu_buffer_rsrc_t ra,
                                         __amdgpu_buffer_rsrc_t rb,
                                         __amdgpu_buffer_rsrc_t rs,
@@ -311,7 +352,7 @@ __device__ __forceinline__ void product(char* smem, __amdgpu_buffer_rsrc_t ra,
       stage_a<S>(to, ra, rs, at, first + j + AHEAD, s_stride, wave);
       stage_b<S>(to, rb, at, first + j + AHEAD, wave);
     }
-    compute<S>(smem + now * S::STAGE, fb, wm, wn, lane, acc);
+    compute<S, EXACT>(smem + now * S::STAGE, fb, wm, wn, lane, acc);
     // the stage is free for the load behind the next barrier
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     if (S::FP8) fb = sbc[first + min(j + 1, count - 1)];
@@ -351,15 +392,19 @@ __device__ __forceinline__ FewStep<FP8, RT> few_step(
   return r;
 }
 
-template <bool FP8, int RT>
+template <bool FP8, bool EXACT, int RT>
 __device__ __forceinline__ void few_multiply(const FewStep<FP8, RT>& s,
                                              f32x4 (&acc)[RT]) {
 #pragma unroll
   for (int i = 0; i < RT; ++i) {
     if constexpr (FP8) {
-      const f32x4 p = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-          both(s.b), both(s.a[i]), f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0,
-          0);
+      f32x4 p;
+      if constexpr (EXACT)
+        p = exact_product(s.b, s.a[i]);
+      else
+        p = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+            both(s.b), both(s.a[i]), f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0,
+            0);
 #pragma unroll
       for (int r = 0; r < 4; ++r)
         acc[i][r] = __builtin_fmaf(p[r], s.f[i], acc[i][r]);
@@ -373,7 +418,7 @@ __device__ __forceinline__ void few_multiply(const FewStep<FP8, RT>& s,
   }
 }
 
-template <bool FP8, int RT>
+template <bool FP8, bool EXACT, int RT>
 __device__ __forceinline__ void few_product(
     const uint8_t* const (&a)[RT], const uint8_t* b,
     const float* const (&sa)[RT], int64_t s_rows, const float* sb, int first,
@@ -394,14 +439,14 @@ __device__ __forceinline__ void few_product(
                                     min(s + U + u, last - 1));
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (s + u < last) few_multiply<FP8, RT>(now[u], acc);
+      if (s + u < last) few_multiply<FP8, EXACT>(now[u], acc);
 #pragma unroll
     for (int u = 0; u < U; ++u) now[u] = next[u];
   }
 }
 
 // one row tile
-template <bool FP8>
+template <bool FP8, bool EXACT>
 __device__ __forceinline__ f32x4 few_product(const uint8_t* a,
                                              const uint8_t* b, const float* sa,
                                              int64_t s_rows, const float* sb,
@@ -409,7 +454,7 @@ __device__ __forceinline__ f32x4 few_product(const uint8_t* a,
   const uint8_t* const as[1] = {a};
   const float* const sas[1] = {sa};
   f32x4 acc[1];
-  few_product<FP8, 1>(as, b, sas, s_rows, sb, first, last, acc);
+  few_product<FP8, EXACT>(as, b, sas, s_rows, sb, first, last, acc);
   return acc[0];
 }
 
