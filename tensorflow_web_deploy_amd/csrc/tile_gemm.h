@@ -181,17 +181,23 @@ __device__ __forceinline__ f16x8 wider(int lo, int hi) {
   return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-__device__ __forceinline__ f32x4 exact_product(const i32x4 (&b)[2],
-                                               const i32x4 (&a)[2]) {
-  f32x4 p = {0.f, 0.f, 0.f, 0.f};
+// of NT tiles of B with one of A: a chain of 4 instructions each, in turn
+template <int NT>
+__device__ __forceinline__ void exact_products(const i32x4 (&b)[NT][2],
+                                               const i32x4 (&a)[2],
+                                               f32x4 (&p)[NT]) {
+#pragma unroll
+  for (int t = 0; t < NT; ++t) p[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int h = 0; h < 2; ++h)
 #pragma unroll
-    for (int i = 0; i < 4; i += 2)
-      p = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-          wider(b[h][i], b[h][i + 1]), wider(a[h][i], a[h][i + 1]), p, 0, 0,
-          0);
-  return p;
+    for (int i = 0; i < 4; i += 2) {
+      const f16x8 wide = wider(a[h][i], a[h][i + 1]);
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+        p[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+            wider(b[t][h][i], b[t][h][i + 1]), wide, p[t], 0, 0, 0);
+    }
 }
 
 template <class S>
@@ -238,13 +244,13 @@ __device__ __forceinline__ void compute(const char* lds, float sb, int wm,
     for (int i = 0; i < S::MT; ++i) {
       const FragA<S> a = read_a<S>(lds, wm, i, lane);
       const float f = a.f * sb;
+      f32x4 p[S::NT];
+      exact_products(b, a.v, p);
 #pragma unroll
-      for (int t = 0; t < S::NT; ++t) {
-        const f32x4 p = exact_product(b[t], a.v);
+      for (int t = 0; t < S::NT; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          acc[i][t][r] = __builtin_fmaf(p[r], f, acc[i][t][r]);
-      }
+          acc[i][t][r] = __builtin_fmaf(p[t][r], f, acc[i][t][r]);
     }
   } else if constexpr (S::FP8) {
     // Three things at a time: rows i + 2 are read, rows i multiplied, and the
@@ -370,7 +376,7 @@ __device__ __forceinline__ void product(char* smem, __amdgpu_buffer_rsrc_t ra,
 // lane / 16 * 4 + 0..3.
 template <bool FP8, int RT>
 struct FewStep {
-  i32x4 a[RT][2], b[2];
+  i32x4 a[RT][2], b[1][2];
   float f[RT];
 };
 
@@ -382,7 +388,7 @@ __device__ __forceinline__ FewStep<FP8, RT> few_step(
   const int64_t k = (int64_t)step * STEP;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    r.b[h] = *(const i32x4*)(b + k + h * 64);
+    r.b[0][h] = *(const i32x4*)(b + k + h * 64);
 #pragma unroll
     for (int i = 0; i < RT; ++i) r.a[i][h] = *(const i32x4*)(a[i] + k + h * 64);
   }
@@ -398,12 +404,13 @@ __device__ __forceinline__ void few_multiply(const FewStep<FP8, RT>& s,
 #pragma unroll
   for (int i = 0; i < RT; ++i) {
     if constexpr (FP8) {
-      f32x4 p;
+      f32x4 q[1];
+      f32x4& p = q[0];
       if constexpr (EXACT)
-        p = exact_product(s.b, s.a[i]);
+        exact_products(s.b, s.a[i], q);
       else
         p = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-            both(s.b), both(s.a[i]), f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0,
+            both(s.b[0]), both(s.a[i]), f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0,
             0);
 #pragma unroll
       for (int r = 0; r < 4; ++r)
@@ -412,7 +419,7 @@ __device__ __forceinline__ void few_multiply(const FewStep<FP8, RT>& s,
 #pragma unroll
       for (int h = 0; h < 2; ++h)
         acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-            __builtin_bit_cast(bf16x8, s.b[h]),
+            __builtin_bit_cast(bf16x8, s.b[0][h]),
             __builtin_bit_cast(bf16x8, s.a[i][h]), acc[i], 0, 0, 0);
     }
   }
