@@ -174,9 +174,10 @@ __device__ __forceinline__ DenseTile dense_tile(
   at.s = (uint32_t)(m0 + min(scale_row<S>(wave, lane), rows - 1)) * 4;
   const int wave_m = wave / S::WN * S::MT * 16;
   const int wave_n = wave % S::WN * S::NT * 16;
-  product<S, false, false>(smem, ra, rb, rs, at, first, count, (uint32_t)d.M * 4,
-             d.SB + (int64_t)min((n0 + wave_n) / 128, (d.N - 1) / 128) * all,
-             wave, lane, acc);
+  const float* sb =
+      d.SB + (int64_t)min((n0 + wave_n) / 128, (d.N - 1) / 128) * all;
+  product<S, false, false>(smem, ra, rb, rs, at, first, count,
+                           (uint32_t)d.M * 4, sb, wave, lane, acc);
   return {m0, n0, wave_m, wave_n};
 }
 

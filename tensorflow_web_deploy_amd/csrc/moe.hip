@@ -1172,10 +1172,10 @@ bool goes_directly(int64_t N, int64_t E) {
 
 // Rows of a tile: 32, 64 or 128, whatever costs least. Both products take as
 // many rounds over the chip as their tiles need, two of them a CU (of 64 rows
-// in e4m3 three, which then take 1.27 times as long), a little less than a whole
-// one if each lies alone; a round takes its steps and what lies before and
-// behind them. Measured, in us, for 32 / 64 / 128 rows and N rows in all: 16
-// experts of 768 x 1536 in bf16, N = 256: 29.4 / 33.3 / 41.9, N = 2048:
+// in e4m3 three, which then take 1.27 times as long), a little less than a
+// whole one if each lies alone; a round takes its steps and what lies before
+// and behind them. Measured, in us, for 32 / 64 / 128 rows and N rows in all:
+// 16 experts of 768 x 1536 in bf16, N = 256: 29.4 / 33.3 / 41.9, N = 2048:
 // 44.7 / 39.1 / 49.6, N = 6000: 88 / 72 / 67; 128 of 1024 x 704 in e4m3,
 // N = 128: 36.7 / 35.5 / 43.3, N = 8192: 79 / 70 / 82, N = 48000:
 // 302 / 211 / 207. Over 124 such cases the costs below chose a tile that is
