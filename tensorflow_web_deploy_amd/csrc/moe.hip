@@ -941,7 +941,7 @@ __global__ __launch_bounds__(S::THREADS, 2) void experts_kernel(Experts p) {
   // side by the sums' error, and each counts as a step of 2^-4: where rows are
   // so few that the weights' way from memory bounds, the sums keep all of f32:
   // 33 rows for 64 experts are off by 0.0017 in all, as bf16's rounding alone,
-  // and not by up to 0.0037, for 1 us of 27.
+  // and not by up to 0.0037, for 1 to 2 us of 27.
   constexpr bool EXACT = FIRST && S::FP8 && S::BM == 32;
   const float* sb = S::FP8 ? p.SB + ((int64_t)e * blocks_n +
                                      min(wave_n0 / 128, blocks_n - 1)) * p.steps
