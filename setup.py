@@ -4,7 +4,9 @@ Build:  PYTORCH_ROCM_ARCH=gfx950 python setup.py build_ext --inplace
 The built .so lands inside tensorflow_web_deploy_amd/ so it travels to
 GPU boxes with the repo snapshot.
 """
+import glob
 import os
+import zlib
 
 os.environ.setdefault("PYTORCH_ROCM_ARCH", "gfx950")
 
@@ -13,6 +15,11 @@ from torch.utils import cpp_extension  # noqa: E402
 
 ROOT = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(ROOT, "tensorflow_web_deploy_amd", "csrc")
+
+# The build knows the sources alone: with this on their command lines a changed
+# header compiles them again.
+HEADERS = "-DCSRC_HEADERS=%d" % zlib.crc32(b"".join(
+    open(h, "rb").read() for h in sorted(glob.glob(os.path.join(CSRC, "*.h")))))
 
 ext = cpp_extension.CUDAExtension(
     name="tensorflow_web_deploy_amd._hipops",
@@ -32,10 +39,10 @@ ext = cpp_extension.CUDAExtension(
         os.path.join(CSRC, "moe.hip"),
     ],
     extra_compile_args={
-        "cxx": ["-O3", "-std=c++17"],
+        "cxx": ["-O3", "-std=c++17", HEADERS],
         # packed f32 instructions off: some of their forms have given wrong
         # results on this hardware, and -O3 makes them from ordinary code
-        "nvcc": ["-O3", "-std=c++17", "--offload-arch=gfx950",
+        "nvcc": ["-O3", "-std=c++17", HEADERS, "--offload-arch=gfx950",
                  "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"],
     },
 )
