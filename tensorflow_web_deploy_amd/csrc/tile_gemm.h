@@ -435,16 +435,18 @@ __device__ __forceinline__ void few_product(
 #pragma unroll
   for (int i = 0; i < RT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   if (first >= last) return;
+  // No step is loaded that isn't there: one set of registers more, filled with
+  // the last step once more, cost 1.6 us of 5.
   FewStep<FP8, RT> now[U], next[U];
 #pragma unroll
   for (int u = 0; u < U; ++u)
-    now[u] = few_step<FP8, RT>(a, b, sa, s_rows, sb, min(first + u, last - 1));
+    if (u == 0 || first + u < last)
+      now[u] = few_step<FP8, RT>(a, b, sa, s_rows, sb, first + u);
   for (int s = first; s < last; s += U) {
-    if (s + U < last)
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        next[u] = few_step<FP8, RT>(a, b, sa, s_rows, sb,
-                                    min(s + U + u, last - 1));
+    for (int u = 0; u < U; ++u)
+      if (s + U + u < last)
+        next[u] = few_step<FP8, RT>(a, b, sa, s_rows, sb, s + U + u);
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (s + u < last) few_multiply<FP8, EXACT>(now[u], acc);
