@@ -253,10 +253,10 @@ __device__ __forceinline__ void finish4(const Dense& d, int64_t m, int n,
 
 // Up to 16 RT rows: 16 columns a workgroup, K cut into 8 parts, a wave each;
 // wave i finishes row tile i. Bound by the time the weights take to come:
-// 1 x 768 x 1000 3.3 us, 1 x 25088 x 4096 18.4 (5.6 TB/s).
+// 1 x 768 x 1000 3.1 us, 1 x 25088 x 4096 17.8 (5.8 TB/s). With 4 waves that
+// takes 25.4 us, with 16 18.8.
 template <int RT>
-__global__ __launch_bounds__(512, RT == 1 ? 4 : 2) void gemm_fp8_few_kernel(
-    Dense d) {
+__global__ __launch_bounds__(512, 4) void gemm_fp8_few_kernel(Dense d) {
   __shared__ __attribute__((aligned(16))) float part[RT * 8 * 256];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -365,6 +365,12 @@ void run(Dense d, hipStream_t stream) {
   }
 }
 
+template <int RT>
+void run_few(const Dense& d, hipStream_t stream) {
+  hipLaunchKernelGGL((gemm_fp8_few_kernel<RT>), dim3(up(d.N, 16)), dim3(512),
+                     0, stream, d);
+}
+
 enum class Way { FEW, TILE64, TILE128, TILE160, TILE256 };
 
 struct Plan {
@@ -385,10 +391,10 @@ struct Plan {
 Plan plan(int M, int N, int Kp) {
   const int all = Kp / STEP;
   // Few rows, in us as such and as the best tiles: 1 x 4096 x 4096 5.3 / 9.5,
-  // 16 x 4096 x 4096 6.8 / 10.5, 16 x 25088 x 4096 25.5 / 25.4. Every 16
+  // 16 x 4096 x 4096 6.6 / 10.5, 16 x 25088 x 4096 24.9 / 25.4. Every 16
   // columns read all rows again, so more than 16 rows are few only where
-  // neither side is long: 32 x 768 x 1000 4.9 / 6.9, 32 x 4096 x 4096
-  // 8.8 / 11.6, but 32 x 8192 x 2048 14.4 / 13.4, 32 x 1024 x 6000 8.8 / 8.0.
+  // neither side is long: 32 x 768 x 1000 3.8 / 6.9, 32 x 4096 x 4096
+  // 8.6 / 11.6, but 32 x 8192 x 2048 14.4 / 13.4, 32 x 1024 x 6000 8.8 / 8.0.
   if (M <= 16 || (M <= 32 && N <= 4096 && Kp <= 4096))
     return {Way::FEW, 1, all};
   Plan best{Way::TILE128, 1, all};
@@ -470,11 +476,9 @@ void launch_gemm_fp8(const void* A, const float* SA, const void* B,
   switch (p.way) {
     case Way::FEW:
       if (M <= 16)
-        hipLaunchKernelGGL((gemm_fp8_few_kernel<1>), dim3(up(N, 16)),
-                           dim3(512), 0, stream, d);
+        run_few<1>(d, stream);
       else
-        hipLaunchKernelGGL((gemm_fp8_few_kernel<2>), dim3(up(N, 16)),
-                           dim3(512), 0, stream, d);
+        run_few<2>(d, stream);
       break;
     case Way::TILE64:
       if (p.slices > 1)

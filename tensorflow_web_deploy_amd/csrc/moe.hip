@@ -961,8 +961,11 @@ __global__ __launch_bounds__(S::THREADS, 2) void experts_kernel(Experts p) {
 // Without a plan, the first product: CW * 16 columns of an assignment a
 // workgroup, K cut into KS parts, a wave each. The 16 rows are all the same.
 // Bound by the time its weights take to come: 2 assignments, 768 x 1536 in
-// bf16, 5.5 us. K in 8 parts took up to 20% longer, 4 steps on their way for 2
-// up to 45%.
+// bf16, 4.2 us. One tile of 16 columns with K in 8 parts, or two with 4, for a
+// layer of 1 row: 9.9 / 10.5 us, 2 of 8 experts of 2048 x 2048 13.3 / 15.1;
+// where half as wide workgroups are more than CUs, 2 rows of 4 experts, 1024 x
+// 704, 11.3 / 11.1. 16 waves (e4m3, K in 2 parts: 13.6 -> 14.6) and 4 were
+// slower.
 template <bool FP8, int CW, int KS>
 __global__ __launch_bounds__(512, 4) void experts_hidden_kernel(Experts p) {
   static_assert(CW * KS == 8 && (!FP8 || CW == 8));
@@ -1027,7 +1030,7 @@ __global__ __launch_bounds__(512, 4) void experts_hidden_kernel(Experts p) {
 // Without a plan, the second product and the sum over a token's experts: 16
 // columns of a token a workgroup, its waves share the experts and, if there
 // are fewer than 8, K. The 16 rows are all the same one. Bound as above: 1 row
-// of 2 experts, 1536 x 768 in bf16, 6.3 us, 7.2 with K in one piece.
+// of 2 experts, 1536 x 768 in bf16, 5.4 us, 0.7 more with K in one piece.
 template <bool FP8>
 __global__ __launch_bounds__(512, 4) void experts_sum_kernel(
     Experts p, const __bf16* residual, int64_t ldr, __bf16* Y, int64_t ldy) {
@@ -1285,10 +1288,20 @@ void run_mlp(const MoeMlp& m, const Layout& l, char* ws, hipStream_t stream) {
   p.H = ws + l.h;
   p.SH = (float*)(ws + l.sh);
   if (l.direct) {
-    constexpr int CW = FP8 ? 8 : 2;
-    p.tiles_n = up(p.np, CW * 16);
-    hipLaunchKernelGGL((experts_hidden_kernel<FP8, CW, 8 / CW>),
-                       dim3(N * p.tiles_n), dim3(512), 0, stream, p);
+    auto hidden = [&](auto cw, auto ks) {
+      constexpr int CW = decltype(cw)::value, KS = decltype(ks)::value;
+      p.tiles_n = up(p.np, CW * 16);
+      hipLaunchKernelGGL((experts_hidden_kernel<FP8, CW, KS>),
+                         dim3(N * p.tiles_n), dim3(CW * KS * 64), 0, stream,
+                         p);
+    };
+    using std::integral_constant;
+    if constexpr (FP8)  // the waves share the scale of a block of columns
+      hidden(integral_constant<int, 8>(), integral_constant<int, 1>());
+    else if (N * up(p.np, 32) <= 128)  // twice as many fit, one to a CU
+      hidden(integral_constant<int, 1>(), integral_constant<int, 8>());
+    else
+      hidden(integral_constant<int, 2>(), integral_constant<int, 4>());
   } else if (l.BM == 32) {
     run_first<Tile32<FP8, true>>(p, stream);
   } else if (l.BM == 64) {

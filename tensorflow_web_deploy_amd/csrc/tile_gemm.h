@@ -370,7 +370,10 @@ __device__ __forceinline__ void product(char* smem, __amdgpu_buffer_rsrc_t ra,
 
 // The product of up to 16 RT rows with 16 columns by one wave, for calls that
 // read their weights for a few rows: bound by the time that the weights take
-// to come, so they go from memory to registers at once, U steps ahead.
+// to come, so they go from memory to registers at once, a step ahead: more of
+// them was slower at every size (1 x 2048 x 16384, 1 / 2 / 3 / 4: 7.7 / 8.4 /
+// 10.0 / 10.3 us), as fewer waves find room, and a step too many, loaded in
+// vain, cost 0.3 us of 3.5.
 // a[i], b, sa[i]: this lane's row of A, in each row tile, and of B (16 bytes
 // from their start a quarter of the wave) and its row's scale at step 0. As in
 // a tile, a lane ends up with row lane % 16 of each row tile and the columns
@@ -431,27 +434,15 @@ __device__ __forceinline__ void few_product(
     const uint8_t* const (&a)[RT], const uint8_t* b,
     const float* const (&sa)[RT], int64_t s_rows, const float* sb, int first,
     int last, f32x4 (&acc)[RT]) {
-  constexpr int U = 2;
 #pragma unroll
   for (int i = 0; i < RT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   if (first >= last) return;
-  // No step is loaded that isn't there: one set of registers more, filled with
-  // the last step once more, cost 1.6 us of 5.
-  FewStep<FP8, RT> now[U], next[U];
-#pragma unroll
-  for (int u = 0; u < U; ++u)
-    if (u == 0 || first + u < last)
-      now[u] = few_step<FP8, RT>(a, b, sa, s_rows, sb, first + u);
-  for (int s = first; s < last; s += U) {
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (s + U + u < last)
-        next[u] = few_step<FP8, RT>(a, b, sa, s_rows, sb, s + U + u);
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (s + u < last) few_multiply<FP8, EXACT>(now[u], acc);
-#pragma unroll
-    for (int u = 0; u < U; ++u) now[u] = next[u];
+  auto now = few_step<FP8, RT>(a, b, sa, s_rows, sb, first);
+  for (int s = first; s < last; ++s) {
+    FewStep<FP8, RT> next;
+    if (s + 1 < last) next = few_step<FP8, RT>(a, b, sa, s_rows, sb, s + 1);
+    few_multiply<FP8, EXACT>(now, acc);
+    now = next;
   }
 }
 
