@@ -397,14 +397,17 @@ void quant_fp8(torch::Tensor X, torch::Tensor Q, torch::Tensor S,
                    S.data_ptr<float>(), (int)block_rows, cur_stream());
 }
 
-// C[M][N] = act(A @ B^T + bias + residual), C bf16. A [M,Kp] with SA
-// [Kp/128, M], B [N,Kp] with SB [ceil(N/128), Kp/128]: as quant_fp8
-// leaves them with block_rows 1 and 128
+// C[M][N] = act(A @ B^T + bias + residual), C bf16 or f32, residual bf16. A
+// [M,Kp] with SA [Kp/128, M], B [N,Kp] with SB [ceil(N/128), Kp/128]: as
+// quant_fp8 leaves them with block_rows 1 and 128
 void gemm_fp8(torch::Tensor A, torch::Tensor SA, torch::Tensor B,
               torch::Tensor SB, torch::Tensor C,
               c10::optional<torch::Tensor> bias,
               c10::optional<torch::Tensor> residual, int64_t act) {
-  check_type(C, torch::kBFloat16, "C");
+  const bool f32 = C.scalar_type() == torch::kFloat32;
+  TORCH_CHECK(C.scalar_type() == torch::kBFloat16 || (f32 && C.is_cuda()),
+              "C must be BFloat16 or, on a GPU, Float, got ", C.scalar_type(),
+              " on ", C.device());
   check_rows(C, "C");
   check_type(A, kFp8, "A");
   TORCH_CHECK(A.dim() == 2, "A must be 2D");
@@ -438,11 +441,11 @@ void gemm_fp8(torch::Tensor A, torch::Tensor SA, torch::Tensor B,
   check_devices(all);
   if (M == 0) return;
   const c10::DeviceGuard guard(A.device());
-  const int64_t floats = gemm_fp8_workspace((int)M, (int)N, (int)Kp);
+  const int64_t floats = gemm_fp8_workspace((int)M, (int)N, (int)Kp, f32);
   torch::Tensor ws;
   if (floats) ws = torch::empty({floats}, SA.options());
   launch_gemm_fp8(A.data_ptr(), SA.data_ptr<float>(), B.data_ptr(),
-                  SB.data_ptr<float>(), C.data_ptr(), row_stride(C),
+                  SB.data_ptr<float>(), C.data_ptr(), f32, row_stride(C),
                   bias ? bias->data_ptr<float>() : nullptr,
                   residual ? residual->data_ptr() : nullptr,
                   residual ? row_stride(*residual) : 0, (int)M, (int)N,

@@ -112,11 +112,11 @@ void launch_quant_fp8(const void* X, bool f32, int64_t ldx, int64_t M, int K,
                       void* Q, int Kp, float* S, int block_rows,
                       hipStream_t stream);
 // floats that launch_gemm_fp8 needs at `part`
-int64_t gemm_fp8_workspace(int M, int N, int Kp);
-// C = act(A @ B^T + bias + residual), C bf16 with row stride ldc; act: 0 none,
-// 1 relu, 2 relu6, 5 gelu
+int64_t gemm_fp8_workspace(int M, int N, int Kp, bool f32);
+// C = act(A @ B^T + bias + residual), C bf16 or f32 with row stride ldc; act:
+// 0 none, 1 relu, 2 relu6, 5 gelu
 void launch_gemm_fp8(const void* A, const float* SA, const void* B,
-                     const float* SB, void* C, int64_t ldc,
+                     const float* SB, void* C, bool f32, int64_t ldc,
                      const float* bias, const void* residual, int64_t ldr,
                      int M, int N, int Kp, int act, float* part,
                      hipStream_t stream);

@@ -515,8 +515,9 @@ __device__ __forceinline__ void store_run(float* p, int have,
 
 // v Phi(v), the erf-GELU. The normal distribution's tail beyond |v| is
 // Abramowitz and Stegun's 7.1.26, 1/2 t (a1 + .. + a5 t^4) exp(-v^2 / 2) with
-// t = 1 / (1 + p |v| / sqrt 2): off by less than 1e-7, in 13 operations. With
-// erff the activation alone took a quarter of a large product's time.
+// t = 1 / (1 + p |v| / sqrt 2): off by less than 1e-7, as 1 + erf in f32 is, in
+// 13 operations. With erff the activation alone took a quarter of a large
+// product's time; with erfcf 12544 x 768 x 768 into f32 took 45 us, not 38.
 __device__ __forceinline__ float gelu(float v) {
   const float t = __builtin_amdgcn_rcpf(
       __builtin_fmaf(0.3275911f * 0.70710678f, fabsf(v), 1.f));

@@ -436,3 +436,108 @@ def test_gemm_operands_past_4_gb(E):
     c = torch.empty(n, 16, dtype=torch.bfloat16, device="cuda")
     E.gemm_fp8(long, sa, qb, sb, c)
     check_gemm(c[some], part, sa[:, some], qb, sb)
+
+
+# ------------------------------------------------------------ f32 results
+
+
+def check_gemm_f32(got, qa, sa, qb, sb, bias=None, res=None, act=0):
+    """Products of e4m3 values are exact in f32. A block's 128 of them, the
+    blocks (two roundings each: of the scales' product and of the addition),
+    slices of K (32 at most), bias and residual are added in f32, no addition
+    off by more than 2^-23 of the terms' size. The activation's slope is 1.13
+    at most; GELU's tail is off by 1e-7 times the value, under 2^-21 of it,
+    and its operations by less than 2^-20 of the largest that it reaches on
+    the negative side, 0.17."""
+    a, b = values64(qa, sa, 1), values64(qb, sb, 128)
+    y, size = a @ b.t(), a.abs() @ b.abs().t()
+    for add in (bias, res):
+        if add is not None:
+            add = add.cpu().double()
+            y, size = y + add, size + add.abs()
+    ref = act_ref(y, act)
+    n = 128 + 2 * qa.shape[1] / 128 + 32 + 4
+    tol = 1.13 * n * 2.0 ** -23 * size + 2.0 ** -21 * y.abs() + 1e-38
+    if act == 5:
+        tol = tol + 2.0 ** -20 * 0.17
+    off = (got.cpu().double() - ref).abs()
+    assert (off <= tol).all(), (off / tol).max()
+
+
+def test_gemm_refuses_f32_elsewhere(E):
+    for c in (torch.zeros(4, 5), torch.zeros(4, 5, device="meta")):
+        with pytest.raises(RuntimeError, match="C must be"):
+            E.gemm_fp8(**_gemm_args(C=c))
+    with pytest.raises(RuntimeError, match="C must be"):
+        E.gemm_fp8(**_gemm_args(C=torch.zeros(4, 5, dtype=torch.float16)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", GEMMS)
+def test_gemm_f32(E, m, n, k):
+    ops = operands(E, m, n, k, seed=m + n + k)
+    c = torch.full((m, n), math.nan, device="cuda")
+    E.gemm_fp8(*ops, c)
+    check_gemm_f32(c, *ops)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", [0, 1, 2, 5])
+@pytest.mark.parametrize("m,n,k", [(3, 40, 256), (64, 96, 4096),
+                                   (200, 250, 384), (700, 520, 256)])
+def test_gemm_f32_epilogue(E, m, n, k, act):
+    ops = operands(E, m, n, k, seed=act)
+    g = torch.Generator().manual_seed(1)
+    bias = torch.randn(n, generator=g).cuda()
+    res = torch.randn(m, n, generator=g).to(torch.bfloat16).cuda()
+    for b, r in ((bias, None), (None, res), (bias, res)):
+        c = torch.full((m, n), math.nan, device="cuda")
+        E.gemm_fp8(*ops, c, b, r, act)
+        check_gemm_f32(c, *ops, b, r, act)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(6200, 768, 256), (500, 2000, 1024),
+                                   (3000, 2055, 1100)])
+def test_gemm_f32_many_tiles(E, m, n, k):
+    qa, sa, qb, sb = operands(E, m, n, k, seed=m)
+    bias = torch.randn(n, device="cuda")
+    res = torch.randn(m, n, device="cuda").to(torch.bfloat16)
+    c = torch.full((m, n), math.nan, device="cuda")
+    E.gemm_fp8(qa, sa, qb, sb, c, bias, res, 5)
+    assert not c.isnan().any()
+    rows = sorted({0, 1, 63, 64, 127, 128, 255, 256, m - 130, m - 2, m - 1,
+                   *range(5, m, m // 10)})
+    check_gemm_f32(c[rows], qa.view(torch.uint8)[rows].view(E4M3),
+                   sa[:, rows], qb, sb, bias, res[rows], 5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("offset", [0, 1, 8])
+@pytest.mark.parametrize("m,n,k", [(12, 72, 256), (40, 72, 256),
+                                   (40, 71, 8192)])
+def test_gemm_f32_into_a_slice(E, m, n, k, offset):
+    ops = operands(E, m, n, k)
+    wide = torch.full((m + 2, n + 20), 3.0, device="cuda")
+    c = wide[1:m + 1, offset:offset + n]
+    E.gemm_fp8(*ops, c)
+    check_gemm_f32(c, *ops)
+    c.fill_(3.0)
+    assert (wide == 3.0).all()
+
+
+@pytest.mark.gpu
+def test_gemm_f32_in_a_graph(E):
+    ops = operands(E, 40, 200, 8192)
+    c = torch.empty(40, 200, device="cuda")
+    want = torch.empty_like(c)
+    E.gemm_fp8(*ops, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        E.gemm_fp8(*ops, c)
+    for _ in range(3):
+        c.fill_(math.nan)
+        graph.replay()
+        assert torch.equal(c, want)
+        E.gemm_fp8(*ops, want)
+        torch.cuda.synchronize()
