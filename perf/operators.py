@@ -33,13 +33,13 @@ def listed():
         # the patch embeddings of a captured batch of 64 images (196 tokens each) before a projection
         {"name": "quant_batch", "op": "quant", "m": 12544, "k": 768, "x": "bf16"},
         # the classifier of one image: 1000 classes
-        {"name": "gemm_single", "op": "gemm", "m": 1, "k": 768, "n": 1000, "act": "none", "residual": False},
+        {"name": "gemm_single", "op": "gemm", "m": 1, "k": 768, "n": 1000, "out": "bf16", "act": "none", "residual": False},
         # the first dense layer behind a 7x7x512 feature map, 64 images: a hundred megabytes of weights for 64 rows
-        {"name": "gemm_weights", "op": "gemm", "m": 64, "k": 25088, "n": 4096, "act": "relu", "residual": False},
+        {"name": "gemm_weights", "op": "gemm", "m": 64, "k": 25088, "n": 4096, "out": "bf16", "act": "relu", "residual": False},
         # attention's output projection at 64 images, added to the residual stream
-        {"name": "gemm_project", "op": "gemm", "m": 12544, "k": 768, "n": 768, "act": "none", "residual": True},
+        {"name": "gemm_project", "op": "gemm", "m": 12544, "k": 768, "n": 768, "out": "bf16", "act": "none", "residual": True},
         # the large end: a wide hidden layer over many rows, its height no multiple of a tile
-        {"name": "gemm_large", "op": "gemm", "m": 16200, "k": 4096, "n": 8192, "act": "gelu", "residual": False},
+        {"name": "gemm_large", "op": "gemm", "m": 16200, "k": 4096, "n": 8192, "out": "bf16", "act": "gelu", "residual": False},
         # one image's token count against 64 experts, plain softmax routing
         {"name": "route_small", "op": "route", "t": 196, "e": 64, "k": 2, "x": "bf16", "score": "softmax", "bias": False, "groups": 1, "kept": 1,
          "best": 1, "renorm": True, "scale": 1.0, "padding": 0},
@@ -68,7 +68,7 @@ def draw(rng):
         return {"op": op, "m": _log(rng, 1, 16384), "k": _log(rng, 1, 8192), "x": rng.choice(["bf16", "f32"])}
     if op == "gemm":
         while True:
-            c = {"op": op, "m": _log(rng, 1, 16384), "k": _log(rng, 64, 25088), "n": _log(rng, 10, 8192),
+            c = {"op": op, "m": _log(rng, 1, 16384), "k": _log(rng, 64, 25088), "n": _log(rng, 10, 8192), "out": rng.choice(["bf16", "f32"]),
                  "act": rng.choice(sorted(ACTS)), "residual": rng.random() < 0.4}
             if c["m"] * c["k"] * c["n"] <= 16200 * 4096 * 8192 and (c["m"] + c["n"]) * c["k"] <= 1.2e8:
                 return c
@@ -99,8 +99,9 @@ def work(c):
         return {"bytes": n * TYPES[c["x"]].itemsize + c["m"] * _up(c["k"], BLOCK) * (1 + 4 / BLOCK), "flops": 2 * n}
     if c["op"] == "gemm":
         m, n, k = c["m"], c["n"], c["k"]
+        out = TYPES[c["out"]].itemsize
         scales = 4 * _up(k, BLOCK) // BLOCK * (m + _up(n, BLOCK) // BLOCK)
-        return {"bytes": (m + n) * k + scales + 4 * n + m * n * (4 if c["residual"] else 2), "flops": 2 * m * n * k}
+        return {"bytes": (m + n) * k + scales + 4 * n + m * n * (out + (2 if c["residual"] else 0)), "flops": 2 * m * n * k}
     if c["op"] == "route":
         n = c["t"] * c["e"]
         return {"bytes": n * TYPES[c["x"]].itemsize + c["t"] * c["k"] * 8 + (4 * c["e"] if c["bias"] else 0), "flops": 8 * n}
@@ -227,7 +228,7 @@ def _plain_gemm(s):
     y = _values(s["a"], s["sa"]) @ _weight_values(s["b"], s["sb"]).t() + s["bias"]
     if s["res"] is not None:
         y = y + s["res"].float()
-    return _act(y, c["act"]).to(torch.bfloat16)
+    return _act(y, c["act"]).to(TYPES[c["out"]])
 
 
 def _plain_route(s):
@@ -323,7 +324,7 @@ def _own_quant(s):
 
 def _own_gemm(s):
     c = s["c"]
-    y = torch.empty(c["m"], c["n"], dtype=torch.bfloat16, device="cuda")
+    y = torch.empty(c["m"], c["n"], dtype=TYPES[c["out"]], device="cuda")
     _ext().gemm_fp8(s["a"], s["sa"], s["b"], s["sb"], y, s["bias"], s["res"], ACTS[c["act"]])
     return y
 
