@@ -486,8 +486,14 @@ __global__ __launch_bounds__(256) void route_kernel(Route p) {
   }
   __builtin_amdgcn_wave_barrier();
 
+  // equal logits and biases tie in any precision
+  auto ties = [&](int a, int b) {
+    const T* x = (const T*)p.x + t * p.ldx;
+    return (float)x[a] == (float)x[b] && (!p.bias || p.bias[a] == p.bias[b]);
+  };
   float w[4], sum = 0.f;
   int id[4];
+  bool close = false;
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     const int j = q * 16 + l;
@@ -501,12 +507,33 @@ __global__ __launch_bounds__(256) void route_kernel(Route p) {
     if (b.x < 0) continue;
     const float ka = __builtin_bit_cast(float, a.y);
     const float kb = __builtin_bit_cast(float, b.y);
-    if (!(ka - kb > error_of(w[q], ka, p.sigmoid) +
-                        error_of(lds[at.p + b.x], kb, p.sigmoid))) {
-      // equal logits and biases tie in any precision
-      const T* x = (const T*)p.x + t * p.ldx;
-      if (!((float)x[a.x] == (float)x[b.x] &&
-            (!p.bias || p.bias[a.x] == p.bias[b.x])))
+    // Chosen keys that lie apart, each from the next, all lie above what the
+    // last one may be at the least, and b, the largest that isn't chosen, below
+    // it. So do the others where b would with the largest error that any of
+    // them can have: that of the largest score, or, without a bias, b's own.
+    const bool last = j + 1 == p.k;
+    const float pb = last && p.bias ? most : lds[at.p + b.x];
+    if (!(ka - kb >
+          error_of(w[q], ka, p.sigmoid) + error_of(pb, kb, p.sigmoid))) {
+      close = last;
+      if (!ties(a.x, b.x)) safe = false;
+    }
+  }
+  // Where b ties with the last one, each of the others has to lie below or tie.
+  const uint64_t closely = __ballot(close && safe);
+  if (closely >> (lane & 48) & 0xffff) {
+    const int2 a = list[p.k - 1], b = list[p.k];
+    const float ka = __builtin_bit_cast(float, a.y);
+    const float low = ka - error_of(lds[at.p + a.x], ka, p.sigmoid);
+    const float more =
+        error_of(p.bias ? most : lds[at.p + b.x], 0.f, p.sigmoid);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      // a list leaves the chosen keys in place, the other way takes them out
+      const int e = expert_at<V>(l, v);
+      const float y = key[v];
+      if (y > NONE && !(y + 0x1p-23f * fabsf(y) + more < low) &&
+          (y < ka || (y == ka && e > a.x)) && !ties(a.x, e))
         safe = false;
     }
   }

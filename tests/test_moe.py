@@ -686,3 +686,45 @@ def test_mlp_experts_past_4_gb(E, fp8, t):
     y = run(0)
     assert not y.isnan().any() and (y != 0).any(1).all()
     assert torch.equal(y, run(62))
+
+
+# ------------------------------------------------- the last choice of a row
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("score", [0, 1])
+@pytest.mark.parametrize("bias", [None, 0.0, 0.25])
+def test_route_rival_behind_a_tie_at_the_cut(E, score, bias):
+    """The last place and the first one without are equal in 64 bits; a third
+    expert is larger than both by less than 32 bits can tell."""
+    for row, k in (([0, 0, 1e-9, -5], 1), ([3, 0, 0, 1e-8], 2),
+                   ([0, 0, 0, 0, 0, 1e-9], 1), ([5, 4, 3, 0, 0, 0, 1e-9], 4)):
+        x = torch.tensor([row])
+        b = None if bias is None else torch.full((len(row),), bias).cuda()
+        check_route(E, x.cuda(), b, k, score)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("score", [0, 1])
+@pytest.mark.parametrize("e,k,groups,kept", [
+    (8, 1, 1, 1), (8, 3, 1, 1), (64, 2, 1, 1), (64, 8, 1, 1), (64, 13, 1, 1),
+    (64, 14, 1, 1), (256, 8, 1, 1), (256, 8, 8, 4), (512, 20, 1, 1),
+    (100, 33, 1, 1)])
+def test_route_many_ties_at_the_cut(E, score, e, k, groups, kept):
+    """Rows of few values: some large, most equal, here and there one that is
+    larger or smaller by less than 32 bits can tell."""
+    g = torch.Generator().manual_seed(e + k)
+    x = torch.zeros(60, e)
+    at = torch.rand(60, e, generator=g)
+    x[at < 1.5 / e] = 1e-9
+    x[at > 1 - 1.5 / e] = -1e-9
+    x[(at > 0.5) & (at < 0.5 + 0.8 * k / e)] = 1.0
+    x[(at > 0.2) & (at < 0.2 + 0.2 * k / e)] = 1.0 + 2.0 ** -23
+    check_route(E, x.cuda(), None, k, score, groups, kept, 2)
+    # one bias for all where groups' sums are compared: sums of the same terms
+    # in other pairs differ by their roundings in 64 bits
+    b = torch.where(torch.rand(e, generator=g) < 0.3, 0.125, 0.25)
+    b = (b if groups == 1 else torch.full((e,), 0.25)).cuda()
+    check_route(E, x.cuda(), b, k, score, groups, kept, 2)
+    x = x.to(torch.bfloat16)  # equal logits alone
+    check_route(E, x.cuda(), None, k, score, groups, kept, 2)
