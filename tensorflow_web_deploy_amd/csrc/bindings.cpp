@@ -455,6 +455,29 @@ void gemm_fp8(torch::Tensor A, torch::Tensor SA, torch::Tensor B,
 
 // ---- mixture-of-experts layers
 
+// logits [T,E] f32 = X [T,D] bf16 @ W^T. W [3,E,D up to 64s] bf16, filled up
+// with zeros: its three parts add up to the f32 weights, each the rounding of
+// what those before it leave
+void moe_logits(torch::Tensor X, torch::Tensor W, torch::Tensor logits) {
+  check_type(X, torch::kBFloat16, "X");
+  check_rows(X, "X");
+  const int64_t T = X.size(0), D = X.size(1);
+  TORCH_CHECK(T < kMaxRows, "too many rows: ", T);
+  TORCH_CHECK(D >= 1 && D <= 1 << 18, "width must be 1 to 2^18, got ", D);
+  TORCH_CHECK(W.dim() == 3, "W must be 3D");
+  const int64_t E = W.size(1);
+  TORCH_CHECK(E >= 1 && E <= 512, "1 to 512 experts, got ", E);
+  check_whole(W, torch::kBFloat16, {3, E, (D + 63) / 64 * 64}, "W");
+  check_aligned(W, "W");
+  check_whole(logits, torch::kFloat32, {T, E}, "logits");
+  check_devices({{&X, "X"}, {&W, "W"}, {&logits, "logits"}});
+  if (T == 0) return;
+  const c10::DeviceGuard guard(X.device());
+  launch_moe_logits(X.data_ptr(), row_stride(X), W.data_ptr(),
+                    logits.data_ptr<float>(), (int)T, (int)D, (int)E,
+                    cur_stream());
+}
+
 // logits [T,E] bf16|f32 -> ids i32 [T,k], weights f32 [T,k]. score: 0 softmax,
 // 1 sigmoid; bias f32 [E] is added for the choice alone. With groups > 1 the
 // experts are taken from the `kept` groups whose `best` (1 or 2) largest
@@ -660,6 +683,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("SB"), py::arg("C"), py::arg("bias") = py::none(),
         py::arg("residual") = py::none(), py::arg("act") = 0,
         "block-scaled fp8 MFMA GEMM: act(A @ B^T + bias + residual)");
+  m.def("moe_logits", &moe_logits, py::arg("X"), py::arg("W"),
+        py::arg("logits"), "router logits in f32");
   m.def("moe_route", &moe_route, py::arg("logits"), py::arg("bias"),
         py::arg("ids"), py::arg("weights"), py::arg("score") = 0,
         py::arg("groups") = 1, py::arg("kept") = 1, py::arg("best") = 1,

@@ -122,6 +122,10 @@ void launch_gemm_fp8(const void* A, const float* SA, const void* B,
                      hipStream_t stream);
 
 // moe.hip — mixture-of-experts layers
+// Y [T][E] f32 = X [T][D] (row stride ldx) W^T, X bf16; W [3][E][D up to 64s]
+// bf16: the three add up to the weights. E <= 512
+void launch_moe_logits(const void* X, int64_t ldx, const void* W, float* Y,
+                       int T, int D, int E, hipStream_t stream);
 // logits [T][E] (row stride ldx) bf16 or f32 -> the k experts of each row and
 // their weights; rows or experts that have none get id -1 and weight 0.
 // E <= 512, k <= 64, groups <= 64

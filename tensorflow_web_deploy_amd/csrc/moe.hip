@@ -1,4 +1,5 @@
 // Mixture-of-experts layers.
+//   moe_logits logits = x W^T, W in f32
 //   moe_route  scores = softmax(logits) | sigmoid(logits); the k experts with
 //              the largest score + bias, out of the groups that are kept;
 //              their scores, renormalised and scaled, are the weights
@@ -23,6 +24,99 @@ namespace {
 using namespace tile;
 
 int up(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+
+// ----------------------------------------------------------- moe_logits
+
+struct Logits {
+  const __bf16 *X, *W;  // W: [3][E][Dp], the parts of each weight
+  float* Y;
+  int64_t ldx;
+  int T, D, Dp, E;
+};
+
+// 8 values of a row from p on, the ones from `have` on as 0; rows may start
+// anywhere
+__device__ __forceinline__ bf16x8 row8(const __bf16* p, int have) {
+  bf16x8 r;
+  if (have >= 8) {
+    __builtin_memcpy(&r, p, sizeof(r));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r[e] = e < have ? p[e] : (__bf16)0.f;
+  }
+  return r;
+}
+
+// The router's product. Two logits that are close decide which expert runs, so
+// neither the weights nor the result are rounded to bf16: each weight is the
+// sum of three bf16 numbers, whose products with x are exact in f32, and a
+// matrix instruction more for each costs little beside the loads. A wave takes
+// RT x NT tiles of 16 rows and 16 experts, KS of them share K. The two small
+// parts are summed apart: with an infinite value of x they, being 0 as a rule,
+// would make NaN of it. Bound by how long its loads from the L2 take: 196 x
+// 768, 64 experts 4.8 us, 12544 x 768, 64 19 (0.2 PFLOP/s of its instructions);
+// the product into bf16 takes 14 and 23.
+template <int RT, int NT, int KS>
+__global__ __launch_bounds__(512) void logits_kernel(Logits p) {
+  __shared__ __attribute__((aligned(16))) float part[KS > 1 ? 2 * 8 * 256 : 1];
+  const int lane = threadIdx.x & 63, l = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tiles_n = (p.E + NT * 16 - 1) / (NT * 16);
+  const int64_t rows = blockIdx.x / tiles_n;
+  const int n0 = (int)(blockIdx.x - rows * tiles_n) * NT * 16;
+  const int ks = wave % KS;
+  const int64_t m0 = (rows * (8 / KS) + wave / KS) * RT * 16;
+  f32x4 acc[RT][NT] = {}, rest[RT][NT] = {};
+  const __bf16 *x[RT], *w[NT];
+#pragma unroll
+  for (int i = 0; i < RT; ++i)
+    x[i] = p.X + min(m0 + i * 16 + l, (int64_t)p.T - 1) * p.ldx;
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+    w[t] = p.W + (int64_t)min(n0 + t * 16 + l, p.E - 1) * p.Dp;
+  const int64_t next = (int64_t)p.E * p.Dp;
+  const int steps = m0 < p.T ? p.Dp / 32 : 0;
+#pragma unroll 2
+  for (int s = steps * ks / KS; s < steps * (ks + 1) / KS; ++s) {
+    const int k = s * 32 + g * 8;
+    bf16x8 a[RT], b[NT][3];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int j = 0; j < 3; ++j)
+        b[t][j] = *(const bf16x8*)(w[t] + j * next + k);
+#pragma unroll
+    for (int i = 0; i < RT; ++i) a[i] = row8(x[i] + k, p.D - k);
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+            b[t][0], a[i], acc[i][t], 0, 0, 0);
+        rest[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+            b[t][2], a[i], rest[i][t], 0, 0, 0);
+        rest[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+            b[t][1], a[i], rest[i][t], 0, 0, 0);
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < RT; ++i)
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      if (KS > 1 && (i || t)) __syncthreads();  // the last sum has been read
+      const f32x4 sum = few_join<KS>(acc[i][t], part, wave / KS, ks, lane);
+      const f32x4 more =
+          few_join<KS>(rest[i][t], part + 8 * 256, wave / KS, ks, lane);
+      const int64_t m = m0 + i * 16 + l;
+      const int n = n0 + t * 16 + g * 4;
+      if (ks || m >= p.T) continue;
+      float v[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        v[c] = fabsf(sum[c]) < INFINITY ? sum[c] + more[c] : sum[c];
+      store_run(p.Y + m * p.E + n, p.E - n, v);
+    }
+}
 
 // ------------------------------------------------------------ moe_route
 
@@ -1374,6 +1468,35 @@ void run_mlp(const MoeMlp& m, const Layout& l, char* ws, hipStream_t stream) {
 }
 
 }  // namespace
+
+void launch_moe_logits(const void* X, int64_t ldx, const void* W, float* Y,
+                       int T, int D, int E, hipStream_t stream) {
+  const Logits p{(const __bf16*)X, (const __bf16*)W, Y, ldx, T, D,
+                 up(D, 64) * 64, E};
+  auto go = [&](auto rt, auto nt, auto ks) {
+    constexpr int RT = decltype(rt)::value, NT = decltype(nt)::value,
+                  KS = decltype(ks)::value;
+    hipLaunchKernelGGL((logits_kernel<RT, NT, KS>),
+                       dim3(up(T, 8 / KS * RT * 16) * up(E, NT * 16)),
+                       dim3(512), 0, stream, p);
+  };
+  // Few tiles: all 8 waves share K; many: each load serves more products. In
+  // us, for <1, 1, 8> / <2, 1, 4> / <4, 2, 4>: 1 x 768, 64 experts: 4.2 / 4.9 /
+  // 9.6, 1568 x 768, 64: 7.6 / 9.1 / 18, 12544 x 768, 8: 9.7 / 7.7 / 14,
+  // 3136 x 768, 64: 12.9 / 9.2 / 18, 12544 x 768, 64: 36 / 29 / 19, 256:
+  // 130 / 88 / 72.
+  using std::integral_constant;
+  const int64_t tiles = (int64_t)up(T, 16) * up(E, 16);
+  if (tiles <= 512)
+    go(integral_constant<int, 1>(), integral_constant<int, 1>(),
+       integral_constant<int, 8>());
+  else if (tiles <= 1536)
+    go(integral_constant<int, 2>(), integral_constant<int, 1>(),
+       integral_constant<int, 4>());
+  else
+    go(integral_constant<int, 4>(), integral_constant<int, 2>(),
+       integral_constant<int, 4>());
+}
 
 void launch_moe_route(const void* X, bool f32, int64_t ldx, const float* bias,
                       int* ids, float* weights, int T, int E, int k,

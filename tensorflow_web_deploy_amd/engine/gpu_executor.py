@@ -192,6 +192,22 @@ class GpuExecutor:
                                                     else w.t())
         return self._weights[key]
 
+    def _prep_router_weight(self, wname: str):
+        """[K, E] -> [3, E, K filled up with zeros] in bf16: the weight's
+        rounding and those of what is left of it"""
+        key = wname + "/parts"
+        if key not in self._weights:
+            w = torch.from_numpy(np.ascontiguousarray(
+                self.consts[wname], np.float32)).t()
+            K = w.shape[1]
+            w = torch.nn.functional.pad(w, (0, _pad64(K) - K))
+            parts = []
+            for _ in range(3):
+                parts.append(w.to(torch.bfloat16))
+                w = w - parts[-1].float()
+            self._weights[key] = torch.stack(parts).to(self.device)
+        return self._weights[key]
+
     def _prep_expert_weight(self, wname: str):
         """[E, K, N] -> [E, N, K filled up with zeros] and, in e4m3, the
         scales of each expert"""
@@ -544,7 +560,7 @@ class GpuExecutor:
             elif op == "MoeMLP":
                 xn, rn, w1n, b1n, w2n, b2n = node.inputs[:6]
                 at = node.attrs
-                wr, K, NE, _, Ep = self._prep_dense_weight(rn, False)
+                K, NE = self.consts[rn].shape
                 A2 = bufs[xn].view(-1, K)
                 M = A2.shape[0]
                 w1, s1 = self._prep_expert_weight(w1n)
@@ -553,12 +569,20 @@ class GpuExecutor:
                 b2 = self._bias(b2n, 0).view(NE, -1)
                 rb = self._bias(node.inputs[6] if len(node.inputs) > 6
                                 else None, NE)
-                lg = torch.zeros((M, Ep), dtype=torch.bfloat16, device=dev)
+                if at.get("logits") == "f32":
+                    wr = self._prep_router_weight(rn)
+                    lg = torch.zeros((M, NE), device=dev)
+                    steps.append(lambda A2=A2, wr=wr, lg=lg:
+                                 E.moe_logits(A2, wr, lg))
+                else:
+                    wr, _, _, _, Ep = self._prep_dense_weight(rn, False)
+                    lg = torch.zeros((M, Ep), dtype=torch.bfloat16,
+                                     device=dev)
+                    steps.append(lambda A2=A2, wr=wr, lg=lg, K=K:
+                                 E.gemm_bf16(A2, wr, lg, None, None, K, 0))
                 ids = torch.zeros((M, int(at["k"])), dtype=torch.int32,
                                   device=dev)
                 pw = torch.zeros(ids.shape, device=dev)
-                steps.append(lambda A2=A2, wr=wr, lg=lg, K=K:
-                             E.gemm_bf16(A2, wr, lg, None, None, K, 0))
                 how = (("softmax", "sigmoid").index(at["score"]),
                        int(at["groups"]), int(at["kept"]), int(at["best"]),
                        bool(at["renorm"]), float(at["scale"]))

@@ -165,12 +165,19 @@ class GraphBuilder:
     def moe(self, x: str, name: str, dim: int, hidden: int, experts: int,
             k: int, score: str = "softmax", groups: int = 1, kept: int = 1,
             best: int = 1, renorm: bool = True, scale: float = 1.0,
-            act: str = "gelu", router_bias: bool = False) -> str:
+            act: str = "gelu", router_bias: bool = False,
+            logits: str = "bf16") -> str:
         """Mixture of experts over the last axis: a router without a bias of
         its own scores the experts, the k best ones (router_bias added for
         the choice alone; out of the `kept` groups of experts whose `best`
         largest add up to the most) each run act(x W1 + b1) W2 + b2, and
-        their scores weight the sum."""
+        their scores weight the sum. logits: the type in which the GPU keeps
+        the router's weights and logits. In bf16, as a graph has it that
+        doesn't say, logits that are close become equal, the more often the
+        more experts there are, and the lower index wins; in f32 the choice
+        is that of the products."""
+        if logits not in ("bf16", "f32"):
+            raise ValueError(f"logits must be bf16 or f32, got {logits}")
         ins = [x,
                self.weight(f"{name}/router/w", (dim, experts),
                            scale=float(np.sqrt(1.0 / dim)))]
@@ -186,7 +193,7 @@ class GraphBuilder:
                     experts)).astype(np.float32)))
         return self.node("MoeMLP", name, ins, k=k, score=score, groups=groups,
                          kept=kept, best=best, renorm=renorm,
-                         scale=float(scale), act=act)
+                         scale=float(scale), act=act, logits=logits)
 
     def softmax(self, x: str, name: str = "softmax") -> str:
         return self.node("Softmax", name, [x])

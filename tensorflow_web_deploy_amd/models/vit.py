@@ -130,7 +130,7 @@ def build_vit_b16(seed: int = 0, num_classes: int = NUM_CLASSES,
         ln2 = _layernorm(b, y, f"layer{i}/ln2", DIM)
         if experts and i % 2:
             mlp = b.moe(ln2, f"layer{i}/moe", DIM, MLP, experts,
-                        experts_per_token)
+                        experts_per_token, logits="f32")
         else:
             mlp = _mlp(b, ln2, f"layer{i}/mlp")
         y = b.node("AddV2", f"layer{i}/res2", [mlp, y])

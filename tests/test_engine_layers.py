@@ -297,3 +297,61 @@ def test_fp8_lenet():
         (8, 28, 28, 1), dtype=np.float32))
     assert p.shape == (8, 10) and (p >= 0).all()
     np.testing.assert_allclose(p.sum(1), 1.0, atol=1e-3)
+
+
+# ----------------------------------------------------- the router's logits
+
+
+def test_vit_routes_on_f32():
+    from tensorflow_web_deploy_amd.models import vit
+    g = ir.optimize(ir.from_graphdef(vit.build_vit_b16(experts=2),
+                                     outputs=["softmax"]))
+    moe = [n for n in g.nodes if n.op == "MoeMLP"]
+    assert moe and all(n.attrs["logits"] == "f32" for n in moe)
+
+
+def test_builder_refuses_other_logits():
+    with pytest.raises(ValueError, match="logits"):
+        model(dict(experts=4, k=1, logits="f16"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp8"])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_router_decides_on_f32_logits(dtype, score, monkeypatch):
+    """The engine's choices against those on logits in 64 bits, of the same
+    bf16 rows and the graph's own weights: another expert only where the
+    scores lie within what the f32 sums may be off. Logits rounded to bf16
+    choose others in some rows."""
+    from test_moe import logits_error
+    from tensorflow_web_deploy_amd.ops.native import ext
+    E, k = ext(), 4
+    g = graph(dict(experts=64, k=k, score=score, logits="f32"))
+    seen = []
+    route = E.moe_route
+
+    def spy(logits, bias, ids, *a):
+        route(logits, bias, ids, *a)
+        seen.append((logits, ids))
+
+    monkeypatch.setattr(E, "moe_route", spy)
+    eng = engine(g, dtype=dtype, use_hip_graphs=False)
+    eng.ex.run({"input": torch.from_numpy(images(40))})
+    torch.cuda.synchronize()
+    (logits, ids), = seen
+    assert logits.dtype == torch.float32
+    x = eng.ex._plans[40].bufs["branches"].view(-1, DIM).cpu().double()
+    w = torch.from_numpy(g.consts["experts/router/w"]).t().contiguous()
+    exact, err = x @ w.double().t(), logits_error(x, w)
+    p = (torch.softmax(exact, -1) if score == "softmax"
+         else torch.sigmoid(exact))
+    # a score moves by no more than itself times two logits' errors
+    err = 2 * err.amax(1, keepdim=True) * p * 1.01 + 2.0 ** -50
+    best = p.sort(-1, descending=True).values[:, :k]
+    mine = p.gather(1, ids.cpu().long())
+    assert (mine >= best - 2 * err.amax(1, keepdim=True)).all()
+    a = ("softmax", "sigmoid").index(score), 1, 1, 1, True, 1.0
+    want = route_ref(exact, None, k, *a)[0]
+    rounded = route_ref(exact.to(torch.bfloat16), None, k, *a)[0]
+    assert (rounded != want).any()
+    assert (ids.cpu() != want).sum() * 10 < (rounded != want).sum()

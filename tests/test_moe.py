@@ -728,3 +728,127 @@ def test_route_many_ties_at_the_cut(E, score, e, k, groups, kept):
     check_route(E, x.cuda(), b, k, score, groups, kept, 2)
     x = x.to(torch.bfloat16)  # equal logits alone
     check_route(E, x.cuda(), None, k, score, groups, kept, 2)
+
+
+# ------------------------------------------------------------ moe_logits
+
+
+def in_parts(w):
+    """f32 [E, D] as the sum of three bf16 numbers each, D filled up to 64s"""
+    w = torch.nn.functional.pad(w, (0, -w.shape[1] % 64))
+    parts = []
+    for _ in range(3):
+        parts.append(w.to(torch.bfloat16))
+        w = w - parts[-1].float()
+    return torch.stack(parts)
+
+
+@pytest.mark.parametrize("kw,word", [
+    ({"X": torch.zeros(3, 100)}, "X must be BFloat16"),
+    ({"X": torch.zeros(100, 3, dtype=torch.bfloat16).t()}, "contiguous rows"),
+    ({"X": torch.zeros(300, dtype=torch.bfloat16)}, "2D"),
+    ({"X": torch.zeros(3, 0, dtype=torch.bfloat16)}, "width must be"),
+    ({"X": torch.empty(1 << 27, 100, dtype=torch.bfloat16, device="meta")},
+     "too many rows"),
+    ({"W": torch.zeros(3, 8, 128)}, "W must be BFloat16"),
+    ({"W": torch.zeros(3, 8, 100, dtype=torch.bfloat16)}, "W must be"),
+    ({"W": torch.zeros(2, 8, 128, dtype=torch.bfloat16)}, "W must be"),
+    ({"W": torch.zeros(3, 513, 128, dtype=torch.bfloat16)}, "512 experts"),
+    ({"W": torch.zeros(3 * 8 * 128 + 4, dtype=torch.bfloat16)[4:].view(
+        3, 8, 128)}, "W must start at a multiple of 16"),
+    ({"logits": torch.zeros(3, 8, dtype=torch.bfloat16)}, "logits must be"),
+    ({"logits": torch.zeros(3, 7)}, "logits must be"),
+    ({}, "X must be on GPU"),
+])
+def test_logits_refuses(E, kw, word):
+    a = {"X": torch.zeros(3, 100, dtype=torch.bfloat16),
+         "W": torch.zeros(3, 8, 128, dtype=torch.bfloat16),
+         "logits": torch.zeros(3, 8)}
+    a.update(kw)
+    with pytest.raises(RuntimeError, match=word):
+        E.moe_logits(**a)
+
+
+def logits_error(x, w):
+    """3 D products, which are exact, added in f32, no addition off by more
+    than 2^-23 of the terms' size; what three bf16 numbers lose of an f32 one
+    is under 2^-24 of it."""
+    n = 3 * w.shape[1] + 32
+    return n * 2.0 ** -23 * (x.double().abs() @ w.double().abs().t())
+
+
+def check_logits(E, x, w):
+    got = torch.full((x.shape[0], w.shape[0]), math.nan, device="cuda")
+    E.moe_logits(x, in_parts(w).cuda(), got)
+    x = x.cpu()
+    off = (got.cpu().double() - x.double() @ w.double().t()).abs()
+    assert (off <= logits_error(x, w) + 1e-38).all()
+    return got
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t,d,e", [
+    (1, 1, 1), (1, 768, 64), (3, 64, 16), (16, 100, 17), (17, 7, 33),
+    (64, 72, 12), (65, 130, 500), (196, 768, 64), (1000, 2048, 8),
+    (1030, 513, 130), (5000, 200, 64), (9001, 100, 35)])
+def test_logits(E, t, d, e):
+    g = torch.Generator().manual_seed(t + d + e)
+    x = torch.randn(t, d, generator=g).to(torch.bfloat16)
+    w = torch.randn(e, d, generator=g) * d ** -0.5
+    check_logits(E, x.cuda(), w)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [5, 3000])
+def test_logits_of_rows_that_lie_apart(E, t):
+    g = torch.Generator().manual_seed(t)
+    wide = torch.randn(t, 151, generator=g).to(torch.bfloat16).cuda()
+    w = torch.randn(20, 97, generator=g)
+    for at in (0, 1, 8):
+        check_logits(E, wide[:, at:at + 97], w)
+    assert check_logits(E, wide[:0, :97], w).shape == (0, 20)
+    x = far_rows(5, 97, 2 ** 30 + 3)
+    x.copy_(wide[:5, :97])
+    check_logits(E, x, w)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [6, 3000])
+def test_logits_of_infinite_rows(E, t):
+    """As the products by definition: infinite by the weight's sign, NaN where
+    two of them differ; the other rows aren't touched."""
+    g = torch.Generator().manual_seed(t)
+    x = torch.randn(t, 80, generator=g).to(torch.bfloat16)
+    w = torch.randn(10, 80, generator=g).bfloat16().float()  # parts are 0
+    want = check_logits(E, x.cuda(), w)
+    x[1, 3], x[2, 4], x[2, 5], x[4, 79] = (math.inf, math.inf, math.inf,
+                                           -math.inf)
+    x[5, 0] = math.nan
+    got = torch.empty_like(want)
+    E.moe_logits(x.cuda(), in_parts(w).cuda(), got)
+    ref = x.double() @ w.double().t()
+    for r in (1, 2, 4, 5):
+        assert torch.equal(got[r].cpu().isnan(), ref[r].isnan())
+        assert torch.equal(got[r].cpu().nan_to_num(nan=0, posinf=1, neginf=-1),
+                           ref[r].float().nan_to_num(nan=0, posinf=1,
+                                                     neginf=-1))
+        got[r] = want[r]
+    assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+def test_logits_in_a_graph(E):
+    g = torch.Generator().manual_seed(1)
+    x = torch.zeros(300, 96, dtype=torch.bfloat16, device="cuda")
+    w = in_parts(torch.randn(24, 96, generator=g)).cuda()
+    y, eager = (torch.empty(300, 24, device="cuda") for _ in range(2))
+    E.moe_logits(x, w, y)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        E.moe_logits(x, w, y)
+    for _ in range(3):
+        x.copy_(torch.randn(300, 96, generator=g))
+        graph.replay()
+        E.moe_logits(x, w, eager)
+        torch.cuda.synchronize()
+        assert torch.equal(y, eager)
