@@ -365,8 +365,9 @@ void check_devices(c10::ArrayRef<std::pair<const torch::Tensor*, const char*>>
 }
 
 // a launch holds fewer than 2^32 threads along x: with 16 rows, or a tile of
-// 128 x 128, to a workgroup of 256
+// 128 x 128, to a workgroup of 256, or 16 columns to one of 512
 constexpr int64_t kMaxRows = 1 << 27, kMaxTiles = 1 << 24;
+constexpr int64_t kMaxColumns = (1 << 27) - 16;
 
 int64_t blocks128(int64_t n) { return (n + 127) / 128; }
 
@@ -415,7 +416,7 @@ void gemm_fp8(torch::Tensor A, torch::Tensor SA, torch::Tensor B,
   TORCH_CHECK(Kp >= 128 && Kp % 128 == 0 && Kp <= 1 << 22,
               "A must hold whole blocks of 128 along K, 2^22 values at most, "
               "got ", Kp);
-  TORCH_CHECK(N >= 1 && N < kMaxRows && M < kMaxRows &&
+  TORCH_CHECK(N >= 1 && N <= kMaxColumns && M < kMaxRows &&
                   blocks128(M) * blocks128(N) < kMaxTiles,
               "C is too large or has no columns: ", C.sizes());
   TORCH_CHECK(M * (Kp / 128) < 1 << 30, "SA is too large");
@@ -467,6 +468,9 @@ void moe_logits(torch::Tensor X, torch::Tensor W, torch::Tensor logits) {
   TORCH_CHECK(W.dim() == 3, "W must be 3D");
   const int64_t E = W.size(1);
   TORCH_CHECK(E >= 1 && E <= 512, "1 to 512 experts, got ", E);
+  // 128 rows and 32 experts to a workgroup of 512 threads
+  TORCH_CHECK((T + 127) / 128 * ((E + 31) / 32) < 1 << 23,
+              "too many rows: ", T);
   check_whole(W, torch::kBFloat16, {3, E, (D + 63) / 64 * 64}, "W");
   check_aligned(W, "W");
   check_whole(logits, torch::kFloat32, {T, E}, "logits");

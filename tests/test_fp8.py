@@ -541,3 +541,12 @@ def test_gemm_f32_in_a_graph(E):
         assert torch.equal(c, want)
         E.gemm_fp8(*ops, want)
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("m,n", [(4, (1 << 27) - 1), (16, (1 << 27) - 15),
+                                 (20, (1 << 27) - 1)])
+def test_gemm_refuses_a_launch_too_large(E, m, n):
+    """16 columns to 512 threads: a launch of 2^32 threads isn't one."""
+    c = torch.empty(m, n, dtype=torch.bfloat16, device="meta")
+    with pytest.raises(RuntimeError, match="C is too large"):
+        E.gemm_fp8(**_gemm_args(m=m, C=c))

@@ -852,3 +852,13 @@ def test_logits_in_a_graph(E):
         E.moe_logits(x, w, eager)
         torch.cuda.synchronize()
         assert torch.equal(y, eager)
+
+
+def test_logits_refuses_a_launch_too_large(E):
+    """128 rows and 32 experts to 512 threads, fewer than 2^32 of them"""
+    t = 1 << 26
+    with pytest.raises(RuntimeError, match="too many rows"):
+        E.moe_logits(
+            torch.empty(t, 64, dtype=torch.bfloat16, device="meta"),
+            torch.zeros(3, 512, 64, dtype=torch.bfloat16),
+            torch.empty(t, 512, device="meta"))
