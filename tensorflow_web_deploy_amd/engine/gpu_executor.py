@@ -188,8 +188,8 @@ class GpuExecutor:
         if key not in self._weights:
             w = torch.from_numpy(np.ascontiguousarray(
                 self.consts[wname], np.float32))
-            self._weights[key] = self._quant_weight(w if transpose_b
-                                                    else w.t())
+            w = w if transpose_b else w.t()
+            self._weights[key] = *self._quant_weight(w), w.shape[1]
         return self._weights[key]
 
     def _prep_router_weight(self, wname: str):
@@ -361,10 +361,11 @@ class GpuExecutor:
                 continue
             if self.fp8 and self._is_dense(node):
                 q, qs = rounded[node.inputs[0]]
-                wt, ws = self._prep_dense_weight_fp8(
+                wt, ws, K = self._prep_dense_weight_fp8(
                     node.inputs[1], bool(node.attrs.get("transpose_b")))
                 N = wt.shape[0]
-                assert q.shape[1] == wt.shape[1], \
+                # q and wt are filled up to whole blocks: they don't tell
+                assert shapes[node.inputs[0]][-1] == K, \
                     f"dense K mismatch {node.name}"
                 bias = self._bias(node.attrs.get("bias"), N)
                 act = (2 if node.attrs.get("relu6") else
@@ -561,6 +562,12 @@ class GpuExecutor:
                 xn, rn, w1n, b1n, w2n, b2n = node.inputs[:6]
                 at = node.attrs
                 K, NE = self.consts[rn].shape
+                Hd = self.consts[w1n].shape[2]
+                # filled up to whole steps below: what they are is seen here
+                assert (shapes[xn][-1] == K
+                        and self.consts[w1n].shape == (NE, K, Hd)
+                        and self.consts[w2n].shape == (NE, Hd, K)), \
+                    f"experts' widths mismatch {node.name}"
                 A2 = bufs[xn].view(-1, K)
                 M = A2.shape[0]
                 w1, s1 = self._prep_expert_weight(w1n)

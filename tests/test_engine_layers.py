@@ -355,3 +355,48 @@ def test_router_decides_on_f32_logits(dtype, score, monkeypatch):
     rounded = route_ref(exact.to(torch.bfloat16), None, k, *a)[0]
     assert (rounded != want).any()
     assert (ids.cpu() != want).sum() * 10 < (rounded != want).sum()
+
+
+# ------------------------------------------- weights of another width
+
+
+def mismatched(op):
+    """Rows of 16 values: before a dense weight for 24 of them, before experts
+    for 8."""
+    b = GraphBuilder(seed=1)
+    x = b.placeholder("input", [-1, H, W, C])
+    x = b.reshape(x, "tokens", [-1, H * W * C // 16, 16])
+    if op == "experts":
+        x = b.moe(x, "layer", 8, 40, experts=4, k=2)
+    elif op == "DenseND":
+        x = b.node("BatchMatMulV2", "layer", [x, b.weight("w", (24, 16))])
+        x = b.node("AddV2", "layer/bias", [
+            x, b.const("layer/b", np.zeros(16, np.float32))])
+    else:
+        x = b.reshape(x, "rows", [-1, 16])
+        x = b.dense(x, "layer", 24, 16)
+    b.node("Relu", "out", [x])
+    return ir.optimize(ir.from_graphdef(b.graphdef(), outputs=["out"]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp8"])
+@pytest.mark.parametrize("op", ["Dense", "DenseND", "experts"])
+def test_a_weight_of_another_width_is_refused(op, dtype):
+    g = mismatched(op)
+    eng = engine(g, dtype=dtype, use_hip_graphs=False)
+    with pytest.raises((AssertionError, RuntimeError),
+                       match="mismatch|invalid for input of size"):
+        eng.ex.run({"input": torch.from_numpy(images(4))})
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp8"])
+@pytest.mark.parametrize("part,shape", [("fc1", (6, 70, HID)),
+                                        ("fc2", (6, HID - 4, DIM))])
+def test_experts_of_another_width_are_refused(part, shape, dtype):
+    g = graph(MIXES[0])
+    g.consts[f"experts/{part}/w"] = np.ones(shape, np.float32)
+    eng = engine(g, dtype=dtype, use_hip_graphs=False)
+    with pytest.raises(AssertionError, match="mismatch"):
+        eng.ex.run({"input": torch.from_numpy(images(4))})
