@@ -168,17 +168,21 @@ __device__ __forceinline__ DenseTile dense_tile(
   const auto rb = buffer(d.B + (int64_t)n0 * d.Kp, (uint32_t)cols * d.Kp);
   const auto rs = buffer(d.SA, (uint32_t)all * d.M * 4);
   Rows<S> at;
-  rows_of_a<S>(at, wave, lane,
-               [&](int r) { return (uint32_t)min(r, rows - 1) * d.Kp; });
-  rows_of_b<S>(at, wave, lane,
-               [&](int r) { return (uint32_t)min(r, cols - 1) * d.Kp; });
-  at.s = (uint32_t)(m0 + min(scale_row<S>(wave, lane), rows - 1)) * 4;
+  auto row_a = [&](int r) { return (uint32_t)min(r, rows - 1) * d.Kp; };
+  auto row_b = [&](int r) { return (uint32_t)min(r, cols - 1) * d.Kp; };
+  auto row_s = [&](int r) { return (uint32_t)(m0 + min(r, rows - 1)) * 4; };
+  rows_of_a<S>(at, wave, lane, row_a);
+  rows_of_b<S>(at, wave, lane, row_b);
+  at.s = row_s(scale_row<S>(wave, lane));
   const int wave_m = wave / S::WN * S::MT * 16;
   const int wave_n = wave % S::WN * S::NT * 16;
   const float* sb =
       d.SB + (int64_t)min((n0 + wave_n) / 128, (d.N - 1) / 128) * all;
-  product<S, false, EXACT>(smem, ra, rb, rs, at, first, count,
-                           (uint32_t)d.M * 4, sb, wave, lane, acc);
+  const bool odd =
+      product<S, false, EXACT>(smem, ra, rb, rs, at, first, count,
+                               (uint32_t)d.M * 4, sb, wave, lane, acc);
+  mend_sums<S, EXACT>(ra, rb, rs, row_a, row_b, row_s, first, count,
+                      (uint32_t)d.M * 4, sb, wave, lane, odd, acc);
   return {m0, n0, wave_m, wave_n};
 }
 

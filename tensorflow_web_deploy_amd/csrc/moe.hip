@@ -1033,9 +1033,8 @@ __global__ __launch_bounds__(S::THREADS, 2) void experts_kernel(Experts p) {
                                  (uint32_t)(rows * p.a_row));
   const auto rs = buffer(p.SA, p.sa_rows * 4 * p.steps);
   Rows<S> at;
-  rows_of_b<S>(at, wave, lane, [&](int r) {
-    return (uint32_t)(min(r, cols - 1) * b_row);
-  });
+  auto row_b = [&](int r) { return (uint32_t)(min(r, cols - 1) * b_row); };
+  rows_of_b<S>(at, wave, lane, row_b);
   // The weights go ahead, as where the tile's rows lie is still to come: 33
   // rows of 1000 for 64 experts in e4m3 10.5 -> 9.4 us (8-bit products).
   int row[S::CA], scale = min(scale_row<S>(wave, lane), rows - 1);
@@ -1067,8 +1066,22 @@ __global__ __launch_bounds__(S::THREADS, 2) void experts_kernel(Experts p) {
   const float* sb = S::FP8 ? p.SB + ((int64_t)e * blocks_n +
                                      min(wave_n0 / 128, blocks_n - 1)) * p.steps
                            : nullptr;
-  product<S, true, EXACT>(smem, ra, rb, rs, at, 0, p.steps, p.sa_rows * 4, sb,
-                          wave, lane, acc);
+  const bool odd =
+      product<S, true, EXACT>(smem, ra, rb, rs, at, 0, p.steps, p.sa_rows * 4,
+                              sb, wave, lane, acc);
+  if constexpr (S::FP8) {
+    auto row_of = [&](int r) {
+      r = at0 + min(r, rows - 1);
+      return FIRST ? p.order[r] / p.k : r;
+    };
+    mend_sums<S, EXACT>(
+        ra, rb, rs,
+        [&](int r) {
+          return (uint32_t)((row_of(r) - (FIRST ? 0 : at0)) * p.a_row);
+        },
+        row_b, [&](int r) { return (uint32_t)row_of(r) * 4; }, 0, p.steps,
+        p.sa_rows * 4, sb, wave, lane, odd, acc);
+  }
 
   const int row0 = wm * S::MT * 16;
   if (rows == S::BM && n0 + S::BN <= p.n)

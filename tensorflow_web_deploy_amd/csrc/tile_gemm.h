@@ -223,18 +223,49 @@ __device__ __forceinline__ i32x8 both(const i32x4 (&v)[2]) {
   return __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
+// the column, counted from the tile's first, that row i16 of a wave's tile t of
+// B stands for
+template <class S>
+__device__ __forceinline__ int column_of(int wn, int t, int i16) {
+  constexpr int Q = S::W / 4;
+  return wn * S::NT * 16 + t / Q * 4 * S::W + (i16 >> 2) * S::W + t % Q * 4 +
+         (i16 & 3);
+}
+
+// Blocks are scaled by the product of their two scales, which may leave the
+// range of f32 where the scaled block doesn't: by an infinite one a block of 0
+// becomes NaN, a subnormal one has lost bits. Both are factors above 1, or below,
+// then, and one after the other they lose nothing.
+struct Factors {
+  float most = 0.f, least = 1.f;
+
+  __device__ __forceinline__ void see(float f) {
+    most = fmaxf(most, fabsf(f));
+    least = fminf(least, fabsf(f));
+  }
+  __device__ __forceinline__ bool odd() const {
+    return !(most < INFINITY && least >= 0x1p-126f);
+  }
+};
+
+__device__ __forceinline__ float add_scaled(float sum, float p, float sa,
+                                            float sb) {
+  const float f = sa * sb;
+  return __builtin_amdgcn_classf(f, 0x108)  // normal
+             ? __builtin_fmaf(p, f, sum)
+             : sum + p * sa * sb;
+}
+
 template <class S, bool EXACT>
 __device__ __forceinline__ void compute(const char* lds, float sb, int wm,
-                                        int wn, int lane,
+                                        int wn, int lane, Factors& seen,
                                         f32x4 (&acc)[S::MT][S::NT]) {
   const int i16 = lane & 15, g = lane >> 4;
   const char* ldsb = lds + S::BM * STEP;
   i32x4 b[S::NT][2];
 #pragma unroll
   for (int t = 0; t < S::NT; ++t) {
-    constexpr int Q = S::W / 4;
-    const int n = wn * S::NT * 16 + t / Q * 4 * S::W + (i16 >> 2) * S::W +
-                  t % Q * 4 + (i16 & 3);
+    const int n = column_of<S>(wn, t, i16);
     const char* row = ldsb + n * STEP;
     const int key = key_b<S>(n);
     b[t][0] = *(const i32x4*)(row + ((g ^ key) << 4));
@@ -245,6 +276,7 @@ __device__ __forceinline__ void compute(const char* lds, float sb, int wm,
     for (int i = 0; i < S::MT; ++i) {
       const FragA<S> a = read_a<S>(lds, wm, i, lane);
       const float f = a.f * sb;
+      seen.see(f);
       f32x4 p[S::NT];
       exact_products(b, a.v, p);
 #pragma unroll
@@ -281,6 +313,10 @@ __device__ __forceinline__ void compute(const char* lds, float sb, int wm,
             acc[i - 1][t][r] = __builtin_fmaf(p[(i - 1) & 1][t][r],
                                               f[(i - 1) & 1],
                                               acc[i - 1][t][r]);
+        if (t == S::NT - 1 && i < S::MT && (i & 1 || i == S::MT - 1)) {
+          if (i & 1) seen.see(f[0]);
+          seen.see(f[i & 1]);
+        }
         __builtin_amdgcn_sched_barrier(0);
       }
     }
@@ -308,9 +344,9 @@ __device__ __forceinline__ void compute(const char* lds, float sb, int wm,
 
 // Steps [first, first + count) of the product. sb: the scales of the wave's
 // columns, one a step. B_SENT: send_b has been called. EXACT: e4m3 by the f16
-// instruction.
+// instruction. The answer: whether one of this lane's factors was odd.
 template <class S, bool B_SENT, bool EXACT>
-__device__ __forceinline__ void product(char* smem, __amdgpu_buffer_rsrc_t ra,
+__device__ __forceinline__ bool product(char* smem, __amdgpu_buffer_rsrc_t ra,
                                         __amdgpu_buffer_rsrc_t rb,
                                         __amdgpu_buffer_rsrc_t rs,
                                         const Rows<S>& at, int first,
@@ -336,6 +372,7 @@ __device__ __forceinline__ void product(char* smem, __amdgpu_buffer_rsrc_t ra,
   const auto sbc =
       (const __attribute__((address_space(4))) float*)(uintptr_t)sb;
   float fb = S::FP8 && count > 0 ? sbc[first] : 0.f;
+  Factors seen;
   int now = 0, next = AHEAD % S::DEPTH;
   for (int j = 0; j < count; ++j) {
     // step j has landed once only the later ones are still on their way
@@ -359,12 +396,79 @@ __device__ __forceinline__ void product(char* smem, __amdgpu_buffer_rsrc_t ra,
       stage_a<S>(to, ra, rs, at, first + j + AHEAD, s_stride, wave);
       stage_b<S>(to, rb, at, first + j + AHEAD, wave);
     }
-    compute<S, EXACT>(smem + now * S::STAGE, fb, wm, wn, lane, acc);
+    compute<S, EXACT>(smem + now * S::STAGE, fb, wm, wn, lane, seen,
+                      acc);
     // the stage is free for the load behind the next barrier
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     if (S::FP8) fb = sbc[first + min(j + 1, count - 1)];
     now = now + 1 == S::DEPTH ? 0 : now + 1;
     next = next + 1 == S::DEPTH ? 0 : next + 1;
+  }
+  return seen.odd();
+}
+
+// The sums that a product with an odd factor has left, again and carefully, if
+// it shows in them: some aren't finite, or lie between 2^-126 and 2^-103, where
+// blocks with a subnormal factor end up (2^25 of 2^-126 and of 2^-149). Each
+// wave for itself, from memory to registers, with the rows that row_a, row_b
+// and row_s (a scale's offset) give. The largest and the least of the factors
+// cost the steps 0 to 1%; a class test of each and an OR 2% (16200 x 4096 x 8192
+// 540 / 544 / 552 us), a test of each sum behind the steps up to 9% (12544 x 768
+// x 2304 32.6 / 35.6).
+template <class S, bool EXACT, class A, class B, class C>
+__device__ __forceinline__ void mend_sums(
+    __amdgpu_buffer_rsrc_t ra, __amdgpu_buffer_rsrc_t rb,
+    __amdgpu_buffer_rsrc_t rs, A row_a, B row_b, C row_s, int first, int count,
+    uint32_t s_stride, const float* sb, int wave, int lane, bool odd,
+    f32x4 (&acc)[S::MT][S::NT]) {
+  if (!__any(odd)) return;
+  odd = false;
+#pragma unroll
+  for (int i = 0; i < S::MT; ++i)
+#pragma unroll
+    for (int t = 0; t < S::NT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        // NaN, infinite or subnormal
+        odd |= __builtin_amdgcn_classf(acc[i][t][r] * 0x1p-23f, 0x297);
+  if (!__any(odd)) return;
+  // nothing of this is to be computed ahead, where it would take registers
+  asm volatile("" : "+v"(lane), "+s"(wave));
+  const int wm = wave / S::WN, wn = wave % S::WN, g = lane >> 4;
+  auto load16 = [](__amdgpu_buffer_rsrc_t r, uint32_t at, int step) {
+    return __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                         r, (int)at, step * STEP, 0));
+  };
+#pragma unroll
+  for (int i = 0; i < S::MT; ++i) {
+    const int m = wm * S::MT * 16 + i * 16 + (lane & 15);
+    const uint32_t at_a = row_a(m) + g * 16, at_s = row_s(m);
+#pragma unroll
+    for (int t = 0; t < S::NT; ++t) acc[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+    for (int j = first; j < first + count; ++j) {
+      const i32x4 a[2] = {load16(ra, at_a, j), load16(ra, at_a + 64, j)};
+      const float sa = __builtin_bit_cast(
+          float, __builtin_amdgcn_raw_buffer_load_b32(
+                     rs, (int)at_s, (int)(j * s_stride), 0));
+#pragma unroll
+      for (int t = 0; t < S::NT; ++t) {
+        const uint32_t at_b =
+            row_b(column_of<S>(wn, t, lane & 15)) + g * 16;
+        const i32x4 b[1][2] = {
+            {load16(rb, at_b, j), load16(rb, at_b + 64, j)}};
+        f32x4 p[1];
+        if constexpr (EXACT)
+          exact_products(b, a, p);
+        else
+          p[0] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+              both(b[0]), both(a), f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0,
+              0);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          acc[i][t][r] = add_scaled(acc[i][t][r], p[0][r], sa, sb[j]);
+      }
+    }
   }
 }
 
@@ -381,7 +485,7 @@ __device__ __forceinline__ void product(char* smem, __amdgpu_buffer_rsrc_t ra,
 template <bool FP8, int RT>
 struct FewStep {
   i32x4 a[RT][2], b[1][2];
-  float f[RT];
+  float sa[RT], sb;
 };
 
 template <bool FP8, int RT>
@@ -397,8 +501,8 @@ __device__ __forceinline__ FewStep<FP8, RT> few_step(
     for (int i = 0; i < RT; ++i) r.a[i][h] = *(const i32x4*)(a[i] + k + h * 64);
   }
 #pragma unroll
-  for (int i = 0; i < RT; ++i)
-    r.f[i] = FP8 ? sa[i][step * s_rows] * sb[step] : 0.f;
+  for (int i = 0; i < RT; ++i) r.sa[i] = FP8 ? sa[i][step * s_rows] : 0.f;
+  r.sb = FP8 ? sb[step] : 0.f;
   return r;
 }
 
@@ -418,7 +522,7 @@ __device__ __forceinline__ void few_multiply(const FewStep<FP8, RT>& s,
             0, 0);
 #pragma unroll
       for (int r = 0; r < 4; ++r)
-        acc[i][r] = __builtin_fmaf(p[r], s.f[i], acc[i][r]);
+        acc[i][r] = add_scaled(acc[i][r], p[r], s.sa[i], s.sb);
     } else {
 #pragma unroll
       for (int h = 0; h < 2; ++h)

@@ -550,3 +550,51 @@ def test_gemm_refuses_a_launch_too_large(E, m, n):
     c = torch.empty(m, n, dtype=torch.bfloat16, device="meta")
     with pytest.raises(RuntimeError, match="C is too large"):
         E.gemm_fp8(**_gemm_args(m=m, C=c))
+
+
+# ------------------------- scales whose product leaves the range of f32
+
+WAYS = [(2, 8, 256), (20, 100, 512), (40, 72, 384), (40, 70, 8192),
+        (300, 96, 2048), (500, 520, 1024), (6200, 768, 256), (12500, 761, 128),
+        (4000, 4055, 512), (2300, 2000, 384)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,n,k", WAYS)
+def test_gemm_zero_block_with_any_scales(E, m, n, k, dtype):
+    """A block of weights that are all zero adds nothing, however large its
+    scale and those of the rows are."""
+    qa, sa, qb, sb = operands(E, m, n, k + 128, seed=m)
+    qb.view(torch.uint8)[:, 128:256] = 0
+    want = torch.full((m, n), math.nan, dtype=dtype, device="cuda")
+    E.gemm_fp8(qa, sa, qb, sb, want)
+    sa[1], sb[:, 1] = 0.0, 1.0
+    assert want.isfinite().all()
+    sa[1, ::3], sa[1, 1::3], sb[:, 1] = 1e30, 3e38, 1e20
+    got = torch.full_like(want, math.nan)
+    E.gemm_fp8(qa, sa, qb, sb, got)
+    assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,n,k", WAYS)
+def test_gemm_scales_far_from_one(E, m, n, k, dtype):
+    """Both scales near 2^-73, and near 2^66 with weights of 2^-9 in one
+    place: the result is that of scales near 1 times a power of two. Off by
+    the rounding to C's type, and by two f32 roundings more a block."""
+    eps = torch.finfo(dtype).eps / 2 + (k / 128 + 1) * 3 * 2.0 ** -24
+    sa = torch.full((k // 128, m), 1.3, device="cuda")
+    sb = torch.full((up128(n) // 128, k // 128), 1.2, device="cuda")
+    for value, e in ((448.0, -73), (2.0 ** -9, 66)):
+        qa = torch.full((m, k), value, device="cuda").to(E4M3)
+        qb = torch.full((n, k), value, device="cuda").to(E4M3)
+        if e > 0:  # one product a row, 2^-18
+            qa.view(torch.uint8)[:, 1:] = 0
+        c = torch.full((m, n), math.nan, dtype=dtype, device="cuda")
+        E.gemm_fp8(qa, sa * 2.0 ** e, qb, sb * 2.0 ** e, c)
+        want = (value ** 2 * (k if e < 0 else 1) * sa[0, 0].double().item()
+                * sb[0, 0].double().item())
+        off = (c.double() * 2.0 ** (-2 * e) / want - 1).abs().max().item()
+        assert off <= eps, (e, off, eps)

@@ -862,3 +862,29 @@ def test_logits_refuses_a_launch_too_large(E):
             torch.empty(t, 64, dtype=torch.bfloat16, device="meta"),
             torch.zeros(3, 512, 64, dtype=torch.bfloat16),
             torch.empty(t, 512, device="meta"))
+
+
+# ------------------------- scales whose product leaves the range of f32
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t,e,k", [(1, 4, 2), (8, 4, 2), (40, 8, 2),
+                                   (1500, 4, 2), (9000, 4, 2)])
+def test_mlp_zero_blocks_with_any_scales(E, t, e, k):
+    """Blocks of weights that are all zero add nothing, however large their
+    scales and those of the rows are: in the first product by rows that are
+    large there, in the second by the hidden values' bias."""
+    layer = Layer(E, True, e, 256, 300)
+    x, ids, w = some_rows(t, e, k, 256)
+    x[:, 128:] = 0
+    layer.w[0].view(torch.uint8)[:, :, 128:] = 0
+    layer.w[1].view(torch.uint8)[:, :, 128:256] = 0
+    layer.s[0][:, :, 1] = 1.0
+    layer.s[1][:, :, 1] = 1.0
+    want = layer(x, ids, w, None, 5)
+    layer.check(want, x, ids, w, None, 5)
+    x[:, 128:] = 1e35
+    layer.b1[:, 128:256] = 1e35
+    layer.s[0][:, :, 1] = 1e20
+    layer.s[1][:, :, 1] = 1e20
+    assert torch.equal(layer(x, ids, w, None, 5), want)
