@@ -156,9 +156,10 @@ def route_experts(logits, bias, k, score="softmax", groups=1, kept=1, best=1,
                   renorm=True, scale=1.0):
     """The k experts of each row, the lower index first among equals, and
     their weights; places that no expert is left for get id -1 and weight 0
-    (moe_route's definition, in plain torch ops)."""
+    (moe_route's definition, in plain torch ops). Decided in 64 bits whatever
+    the logits' type, which the weights are rounded to."""
     shut = ~(logits > -math.inf)
-    x = logits.masked_fill(shut, -math.inf)
+    x = logits.double().masked_fill(shut, -math.inf)
     if score == "sigmoid":
         p = torch.sigmoid(x)
     else:
@@ -186,7 +187,7 @@ def route_experts(logits, bias, k, score="softmax", groups=1, kept=1, best=1,
     if renorm:
         total = w.sum(-1, keepdim=True)
         w = torch.where(total > 0, w / total, 0.0)
-    return ids.masked_fill(none, -1), w * scale
+    return ids.masked_fill(none, -1), (w * scale).to(logits.dtype)
 
 
 @cpu_op("MoeMLP")

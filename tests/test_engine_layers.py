@@ -400,3 +400,24 @@ def test_experts_of_another_width_are_refused(part, shape, dtype):
     eng = engine(g, dtype=dtype, use_hip_graphs=False)
     with pytest.raises(AssertionError, match="mismatch"):
         eng.ex.run({"input": torch.from_numpy(images(4))})
+
+
+# --------------------------------- choices by the CPU, on logits in f32
+
+
+@pytest.mark.parametrize("score", [0, 1])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_route_experts_decides_in_64_bits(score, dtype):
+    """Scores that f32 can't tell apart; the weights are of the rows' type."""
+    g = torch.Generator().manual_seed(score)
+    x = (torch.randint(0, 40, (60, 16), generator=g) * 1e-9).to(dtype)
+    x[:20] += 1 + torch.randint(0, 4, (20, 16), generator=g) * 2.0 ** -23
+    x[0] = torch.tensor([0, 0, 1e-9, -5] * 4).to(dtype)
+    bias = torch.randint(0, 3, (16,), generator=g) * 2.0 ** -26 + 0.25
+    for b in (None, bias):
+        ids, w = route_experts(x, b, 4, ("softmax", "sigmoid")[score],
+                               scale=2.5)
+        want = route_ref(x, b, 4, score, 1, 1, 1, True, 2.5)
+        assert w.dtype == dtype and torch.equal(ids.int(), want[0])
+        off = (w.double() - want[1]).abs()
+        assert (off <= torch.finfo(dtype).eps * want[1]).all()
