@@ -635,13 +635,15 @@ __global__ __launch_bounds__(256) void route_kernel(Route p) {
   if (p.renorm && id[0] >= 0 && !(sum > 1e-30f)) safe = false;
   const uint64_t unsafe = __ballot(!safe);
   const bool again = unsafe >> (lane & 48) & 0xffff;
-  const float scale = p.renorm ? (sum > 0.f ? p.scale / sum : 0.f) : p.scale;
+  // of all the chosen: no more than 2^100, where the scale over the sum may
+  // leave the range
+  const float over = p.renorm ? (sum > 0.f ? 1.f / sum : 0.f) : 1.f;
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     const int j = q * 16 + l;
     if (j >= p.k || t >= p.T || again) continue;
     p.ids[t * p.k + j] = id[q];
-    p.weights[t * p.k + j] = w[q] * scale;
+    p.weights[t * p.k + j] = w[q] * over * p.scale;
   }
   if (!unsafe) return;
   // the rows of the wave are done with LDS: it now holds numbers of 64 bits

@@ -888,3 +888,12 @@ def test_mlp_zero_blocks_with_any_scales(E, t, e, k):
     layer.s[0][:, :, 1] = 1e20
     layer.s[1][:, :, 1] = 1e20
     assert torch.equal(layer(x, ids, w, None, 5), want)
+
+
+@pytest.mark.gpu
+def test_route_large_scale(E):
+    """The scale over a small sum of scores leaves f32's range, the weights
+    don't."""
+    x = torch.tensor([[-60.0, -61, -62], [-55, -58, -50], [0, 1, 2]]).cuda()
+    for scale in (1e35, 1e38, -1e36):
+        check_route(E, x, None, 2, 1, renorm=True, scale=scale)
