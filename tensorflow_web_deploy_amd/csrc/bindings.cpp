@@ -353,6 +353,45 @@ void check_act(int64_t act) {
               act);
 }
 
+// Whether two tensors, each whole or rows that may lie apart, share a byte.
+// Rows of one width apart from each other may lie beside those of the other.
+bool overlap(const torch::Tensor& a, const torch::Tensor& b) {
+  if (!a.numel() || !b.numel() || a.is_meta() || b.is_meta()) return false;
+  auto rows = [](const torch::Tensor& t) {
+    return t.dim() == 2 && t.size(0) > 1;
+  };
+  auto width = [&](const torch::Tensor& t) {
+    return (rows(t) ? t.size(1) : t.numel()) * (int64_t)t.element_size();
+  };
+  auto apart = [&](const torch::Tensor& t) {
+    return rows(t) ? t.stride(0) * (int64_t)t.element_size() : 0;
+  };
+  auto end = [&](const torch::Tensor& t) {
+    return (uintptr_t)t.data_ptr() +
+           (rows(t) ? (t.size(0) - 1) * apart(t) : 0) + width(t);
+  };
+  const auto pa = (uintptr_t)a.data_ptr(), pb = (uintptr_t)b.data_ptr();
+  if (pa >= end(b) || pb >= end(a)) return false;
+  const int64_t step = apart(a);
+  if (step == 0 || step != apart(b)) return true;
+  const int64_t d = ((int64_t)(pb - pa) % step + step) % step;
+  return d < width(a) || step - d < width(b);
+}
+
+bool same_place(const torch::Tensor& a, const torch::Tensor& b) {
+  return a.data_ptr() == b.data_ptr() && a.scalar_type() == b.scalar_type() &&
+         a.sizes() == b.sizes() &&
+         (a.size(0) <= 1 || a.stride(0) == b.stride(0));
+}
+
+// what is written first, then what it may not lie over
+void check_apart(c10::ArrayRef<std::pair<const torch::Tensor*, const char*>>
+                     tensors) {
+  for (auto& [t, name] : tensors.slice(1))
+    TORCH_CHECK(!overlap(*tensors[0].first, *t), tensors[0].second,
+                " must not overlap ", name);
+}
+
 // all of them on one GPU, which the launches then go to
 void check_devices(c10::ArrayRef<std::pair<const torch::Tensor*, const char*>>
                        tensors) {
@@ -390,6 +429,8 @@ void quant_fp8(torch::Tensor X, torch::Tensor Q, torch::Tensor S,
     check_whole(S, torch::kFloat32, {Kb, M}, "S");
   else
     check_whole(S, torch::kFloat32, {blocks128(M), Kb}, "S");
+  check_apart({{&Q, "Q"}, {&X, "X"}});
+  check_apart({{&S, "S"}, {&X, "X"}, {&Q, "Q"}});
   check_devices({{&X, "X"}, {&Q, "Q"}, {&S, "S"}});
   if (M == 0) return;
   const c10::DeviceGuard guard(X.device());
@@ -439,6 +480,10 @@ void gemm_fp8(torch::Tensor A, torch::Tensor SA, torch::Tensor B,
     check_rows(*residual, "residual");
     all.push_back({&*residual, "residual"});
   }
+  check_apart({{&C, "C"}, {&A, "A"}, {&SA, "SA"}, {&B, "B"}, {&SB, "SB"}});
+  if (bias) check_apart({{&C, "C"}, {&*bias, "bias"}});
+  if (residual && !same_place(C, *residual))
+    check_apart({{&C, "C"}, {&*residual, "residual"}});
   check_devices(all);
   if (M == 0) return;
   const c10::DeviceGuard guard(A.device());
@@ -474,6 +519,7 @@ void moe_logits(torch::Tensor X, torch::Tensor W, torch::Tensor logits) {
   check_whole(W, torch::kBFloat16, {3, E, (D + 63) / 64 * 64}, "W");
   check_aligned(W, "W");
   check_whole(logits, torch::kFloat32, {T, E}, "logits");
+  check_apart({{&logits, "logits"}, {&X, "X"}, {&W, "W"}});
   check_devices({{&X, "X"}, {&W, "W"}, {&logits, "logits"}});
   if (T == 0) return;
   const c10::DeviceGuard guard(X.device());
@@ -516,7 +562,11 @@ void moe_route(torch::Tensor logits, c10::optional<torch::Tensor> bias,
   if (bias) {
     check_whole(*bias, torch::kFloat32, {E}, "bias");
     all.push_back({&*bias, "bias"});
+    check_apart({{&ids, "ids"}, {&*bias, "bias"}});
+    check_apart({{&weights, "weights"}, {&*bias, "bias"}});
   }
+  check_apart({{&ids, "ids"}, {&logits, "logits"}});
+  check_apart({{&weights, "weights"}, {&logits, "logits"}, {&ids, "ids"}});
   check_devices(all);
   if (T == 0) return;
   const c10::DeviceGuard guard(logits.device());
@@ -588,6 +638,10 @@ void moe_mlp(const torch::Tensor& X, const torch::Tensor& ids,
     check_rows(*residual, "residual");
     all.push_back({&*residual, "residual"});
   }
+  for (auto& [t, name] : all)
+    if (t != &Y && !((t == &X || (residual && t == &*residual)) &&
+                     same_place(Y, *t)))
+      check_apart({{&Y, "Y"}, {t, name}});
   check_devices(all);
   if (T == 0) return;
   const c10::DeviceGuard guard(X.device());

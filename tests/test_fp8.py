@@ -598,3 +598,48 @@ def test_gemm_scales_far_from_one(E, m, n, k, dtype):
                 * sb[0, 0].double().item())
         off = (c.double() * 2.0 ** (-2 * e) / want - 1).abs().max().item()
         assert off <= eps, (e, off, eps)
+
+
+# ------------------------------------------------ outputs over inputs
+
+
+def rows_of(buffer, offset, m, n, apart=None, dtype=torch.bfloat16):
+    """m rows of n values within a buffer of bytes"""
+    size = torch.empty(0, dtype=dtype).element_size()
+    b = buffer[offset:]
+    return b[:len(b) // size * size].view(dtype).as_strided(
+        (m, n), (apart or n, 1))
+
+
+def test_gemm_refuses_overlaps(E):
+    b = torch.zeros(1 << 16, dtype=torch.uint8)
+    c = rows_of(b, 1024, 4, 5, 64)
+    same = rows_of(b, 1024, 4, 5, 64)
+    beside = rows_of(b, 1024 + 10, 4, 5, 64)  # the columns behind C's
+    for res in (rows_of(b, 1024 + 8, 4, 5, 64), rows_of(b, 1024 - 8, 4, 5, 64),
+                rows_of(b, 1024 + 128, 4, 5, 64), rows_of(b, 1024, 4, 5, 63),
+                rows_of(b, 1030, 4, 5)):
+        with pytest.raises(RuntimeError, match="C must not overlap residual"):
+            E.gemm_fp8(**_gemm_args(C=c, residual=res))
+    for res in (same, beside, rows_of(b, 1024 + 3 * 128 + 10, 4, 5, 64)):
+        with pytest.raises(RuntimeError, match="A must be on GPU"):
+            E.gemm_fp8(**_gemm_args(C=c, residual=res))
+    for name, t in (("A", rows_of(b, 1024, 4, 128, dtype=E4M3)),
+                    ("SA", rows_of(b, 1024, 1, 4, dtype=torch.float32)),
+                    ("B", rows_of(b, 1408, 5, 128, dtype=E4M3)),
+                    ("SB", rows_of(b, 1024, 1, 1, dtype=torch.float32)),
+                    ("bias", rows_of(b, 1024, 1, 5, dtype=torch.float32)[0])):
+        with pytest.raises(RuntimeError, match=f"C must not overlap {name}$"):
+            E.gemm_fp8(**_gemm_args(C=c, **{name: t}))
+
+
+def test_quant_refuses_overlaps(E):
+    b = torch.zeros(1 << 16, dtype=torch.uint8)
+    x = rows_of(b, 1024, 4, 130)
+    for q, s, word in ((1024, 30000, "Q must not overlap X"),
+                       (1600, 30000, "Q must not overlap X"),
+                       (30000 // 16 * 16, 1024, "S must not overlap X"),
+                       (8192, 8192 + 512, "S must not overlap Q")):
+        with pytest.raises(RuntimeError, match=word):
+            E.quant_fp8(x, rows_of(b, q, 4, 256, dtype=E4M3),
+                        rows_of(b, s, 2, 4, dtype=torch.float32))

@@ -12,7 +12,8 @@ import math
 import pytest
 import torch
 
-from test_fp8 import act_ref, far_rows, quant_ref, up128, values64
+from test_fp8 import (act_ref, far_rows, quant_ref, rows_of, up128,
+                      values64)
 
 E4M3 = torch.float8_e4m3fn
 
@@ -897,3 +898,52 @@ def test_route_large_scale(E):
     x = torch.tensor([[-60.0, -61, -62], [-55, -58, -50], [0, 1, 2]]).cuda()
     for scale in (1e35, 1e38, -1e36):
         check_route(E, x, None, 2, 1, renorm=True, scale=scale)
+
+
+# ------------------------------------------------ outputs over inputs
+
+
+def test_logits_and_route_refuse_overlaps(E):
+    b = torch.zeros(1 << 16, dtype=torch.uint8)
+    f32, i32 = torch.float32, torch.int32
+    x, w = rows_of(b, 0, 3, 100), rows_of(b, 4096, 24, 128).view(3, 8, 128)
+    for at, name in ((8, "X"), (4096 + 6000, "W")):
+        with pytest.raises(RuntimeError,
+                           match=f"logits must not overlap {name}"):
+            E.moe_logits(x, w, rows_of(b, at, 3, 8, dtype=f32))
+    x, bias = rows_of(b, 0, 3, 8, dtype=f32), rows_of(b, 512, 1, 8,
+                                                      dtype=f32)[0]
+    for ids, w, word in ((4, 2048, "ids must not overlap logits"),
+                         (520, 2048, "ids must not overlap bias"),
+                         (2048, 4, "weights must not overlap logits"),
+                         (2048, 520, "weights must not overlap bias"),
+                         (2048, 2056, "weights must not overlap ids")):
+        with pytest.raises(RuntimeError, match=word):
+            E.moe_route(x, bias, rows_of(b, ids, 3, 2, dtype=i32),
+                        rows_of(b, w, 3, 2, dtype=f32))
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_mlp_refuses_overlaps(E, fp8):
+    call = E.moe_mlp_fp8 if fp8 else E.moe_mlp_bf16
+    b = torch.zeros(1 << 16, dtype=torch.uint8)
+    y = rows_of(b, 1024, 3, 100)
+    other = rows_of(b, 1026, 3, 100)
+    for name in ("X", "residual"):
+        a = _mlp_args(fp8)
+        a.update({"Y": y, name: other})
+        with pytest.raises(RuntimeError, match=f"Y must not overlap {name}"):
+            call(**a)
+        a[name] = rows_of(b, 1024, 3, 100)  # Y itself
+        with pytest.raises(RuntimeError, match="must be on GPU"):
+            call(**a)
+    for name in ("ids", "weights", "W1", "W2", "b1", "b2") + (
+            ("S1", "S2") if fp8 else ()):
+        a = _mlp_args(fp8)
+        t = a[name]
+        big = torch.zeros(t.numel() * t.element_size() + 600,
+                          dtype=torch.uint8)
+        a[name] = big[:-600].view(t.dtype).view(t.shape)
+        a["Y"] = rows_of(big[t.numel() * t.element_size() - 4:], 0, 3, 100)
+        with pytest.raises(RuntimeError, match=f"Y must not overlap {name}$"):
+            call(**a)
