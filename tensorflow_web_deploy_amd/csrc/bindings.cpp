@@ -6,6 +6,8 @@
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime.h>
 
+#include <cmath>
+
 #include "kernels.h"
 
 namespace {
@@ -550,6 +552,8 @@ void moe_route(torch::Tensor logits, c10::optional<torch::Tensor> bias,
   TORCH_CHECK(kept >= 1 && kept <= groups, "kept must be 1 to groups, got ",
               kept);
   TORCH_CHECK(best == 1 || best == 2, "best must be 1 or 2, got ", best);
+  TORCH_CHECK(std::isfinite((float)scale), "scale must be finite in f32, got ",
+              scale);
   TORCH_CHECK(ids.dim() == 2, "ids must be 2D");
   const int64_t k = ids.size(1);
   TORCH_CHECK(k >= 1 && k <= 64 && k <= kept * (E / groups),

@@ -947,3 +947,12 @@ def test_mlp_refuses_overlaps(E, fp8):
         a["Y"] = rows_of(big[t.numel() * t.element_size() - 4:], 0, 3, 100)
         with pytest.raises(RuntimeError, match=f"Y must not overlap {name}$"):
             call(**a)
+
+
+@pytest.mark.parametrize("scale", [math.inf, -math.inf, math.nan, 1e39])
+def test_route_refuses_an_infinite_scale(E, scale):
+    """It would make NaN of the 0 that a place without an expert has."""
+    with pytest.raises(RuntimeError, match="scale must be finite"):
+        E.moe_route(torch.zeros(3, 8), None,
+                    torch.zeros(3, 2, dtype=torch.int32), torch.zeros(3, 2),
+                    scale=scale)
