@@ -421,3 +421,18 @@ def test_route_experts_decides_in_64_bits(score, dtype):
         assert w.dtype == dtype and torch.equal(ids.int(), want[0])
         off = (w.double() - want[1]).abs()
         assert (off <= torch.finfo(dtype).eps * want[1]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp8"])
+def test_f32_logits_in_graphs_and_padded_batches(dtype):
+    g = graph(dict(experts=20, k=3, logits="f32"))
+    x = images(8)
+    eng = engine(g, dtype=dtype)
+    first = eng.infer(x)
+    eng.infer(images(8, 1))
+    for _ in range(3):
+        assert np.array_equal(eng.infer(x), first)
+    assert np.array_equal(eng.infer(x[:5]), first[:5])  # 5 rows run as 8
+    eager = engine(g, dtype=dtype, use_hip_graphs=False)
+    assert np.array_equal(eager.infer(x), first)

@@ -956,3 +956,20 @@ def test_route_refuses_an_infinite_scale(E, scale):
         E.moe_route(torch.zeros(3, 8), None,
                     torch.zeros(3, 2, dtype=torch.int32), torch.zeros(3, 2),
                     scale=scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("t", [3, 60, 1500, 2 ** 16 + 70])
+def test_mlp_into_its_input(E, fp8, t):
+    """X as the output, and as the residual too, in every way and pass."""
+    layer = Layer(E, fp8, 6, 64, 72)
+    g = torch.Generator().manual_seed(t)
+    x = torch.randn(t, 64, generator=g).to(torch.bfloat16).cuda()
+    ids = torch.randint(-1, 6, (t, 2), generator=g, dtype=torch.int32).cuda()
+    w = torch.rand(t, 2, generator=g).cuda()
+    for residual in (False, True):
+        want = layer(x, ids, w, x if residual else None, 5)
+        y = x.clone()
+        layer(y, ids, w, y if residual else None, 5, y)
+        assert torch.equal(y, want)
