@@ -696,7 +696,10 @@ void moe_mlp(const torch::Tensor& X, const torch::Tensor& ids,
 // Y[t] = residual[t] + sum_j weights[t,j] (act(X[t] @ W1[e]^T + b1[e])
 //        @ W2[e]^T + b2[e]),  e = ids[t,j]; an id outside of 0..E-1 adds
 // nothing. X, Y, residual bf16 [T,D]; W1 [E,H,D up to 64s], W2
-// [E,D,H up to 64s] bf16, filled up with zeros
+// [E,D,H up to 64s] bf16, filled up with zeros. The activated rows are rounded
+// to bf16, which the second product takes; where assignments are more than 16
+// to 32, the weighted terms to f16 over a power of two for each 64 columns. All
+// sums are f32.
 void moe_mlp_bf16(torch::Tensor X, torch::Tensor ids, torch::Tensor weights,
                   torch::Tensor W1, c10::optional<torch::Tensor> b1,
                   torch::Tensor W2, c10::optional<torch::Tensor> b2,
@@ -706,8 +709,8 @@ void moe_mlp_bf16(torch::Tensor X, torch::Tensor ids, torch::Tensor weights,
 }
 
 // the same on e4m3 weights, each expert's as quant_fp8 leaves them with
-// block_rows 128. X and the hidden rows are rounded to e4m3 with a scale for
-// each 128 values.
+// block_rows 128. X and the activated rows are rounded to e4m3 with a scale for
+// each 128 values, the terms as above.
 void moe_mlp_fp8(torch::Tensor X, torch::Tensor ids, torch::Tensor weights,
                  torch::Tensor W1, torch::Tensor S1,
                  c10::optional<torch::Tensor> b1, torch::Tensor W2,

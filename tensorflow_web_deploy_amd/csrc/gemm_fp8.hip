@@ -25,14 +25,15 @@ using namespace tile;
 
 // ------------------------------------------------------------ quant_fp8
 
-// 12544 x 768 bf16: 7.1 us, 4.1 TB/s; 1 x 768: 2.4 us
+// 12544 x 768 bf16: 7.1 to 7.6 us a call, 4 TB/s; 1 x 768: 2.7 us
 template <typename T>
 __global__ __launch_bounds__(256) void quant_rows_kernel(QuantRows<T> q) {
   q.run(blockIdx.x);
 }
 
 // One workgroup a block of 128 x 128, which it holds in registers between its
-// scale and its values, so that the weight is read once.
+// scale and its values, so that the weight is read once: 4096 x 25088 f32 93 us,
+// 5.5 TB/s; 1536 x 768 4.5.
 template <typename T>
 __global__ __launch_bounds__(256) void quant_tiles_kernel(
     const T* __restrict__ X, int64_t ldx, int64_t M, int K,
@@ -188,10 +189,11 @@ __device__ __forceinline__ DenseTile dense_tile(
 
 // The activation and the residual are the kernel's own, so that its way out
 // holds no choice. Bound by the matrix unit and the VALU, which scales each
-// block: 16200 x 4096 x 8192 with GELU in 256 x 256 tiles 501 us in a clock
-// that isn't lowered yet, 550 later (2.17 and 1.97 PFLOP/s; a library's product
-// with one scale 2.85), of a tile's 63 us 54 in its 32 steps. 12544 x 768 x 768
-// with a residual in 160 x 128 tiles 16.5 us, 3 TB/s.
+// block: 16200 x 4096 x 8192 with GELU in 256 x 256 tiles 545 to 575 us as the
+// card's clock goes (1.9 to 2 PFLOP/s; a library's product with one scale 2.85),
+// the matrix unit busy for 48% of the cycles, the VALU for 53%; of a tile's 63
+// us 54 are its 32 steps. 12544 x 768 x 768 with a residual in 160 x 128 tiles
+// 17.2 to 18.8 us, 3 TB/s.
 template <class S, int KIND, bool RES>
 __global__ __launch_bounds__(S::THREADS, 2) void gemm_fp8_kernel(Dense d) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -258,7 +260,7 @@ __global__ __launch_bounds__(S::THREADS, 2) void gemm_fp8_f32_kernel(Dense d) {
 }
 
 // Split K: the f32 sums of slice blockIdx.y. 64 x 25088 x 4096 in 8 slices:
-// 20 us, 5.1 TB/s.
+// 20 to 21 us, 5 TB/s.
 template <class S, bool EXACT>
 __global__ __launch_bounds__(S::THREADS, 2) void gemm_fp8_slice_kernel(
     Dense d) {
@@ -286,7 +288,7 @@ __global__ __launch_bounds__(S::THREADS, 2) void gemm_fp8_slice_kernel(
 
 // Up to 16 RT rows: 16 columns a workgroup, K cut into 8 parts, a wave each;
 // wave i finishes row tile i. Bound by the time the weights take to come:
-// 1 x 768 x 1000 3.1 us, 1 x 25088 x 4096 17.8 (5.8 TB/s). With 4 waves that
+// 1 x 768 x 1000 3.0 us, 1 x 25088 x 4096 17.8 (5.8 TB/s). With 4 waves that
 // takes 25.4 us, with 16 18.8.
 template <int RT, class T>
 __global__ __launch_bounds__(512, 4) void gemm_fp8_few_kernel(Dense d) {
@@ -425,8 +427,8 @@ struct Plan {
 // lie alone on a CU, of the others two share one where there are more than
 // CUs. Cutting K fills the chip where tiles are few; the slices' f32 planes go
 // out and come back at 4 TB/s, and adding them up is a launch more, 4 us.
-// Measured (tiles of 64 / 128 / 160 / 256 rows, the first two with the best
-// number of slices): 64 x 25088 x 4096: 26.2 / 28.4, without slices 97 / 126;
+// Measured (without residual and activation in a clock not lowered yet, tiles of
+// 64 / 128 / 160 / 256 rows, the first two with the best number of slices): 64 x 25088 x 4096: 26.2 / 28.4, without slices 97 / 126;
 // 512 x 4096 x 4096: 20.1 / 24.6 / 28.3 / 52.7; 2048^3: 14.9 / 15.9 / 19.6 /
 // 31.1; 12544 x 768 x 768: 19.2 / 17.4 / 15.1 / 18.2; 16200 x 4096 x 8192:
 // 695 / 545 / 532 / 507. For f32, 64 / 128 rows: 64 x 25088 x 4096: 28.9 /

@@ -348,8 +348,8 @@ __device__ __forceinline__ int expert_at(int l, int v) {
 // f32, is then done again in 64 bits, so that the choice is that of the scores
 // in 64 bits, the lower index first among equals. That is one row in some
 // hundreds, unless logits repeat a lot. 12544 rows of 256 f32, 8 out of 4 of 8
-// groups: 15 us, of which the rows in 64 bits take 2.5 at the end; bound by the
-// VALU, some 1500 instructions for 4 rows.
+// groups: 14.2 to 15.9 us, of which the rows in 64 bits take 2.5 at the end; bound
+// by the VALU, busy for 63% of the cycles with 1250 instructions for 4 rows.
 template <typename T, int V>
 __global__ __launch_bounds__(256) void route_kernel(Route p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -1004,9 +1004,10 @@ __device__ __forceinline__ void finish_experts(
 // is weighted and goes to its assignment's place, in 16 bits over a power of
 // two. What a tile shares with its neighbours, rows of x or of the weights,
 // comes from its XCD's L2. 25088 assignments of 32 experts, 768 x 1536, bf16,
-// GELU: 81 us and 61 (0.57 and 0.76 PFLOP/s), half of it in the 12 and 24
-// steps, which run at 1.3 PFLOP/s, half in front of them and behind. 65536 of
-// 64 experts, 2048 x 1024, e4m3: 213 and 242 us (1.29 and 1.14).
+// GELU: 80 to 95 us and 61 to 70 as the card's clock goes (0.57 and 0.76 PFLOP/s
+// at best), half of it in the 12 and 24 steps, which run at 1.3 PFLOP/s, half in
+// front of them and behind. 65536 of 64 experts, 2048 x 1024, e4m3: 215 to 230
+// and 246 to 260 us (1.28 and 1.12 at best).
 template <class S, bool FIRST, int KIND>
 __global__ __launch_bounds__(S::THREADS, 2) void experts_kernel(Experts p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -1166,7 +1167,7 @@ __global__ __launch_bounds__(512, 4) void experts_hidden_kernel(Experts p) {
 // Without a plan, the second product and the sum over a token's experts: 16
 // columns of a token a workgroup, its waves share the experts and, if there
 // are fewer than 8, K. The 16 rows are all the same one. Bound as above: 1 row
-// of 2 experts, 1536 x 768 in bf16, 5.4 us, 0.7 more with K in one piece.
+// of 2 experts, 1536 x 768 in bf16, 6.0 us, 0.7 more with K in one piece.
 template <bool FP8>
 __global__ __launch_bounds__(512, 4) void experts_sum_kernel(
     Experts p, const __bf16* residual, int64_t ldr, __bf16* Y, int64_t ldy) {
@@ -1211,7 +1212,7 @@ __global__ __launch_bounds__(512, 4) void experts_sum_kernel(
 
 // Each token adds up its experts' rows, in the order of its list: 8 columns a
 // thread. Bound by HBM: 8192 rows of 8 x 2048 57 us, 5.3 TB/s. Where Y and the
-// residual allow 16 bytes at a time, 12544 x 768 takes 12 us, else 16.
+// residual allow 16 bytes at a time, 12544 x 768 takes 12 to 13 us, else 16.
 __global__ __launch_bounds__(256) void combine_kernel(
     const _Float16* __restrict__ P, const float* __restrict__ SP,
     const int* __restrict__ ids, int E, int k, int D, int Dp,
