@@ -32,8 +32,8 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(QuantRows<T> q) {
 }
 
 // One workgroup a block of 128 x 128, which it holds in registers between its
-// scale and its values, so that the weight is read once: 4096 x 25088 f32 93 us,
-// 5.5 TB/s; 1536 x 768 4.5.
+// scale and its values, so that the weight is read once: 4096 x 25088 f32 93
+// us, 5.5 TB/s; 1536 x 768 4.5.
 template <typename T>
 __global__ __launch_bounds__(256) void quant_tiles_kernel(
     const T* __restrict__ X, int64_t ldx, int64_t M, int K,
@@ -190,10 +190,10 @@ __device__ __forceinline__ DenseTile dense_tile(
 // The activation and the residual are the kernel's own, so that its way out
 // holds no choice. Bound by the matrix unit and the VALU, which scales each
 // block: 16200 x 4096 x 8192 with GELU in 256 x 256 tiles 545 to 575 us as the
-// card's clock goes (1.9 to 2 PFLOP/s; a library's product with one scale 2.85),
-// the matrix unit busy for 48% of the cycles, the VALU for 53%; of a tile's 63
-// us 54 are its 32 steps. 12544 x 768 x 768 with a residual in 160 x 128 tiles
-// 17.2 to 18.8 us, 3 TB/s.
+// card's clock goes (1.9 to 2 PFLOP/s; a library's product with one scale
+// 2.85), the matrix unit busy for 48% of the cycles, the VALU for 53%; of a
+// tile's 63 us 54 are its 32 steps. 12544 x 768 x 768 with a residual in 160 x
+// 128 tiles 17.2 to 18.8 us, 3 TB/s.
 template <class S, int KIND, bool RES>
 __global__ __launch_bounds__(S::THREADS, 2) void gemm_fp8_kernel(Dense d) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -233,10 +233,10 @@ __device__ __forceinline__ void finish4(const Dense& d, int64_t m, int n,
     finish<CLAMP, true, false, T>(d, m, n, v, x.b, x.res);
 }
 
-// The same for f32 results, 4 columns a lane: its steps take 1.6 to 1.8 times as
-// long, bound by the f16 instruction and the conversions for it, and what is
-// added and the activation are looked at as it runs. 16200 x 4096 x 8192 1001
-// us, 1.09 PFLOP/s; 12544 x 768 x 768 28, with a residual and GELU 38.
+// The same for f32 results, 4 columns a lane: its steps take 1.6 to 1.8 times
+// as long, bound by the f16 instruction and the conversions for it, and what
+// is added and the activation are looked at as it runs. 16200 x 4096 x 8192
+// 1001 us, 1.09 PFLOP/s; 12544 x 768 x 768 28, with a residual and GELU 38.
 template <class S>
 __global__ __launch_bounds__(S::THREADS, 2) void gemm_fp8_f32_kernel(Dense d) {
   static_assert(S::W == 4);
@@ -427,13 +427,13 @@ struct Plan {
 // lie alone on a CU, of the others two share one where there are more than
 // CUs. Cutting K fills the chip where tiles are few; the slices' f32 planes go
 // out and come back at 4 TB/s, and adding them up is a launch more, 4 us.
-// Measured (without residual and activation in a clock not lowered yet, tiles of
-// 64 / 128 / 160 / 256 rows, the first two with the best number of slices): 64 x 25088 x 4096: 26.2 / 28.4, without slices 97 / 126;
-// 512 x 4096 x 4096: 20.1 / 24.6 / 28.3 / 52.7; 2048^3: 14.9 / 15.9 / 19.6 /
-// 31.1; 12544 x 768 x 768: 19.2 / 17.4 / 15.1 / 18.2; 16200 x 4096 x 8192:
-// 695 / 545 / 532 / 507. For f32, 64 / 128 rows: 64 x 25088 x 4096: 28.9 /
-// 36.4, 512 x 4096 x 4096: 28.4 / 31.4, 2048^3: 25.3 / 27.5, 16200 x 4096 x
-// 8192: 1168 / 1009.
+// Measured (without residual and activation in a clock not lowered yet, tiles
+// of 64 / 128 / 160 / 256 rows, the first two with the best number of slices):
+// 64 x 25088 x 4096: 26.2 / 28.4, without slices 97 / 126; 512 x 4096 x 4096:
+// 20.1 / 24.6 / 28.3 / 52.7; 2048^3: 14.9 / 15.9 / 19.6 / 31.1; 12544 x 768 x
+// 768: 19.2 / 17.4 / 15.1 / 18.2; 16200 x 4096 x 8192: 695 / 545 / 532 / 507.
+// For f32, 64 / 128 rows: 64 x 25088 x 4096: 28.9 / 36.4, 512 x 4096 x 4096:
+// 28.4 / 31.4, 2048^3: 25.3 / 27.5, 16200 x 4096 x 8192: 1168 / 1009.
 Plan plan(int M, int N, int Kp, bool f32) {
   const int all = Kp / STEP;
   // Few rows, in us as such and as the best tiles: 1 x 4096 x 4096 5.3 / 9.5,

@@ -342,14 +342,15 @@ __device__ __forceinline__ int expert_at(int l, int v) {
 }
 
 // 16 lanes a row, 4 rows a wave: the steps across lanes stay within rows of
-// the register file, and one instruction serves 4 rows (a wave a row took 47 us
-// where this takes 15). Everything is decided in f32; a row where rounding
+// the register file, and one instruction serves 4 rows (a wave a row took 47
+// us where this takes 15). Everything is decided in f32; a row where rounding
 // could change what is chosen or its order, or whose scores leave the range of
 // f32, is then done again in 64 bits, so that the choice is that of the scores
 // in 64 bits, the lower index first among equals. That is one row in some
 // hundreds, unless logits repeat a lot. 12544 rows of 256 f32, 8 out of 4 of 8
-// groups: 14.2 to 15.9 us, of which the rows in 64 bits take 2.5 at the end; bound
-// by the VALU, busy for 63% of the cycles with 1250 instructions for 4 rows.
+// groups: 14.2 to 15.9 us, of which the rows in 64 bits take 2.5 at the end;
+// bound by the VALU, busy for 63% of the cycles with 1250 instructions for 4
+// rows.
 template <typename T, int V>
 __global__ __launch_bounds__(256) void route_kernel(Route p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -1000,12 +1001,12 @@ __device__ __forceinline__ void finish_experts(
 
 // The rows of one tile, all of one expert, times its weights. FIRST: rows are
 // gathered by token, the result is activated, rounded to the layer's type and
-// kept in the order of the experts. Otherwise: rows as they lie, the result
-// is weighted and goes to its assignment's place, in 16 bits over a power of
-// two. What a tile shares with its neighbours, rows of x or of the weights,
-// comes from its XCD's L2. 25088 assignments of 32 experts, 768 x 1536, bf16,
-// GELU: 80 to 95 us and 61 to 70 as the card's clock goes (0.57 and 0.76 PFLOP/s
-// at best), half of it in the 12 and 24 steps, which run at 1.3 PFLOP/s, half in
+// kept in the order of the experts. Otherwise: rows as they lie, the result is
+// weighted and goes to its assignment's place, in 16 bits over a power of two.
+// What a tile shares with its neighbours, rows of x or of the weights, comes
+// from its XCD's L2. 25088 assignments of 32 experts, 768 x 1536, bf16, GELU:
+// 80 to 95 us and 61 to 70 as the card's clock goes (0.57 and 0.76 PFLOP/s at
+// best), half of it in the 12 and 24 steps, which run at 1.3 PFLOP/s, half in
 // front of them and behind. 65536 of 64 experts, 2048 x 1024, e4m3: 215 to 230
 // and 246 to 260 us (1.28 and 1.12 at best).
 template <class S, bool FIRST, int KIND>

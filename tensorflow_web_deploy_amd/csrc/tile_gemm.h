@@ -234,8 +234,8 @@ __device__ __forceinline__ int column_of(int wn, int t, int i16) {
 
 // Blocks are scaled by the product of their two scales, which may leave the
 // range of f32 where the scaled block doesn't: by an infinite one a block of 0
-// becomes NaN, a subnormal one has lost bits. Both are factors above 1, or below,
-// then, and one after the other they lose nothing.
+// becomes NaN, a subnormal one has lost bits. Both are factors above 1, or
+// below, then, and one after the other they lose nothing.
 struct Factors {
   float most = 0.f, least = 1.f;
 
@@ -408,13 +408,13 @@ __device__ __forceinline__ bool product(char* smem, __amdgpu_buffer_rsrc_t ra,
 }
 
 // The sums that a product with an odd factor has left, again and carefully, if
-// it shows in them: some aren't finite, or lie between 2^-126 and 2^-103, where
-// blocks with a subnormal factor end up (2^25 of 2^-126 and of 2^-149). Each
-// wave for itself, from memory to registers, with the rows that row_a, row_b
-// and row_s (a scale's offset) give. The largest and the least of the factors
-// cost the steps 0 to 1%; a class test of each and an OR 2% (16200 x 4096 x 8192
-// 540 / 544 / 552 us), a test of each sum behind the steps up to 9% (12544 x 768
-// x 2304 32.6 / 35.6).
+// it shows in them: some aren't finite, or lie between 2^-126 and 2^-103,
+// where blocks with a subnormal factor end up (2^25 of 2^-126 and of 2^-149).
+// Each wave for itself, from memory to registers, with the rows that row_a,
+// row_b and row_s (a scale's offset) give. The largest and the least of the
+// factors cost the steps 0 to 1%; a class test of each and an OR 2% (16200 x
+// 4096 x 8192 540 / 544 / 552 us), a test of each sum behind the steps up to
+// 9% (12544 x 768 x 2304 32.6 / 35.6).
 template <class S, bool EXACT, class A, class B, class C>
 __device__ __forceinline__ void mend_sums(
     __amdgpu_buffer_rsrc_t ra, __amdgpu_buffer_rsrc_t rb,
