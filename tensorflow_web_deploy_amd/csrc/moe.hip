@@ -164,6 +164,14 @@ __device__ __forceinline__ float sum16(float v) {
   return v + turned<1>(v);
 }
 
+// Between what lanes of a wave write to LDS and what others read of it: the
+// hardware keeps the order, the compiler has to be told to.
+__device__ __forceinline__ void wave_turn() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // what the lanes before this one of its 16 add up to
 template <int SHR>
 __device__ __forceinline__ int shifted(int v) {
@@ -269,7 +277,7 @@ __device__ __forceinline__ void route_exactly(const Route& p, int64_t t,
 #pragma unroll
     for (int v = 0; v < V; ++v)
       if (v * 64 + lane < p.E) lds[v * 64 + lane] = key[v];
-    __builtin_amdgcn_wave_barrier();
+    wave_turn();
     double first = NONE, second = NONE;
     if (lane < p.groups) {
 #pragma unroll 4
@@ -439,7 +447,7 @@ __global__ __launch_bounds__(256) void route_kernel(Route p) {
   if (p.groups > 1) {
     const int size = p.E / p.groups;
     to_lds(at.key, key);
-    __builtin_amdgcn_wave_barrier();
+    wave_turn();
     // no group's sum is off by more than two of the largest score could be
     const float err = 2 * error_of(most, 0.f, p.sigmoid);
 #pragma unroll
@@ -474,7 +482,7 @@ __global__ __launch_bounds__(256) void route_kernel(Route p) {
       lds[at.round + g] =
           fabsf(first) + (second > NONE ? fabsf(second) : 0.f);
     }
-    __builtin_amdgcn_wave_barrier();
+    wave_turn();
     float low = INFINITY, high = NONE;
     uint64_t kept = 0;
 #pragma unroll
@@ -536,13 +544,13 @@ __global__ __launch_bounds__(256) void route_kernel(Route p) {
       const int2 none = make_int2(-1, __builtin_bit_cast(int, NONE));
       list[l] = none;
       if (two) list[l + 16] = none;
-      __builtin_amdgcn_wave_barrier();
+      wave_turn();
 #pragma unroll
       for (int v = 0; v < V; ++v)
         if (key[v] >= bound && key[v] > NONE)
           list[to++] = make_int2(expert_at<V>(l, v),
                                  __builtin_bit_cast(int, key[v]));
-      __builtin_amdgcn_wave_barrier();
+      wave_turn();
       // places that hold nothing come last, each at its own
       const int2 a = list[l];
       const float ka = __builtin_bit_cast(float, a.y);
@@ -554,10 +562,10 @@ __global__ __launch_bounds__(256) void route_kernel(Route p) {
         const float ib = b.x < 0 ? 1040.f + l : (float)b.x;
         rank += rank16(ka, ia, kb, ib);
         const int other = rank16(kb, ib, kb, ib) + rank16(kb, ib, ka, ia);
-        __builtin_amdgcn_wave_barrier();
+        wave_turn();
         list[other] = b;
       }
-      __builtin_amdgcn_wave_barrier();
+      wave_turn();
       list[rank] = a;
     }
   }
@@ -579,7 +587,7 @@ __global__ __launch_bounds__(256) void route_kernel(Route p) {
     if (l == 0)
       list[j] = make_int2(top > NONE ? id : -1, __builtin_bit_cast(int, top));
   }
-  __builtin_amdgcn_wave_barrier();
+  wave_turn();
 
   // equal logits and biases tie in any precision
   auto ties = [&](int a, int b) {
@@ -648,8 +656,7 @@ __global__ __launch_bounds__(256) void route_kernel(Route p) {
   }
   if (!unsafe) return;
   // the rows of the wave are done with LDS: it now holds numbers of 64 bits
-  __builtin_amdgcn_wave_barrier();
-  asm volatile("" ::: "memory");
+  wave_turn();
   for (int r = 0; r < 4; ++r)
     if (unsafe >> (16 * r) & 0xffff)
       route_exactly<T, (V + 3) / 4>(p, t0 + r, (double*)wave_lds, lane);
